@@ -217,7 +217,7 @@ def run(state):
     case = state["case"]
     if kind == "linear":
         w = state["image"] if state["image"] is not None else state["q"].t()
-        return qf.fp8_linear(state["x"], w, state["s"], state["bias"])
+        return qf.fp8_linear(state["x"], w, state["s"], state["bias"], out_features=case["N"])
     if kind == "norm":
         return qf.block_norm_rows(state["x"], state["residual"], state["post"], state["pre"], gate=state["gate"],
                                   gate_act=case["act"], alpha=case["alpha"], eps=1e-6)
