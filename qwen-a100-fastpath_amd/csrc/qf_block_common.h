@@ -1,0 +1,128 @@
+// Device helpers shared by the kernels of libqf_block.so (gfx950).
+#ifndef QF_BLOCK_COMMON_H
+#define QF_BLOCK_COMMON_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "qf_block.h"
+
+namespace qfb {
+
+constexpr int kWave = 64;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+// bf16 <-> fp32 on 32-bit words (element order: low half first)
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ float bf16_f32(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
+// two fp32 -> two bf16 (round to nearest even), `a` in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), bf16x2_t));
+}
+__device__ __forceinline__ void unpack8(u32x4_t v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = bf16_lo(v[i]);
+    f[2 * i + 1] = bf16_hi(v[i]);
+  }
+}
+__device__ __forceinline__ u32x4_t pack8(const float (&f)[8]) {
+  u32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+
+// Lane v of a DPP permutation of x (lanes without a source give 0).
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+// Sum over groups of L lanes (8, 16, 32 or 64), the same in each lane of a group: rotations within rows of 16 lanes, then
+// the wider exchanges.  Every lane of the wavefront active.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp_f32<0xB1>(v);   // quad_perm 1 0 3 2
+  v += dpp_f32<0x4E>(v);   // quad_perm 2 3 0 1
+  v += dpp_f32<0x141>(v);  // row_half_mirror: the other quad of 8 lanes
+  if constexpr (L >= 16) v += dpp_f32<0x140>(v);  // row_mirror: the other 8 of 16 lanes
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  if constexpr (L >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
+template <int L>
+__device__ __forceinline__ float group_max(float v) {  // NaN only where every value is
+  v = fmaxf(v, dpp_f32<0xB1>(v));
+  v = fmaxf(v, dpp_f32<0x4E>(v));
+  v = fmaxf(v, dpp_f32<0x141>(v));
+  if constexpr (L >= 16) v = fmaxf(v, dpp_f32<0x140>(v));
+  if constexpr (L >= 32) v = fmaxf(v, __shfl_xor(v, 16));
+  if constexpr (L >= 64) v = fmaxf(v, __shfl_xor(v, 32));
+  return v;
+}
+
+// Inclusive scan of sums, and the maximum in lane 63, over the wavefront's 64 lanes (every lane active).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: row 0 into 1, row 2 into 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: rows 0, 1 into 2, 3
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
+}
+
+// 16 e4m3 values (a lane's bytes of a weight fragment) as two fragments of 8 bf16; exact (v_cvt_scalef32_pk_bf16_fp8).
+__device__ __forceinline__ void widen16(u32x4_t v, bf16x8_t& lo, bf16x8_t& hi) {
+  u32x4_t a, b;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.f, false));
+    a[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.f, true));
+    b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 + i], 1.f, false));
+    b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 + i], 1.f, true));
+  }
+  lo = __builtin_bit_cast(bf16x8_t, a);
+  hi = __builtin_bit_cast(bf16x8_t, b);
+}
+
+__device__ __forceinline__ u32x4_t load_once(const uint8_t* p) {  // read once: not kept in the caches
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+}
+
+// Lets `fn` have `bytes` of dynamic LDS on the current device; `raised` holds the devices where it has.
+inline bool raise_lds(const void* fn, int bytes, std::atomic<uint64_t>& raised) {
+  int dev = 0;
+  if (bytes <= 64 * 1024) return true;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (bit & raised.load(std::memory_order_relaxed)) return true;
+  if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+  raised.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+}  // namespace qfb
+
+#endif

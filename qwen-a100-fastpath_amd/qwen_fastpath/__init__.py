@@ -18,6 +18,11 @@ from .w8a16 import (  # noqa: F401
     w8a16_mm_rmsnorm,
     w8a8_mm)
 from .spec_attn import gqa_packed_spec_attention  # noqa: F401
+from .fp8 import (  # noqa: F401
+    fp8_from_tiled, fp8_linear, fp8_scale_shape, fp8_to_tiled, fp8_w8a16_mm, fp8_w8a8_mm, qf_fp8_linear,
+    quantize_tokens_fp8)
+from .moe import moe_few_tokens  # noqa: F401
+from .norm import block_norm_rows  # noqa: F401
 from .patches import (  # noqa: F401
     Int8Head,
     W8A16LinearMethod,

@@ -1,0 +1,94 @@
+"""ctypes binding of libqf_block.so, the C ABI declared in include/qf_block.h.
+
+Built in-tree by qwen-a100-fastpath_amd/csrc/Makefile next to this file.  There is no fallback implementation: if the
+library is missing, every GPU entry point raises.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+
+import torch
+
+from ._lib import QFError
+
+LIB_NAME = "libqf_block.so"
+LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
+ABI_VERSION = 1
+
+BLOCK = 128              # QF_FP8_BLOCK
+MAX_DECODE_M = 16        # QF_FP8_MAX_DECODE_M
+NORM_MAX_N = 32768       # QF_BLOCK_NORM_MAX_N
+MOE_MAX_EXPERTS = 512    # QF_MOE_MAX_EXPERTS
+MOE_MAX_TOP_K = 16       # QF_MOE_MAX_TOP_K
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
+ACTS = {"none": 0, "sigmoid": 1}
+
+# Every symbol include/qf_block.h declares.
+EXPORTS = (
+    "qf_block_abi_version",
+    "qf_fp8_w8a16_gemm",
+    "qf_quantize_tokens_fp8",
+    "qf_fp8_w8a8_workspace_bytes",
+    "qf_fp8_w8a8_linear",
+    "qf_block_norm_rows",
+    "qf_moe_few_workspace_bytes",
+    "qf_moe_few_tokens",
+)
+
+_lib: ctypes.CDLL | None = None
+
+
+def load() -> ctypes.CDLL:
+    """Load the library once.  Raises ImportError (never falls back) when it is absent."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    if not os.path.exists(LIB_PATH):
+        raise ImportError(
+            f"{LIB_PATH} is missing: build it with `make -C qwen-a100-fastpath_amd/csrc` "
+            "(or __graft_entry__.build()); its operators have no non-HIP implementation")
+    L = ctypes.CDLL(LIB_PATH)
+    p, i64, i32, sz, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
+    product = [p, i64, p, i64, i32, p, p, p, i64, i32, i32, i32, i32]
+    for name, res, args in (
+            ("qf_block_abi_version", i32, []),
+            ("qf_fp8_w8a16_gemm", i32, product + [p]),
+            ("qf_quantize_tokens_fp8", i32, [p, i64, i32, i32, p, i64, p, p]),
+            ("qf_fp8_w8a8_workspace_bytes", sz, [i32] * 3),
+            ("qf_fp8_w8a8_linear", i32, product + [p, sz, p]),
+            ("qf_block_norm_rows", i32, [p, i64, p, i64, i32, p, p, f32, p, i64, i32, i32, f32, f32, i32, i32, p, i64, p,
+                                         i64, p]),
+            ("qf_moe_few_workspace_bytes", sz, [i32] * 5),
+            ("qf_moe_few_tokens", i32, [p, i64, p, i64, i32, p, p, p, p, p, i64, i32, i32, i32, i32, i32, i32, p, sz, p])):
+        fn = getattr(L, name)
+        fn.restype, fn.argtypes = res, args
+    v = L.qf_block_abi_version()
+    if v != ABI_VERSION:
+        raise ImportError(f"{LIB_PATH}: ABI version {v}, expected {ABI_VERSION}")
+    _lib = L
+    return L
+
+
+def same_gpu(*tensors) -> torch.device:
+    """The GPU that every tensor handed to the library lives on: a host pointer, or another device's, reaching a kernel
+    faults the device."""
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise TypeError(f"expected a GPU tensor, got one on {dev}")
+    for t in tensors[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: all must be on one GPU")
+    return dev
+
+
+def call(name: str, device: torch.device, *args) -> None:
+    """Run an entry point on torch's current stream of `device` (its last argument), whatever the current device is."""
+    fn = getattr(_lib or load(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        raise QFError(rc, name)

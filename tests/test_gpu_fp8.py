@@ -1,0 +1,176 @@
+"""Block-scaled FP8 products on the GPU against 64-bit references (block_helpers) with derived bounds: both arithmetics,
+both weight layouts, odd sizes, and the calls the documentation allows."""
+import pytest
+import torch
+
+import block_helpers as H
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def qf():
+    import qwen_fastpath
+    return qwen_fastpath
+
+
+def _weight_on(qf, q, tiled):
+    return qf.fp8_to_tiled(q.cuda().t()) if tiled else q.cuda().t()
+
+
+def _check(qf, M, N, K, tiled, bias, out, a8, seed=0):
+    g = H.gen(seed)
+    q, s = H.weight(g, N, K)
+    x = H.rows(g, M, K)
+    b = torch.randn(N, generator=g).to(BF16) if bias else None
+    mm = qf.fp8_w8a8_mm if a8 else qf.fp8_w8a16_mm
+    y = mm(x.cuda(), _weight_on(qf, q, tiled), s.cuda(), out, None if b is None else b.cuda(), out_features=N)
+    torch.cuda.synchronize()
+    assert y.dtype == out
+    ref, bound = H.product(x, q, s, b, a8)
+    H.within(y, ref, bound, H.BF16 if out == BF16 else H.F32)
+    return y
+
+
+@pytest.mark.parametrize("N,K", [(64, 128), (7, 64), (1, 192), (2500, 1088), (130, 640)])
+def test_tiled_image(qf, N, K):
+    q, _ = H.weight(H.gen(N), N, K)
+    image = qf.fp8_to_tiled(q.cuda().t())
+    assert torch.equal(image.cpu().view(torch.uint8), H.tiles(q).view(torch.uint8))
+    assert torch.equal(qf.fp8_from_tiled(image, N, K).cpu().view(torch.uint8), q.t().view(torch.uint8))
+
+
+@pytest.mark.parametrize("tiled", [True, False])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 64), (1, 128, 128), (3, 1, 64), (16, 17, 192), (5, 300, 1088), (16, 2500, 2112),
+                                   (2, 129, 8192), (9, 640, 17408), (7, 16640, 256), (16, 33000, 320)])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_decode(qf, M, N, K, tiled, out):
+    _check(qf, M, N, K, tiled, M % 2 == 1, out, False, seed=M + N)
+
+
+@pytest.mark.parametrize("M", range(1, 17))
+def test_decode_every_width(qf, M):
+    _check(qf, M, 272, 640, M % 2 == 0, False, BF16, False, seed=M)
+
+
+@pytest.mark.parametrize("M,K", [(1, 64), (3, 192), (16, 128), (17, 1088), (333, 5120), (2, 17408)])
+def test_quantiser_bits(qf, M, K):
+    x = H.rows(H.gen(M), M, K)
+    x[0, :64] = 0
+    x[M - 1, K - 64:] = 0
+    x[M // 2, 0] = 3e38
+    q, s = qf.quantize_tokens_fp8(x.cuda())
+    qr, sr = H.quantize(x)
+    assert torch.equal(s.cpu(), sr)
+    assert torch.equal(q.cpu().view(torch.uint8) , qr.view(torch.uint8))
+
+
+def test_quantiser_tiny_and_not_finite(qf):
+    x = torch.zeros(4, 256)
+    x[0, :8] = torch.tensor([1, -2, 3, -4, 5, 100, 333, 127.]) * 2.0 ** -133  # subnormal in bf16
+    x[1, 5] = float("inf")
+    x[2, 200] = float("nan")
+    x[3, 7] = 2.0 ** -126
+    x = x.to(BF16)
+    q, s = qf.quantize_tokens_fp8(x.cuda())
+    qr, sr = H.quantize(x)
+    v = q.cpu().double() * s.cpu().double().repeat_interleave(128, 1)
+    r = qr.double() * sr.double().repeat_interleave(128, 1)
+    assert torch.equal(torch.isnan(v[1, :128]), torch.isnan(r[1, :128])) and v[1, 128:].eq(0).all()
+    assert torch.isnan(v[2]).any() and v[2, :128].eq(0).all()
+    for m in (0, 3):
+        assert torch.equal(q.cpu().view(torch.uint8)[m], qr.view(torch.uint8)[m]) and torch.equal(s.cpu()[m], sr[m])
+
+
+@pytest.mark.parametrize("tiled", [True, False])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 64), (17, 1, 128), (17, 128, 192), (64, 300, 1088), (77, 2500, 2112),
+                                   (129, 5120, 256), (300, 130, 8256), (200, 26000, 192), (1030, 8200, 320), (513, 127, 64)])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_w8a8(qf, M, N, K, tiled, out):
+    _check(qf, M, N, K, tiled, M % 2 == 1, out, True, seed=M + N)
+
+
+def test_linear_picks_by_rows_and_keeps_leading_dims(qf):
+    g = H.gen(5)
+    q, s = H.weight(g, 200, 256)
+    x = H.rows(g, 24, 256).cuda()
+    w, s = q.cuda().t(), s.cuda()
+    assert torch.equal(qf.fp8_linear(x[:16], w, s), qf.fp8_w8a16_mm(x[:16], w, s))
+    assert torch.equal(qf.fp8_linear(x, w, s), qf.fp8_w8a8_mm(x, w, s))
+    assert torch.equal(qf.fp8_linear(x.view(2, 3, 4, 256), w, s), qf.fp8_linear(x, w, s).view(2, 3, 4, 200))
+    assert torch.equal(torch.ops.qwen_fastpath.qf_fp8_linear(x, w, s), qf.fp8_linear(x, w, s))
+    assert qf.fp8_linear(x[:0], w, s).shape == (0, 200)
+
+
+@pytest.mark.parametrize("M", [5, 40, 300])
+def test_strided_and_unaligned_inputs(qf, M):
+    g = H.gen(M)
+    q, s = H.weight(g, 200, 320)
+    x = H.rows(g, M, 320)
+    w, sc = q.cuda().t(), s.cuda()
+    y = qf.fp8_linear(x.cuda(), w, sc)
+    wide = torch.zeros(M, 400, dtype=BF16, device="cuda")
+    wide[:, 8:328] = x.cuda()
+    assert torch.equal(qf.fp8_linear(wide[:, 8:328], w, sc), y)
+    wide[:, 3:323] = x.cuda()
+    assert torch.equal(qf.fp8_linear(wide[:, 3:323], w, sc), y)
+    assert torch.equal(qf.fp8_linear(x.cuda().t().contiguous().t(), w, sc), y)
+    rows = torch.zeros(200, 352, dtype=torch.uint8, device="cuda")
+    rows[:, 16:336] = q.cuda().view(torch.uint8)
+    assert torch.equal(qf.fp8_linear(x.cuda(), rows[:, 16:336].view(H.FP8).t(), sc), y)
+
+
+@pytest.mark.parametrize("M", [4, 40])
+def test_not_finite_values_stay_in_their_rows_and_channels(qf, M):
+    g = H.gen(M)
+    q, s = H.weight(g, 200, 320)
+    x = H.rows(g, M, 320)
+    x[1, 300] = float("nan")
+    qb = q.view(torch.uint8)
+    qb[70, 11] = 0x7f  # NaN
+    y = qf.fp8_linear(x.cuda(), q.cuda().t(), s.cuda()).cpu()
+    nan = torch.zeros(M, 200, dtype=torch.bool)
+    nan[1] = True
+    nan[:, 70] = True
+    assert torch.equal(torch.isnan(y), nan)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 2500, 1088), (77, 2500, 2112), (300, 512, 1024)])
+def test_graph_replays_and_repeats_bitwise(qf, M, N, K):
+    g = H.gen(M)
+    q, s = H.weight(g, N, K)
+    w, s = _weight_on(qf, q, True), s.cuda()
+    x = H.rows(g, M, K).cuda()
+    other = H.rows(g, M, K).cuda()
+    want, want_other = (qf.fp8_linear(v, w, s, out_features=N) for v in (x, other))
+    static = x.clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        y = qf.fp8_linear(static, w, s, out_features=N)
+        z = qf.fp8_linear(static, w, s, out_features=N)
+    for v, ref in ((x, want), (other, want_other), (x, want)):
+        static.copy_(v)
+        graph.replay()
+        assert torch.equal(qf.fp8_linear(v, w, s, out_features=N), ref)  # the program's own work between replays
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref) and torch.equal(z, ref)
+
+
+def test_calls_on_two_streams_at_once(qf):
+    g = H.gen(9)
+    q, s = H.weight(g, 1000, 2112)
+    w, s = q.cuda().t(), s.cuda()
+    xs = [H.rows(g, M, 2112).cuda() for M in (40, 300, 7, 129)]
+    want = [qf.fp8_linear(x, w, s) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(qf.fp8_linear(xs[i // 2], w, s))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i // 2])
