@@ -49,9 +49,15 @@ int qf_block_abi_version(void);
 /* y[m, n] = sum over blocks of scale[n / 128, kb] * sum_{k in kb} x[m, k] * q[n, k] (+ bias[n]): x bf16 [M, K] (row
  * stride ldx), w e4m3, scale fp32 [ceil(N / 128), ceil(K / 128)] contiguous, bias bf16 [N] or NULL, y bf16 or fp32
  * [M, N] (row stride ldy).  1 <= M <= 16.  Products are exact, sums fp32, y is rounded once.  x and w 16-byte aligned,
- * ldx % 8 == 0, row-major ldw % 16 == 0, else QF_ERR_UNSUPPORTED. */
+ * ldx % 8 == 0, row-major ldw % 16 == 0, both at most 2^26, else QF_ERR_UNSUPPORTED. */
 int qf_fp8_w8a16_gemm(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, int layout, const float* scale,
-                      const uint16_t* bias, void* y, int64_t ldy, int out_dtype, int M, int N, int K, void* stream);
+                      const uint16_t* bias, void* y, int64_t ldy, int out_dtype, int M, int N, int K, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of qf_fp8_w8a16_gemm: 0 where K is not split (and for sizes that are not served), else
+ * QF_W8A16_COUNTER_BYTES of arrival counters, which must be zero and are left zero, and the partial sums; calls that may
+ * run at the same time need distinct ones (16-byte aligned).  Host-only. */
+size_t qf_fp8_w8a16_workspace_bytes(int M, int N, int K, int layout);
 
 /* xq[m, k] = e4m3(x[m, k] / s_a[m, kb]), s_a[m, kb] = max_{k in kb} |x[m, k]| / 448 in fp32, both roundings to nearest
  * even; a block of zeros has scale 0 and values 0, a block that holds an infinity or NaN gives NaN there.  x bf16 [M, K] (row
@@ -86,7 +92,7 @@ size_t qf_moe_few_workspace_bytes(int T, int E, int top_k, int H, int I);
 /* One mixture-of-experts layer for T <= 16 tokens: token t takes the top_k largest of its E router logits (the lowest
  * index first among equal ones, NaN largest), weighs expert e by c = softmax(logits)[e] (divided by the sum of the
  * chosen ones with renormalize; 0 for a row of -inf only, and an expert of weight 0 is not read for that token), and
- *   y[t] = sum_e c[t, e] * W2_e a_e,   a_e = bf16(silu(Wgate_e x[t]) * (Wup_e x[t])).
+ *   y[t] = sum_e c[t, e] * W2_e a_e,   a_e = silu(Wgate_e x[t]) * (Wup_e x[t]), kept to 16 bits between the products.
  * x bf16 [T, H], logits bf16 or fp32 [T, E] (row stride ldl), y bf16 [T, H].  w13: the TILED image of [E * 2 I, H] (each
  * expert's I gate rows, then its I up rows), s13 fp32 [E, 2, ceil(I / 128), ceil(H / 128)]; w2: the image of [E * H, I],
  * s2 fp32 [E, ceil(H / 128), ceil(I / 128)].  H and I multiples of 64, top_k <= min(E, QF_MOE_MAX_TOP_K), E <=

@@ -105,6 +105,40 @@ __device__ __forceinline__ void widen16(u32x4_t v, bf16x8_t& lo, bf16x8_t& hi) {
   hi = __builtin_bit_cast(bf16x8_t, b);
 }
 
+// s_waitcnt with vmcnt = N and the other counters unconstrained.
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
+}
+
+// 32-bit LDS address of a pointer into the workgroup's LDS
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// Every wavefront is done with the reads before; the copies that it makes visible are those waited for.
+__device__ __forceinline__ void ring_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" : : : "memory");
+}
+
+// A block of K of one weight tile times its token fragments, from zero.
+__device__ __forceinline__ f32x4_t block_product(const u32x4_t (&w)[2], const u32x4_t (&x)[2][2], bool second) {
+  f32x4_t blk = {0.f, 0.f, 0.f, 0.f};
+  bf16x8_t lo, hi;
+  widen16(w[0], lo, hi);
+  blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, __builtin_bit_cast(bf16x8_t, x[0][0]), blk, 0, 0, 0);
+  blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, __builtin_bit_cast(bf16x8_t, x[0][1]), blk, 0, 0, 0);
+  if (second) {
+    widen16(w[1], lo, hi);
+    blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, __builtin_bit_cast(bf16x8_t, x[1][0]), blk, 0, 0, 0);
+    blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, __builtin_bit_cast(bf16x8_t, x[1][1]), blk, 0, 0, 0);
+  }
+  return blk;
+}
+
 __device__ __forceinline__ u32x4_t load_once(const uint8_t* p) {  // read once: not kept in the caches
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
 }

@@ -18,7 +18,11 @@ typedef void __attribute__((address_space(3)))* lptr_t;
 constexpr int kTileN = 16;   // channels of a weight tile
 constexpr int kStepK = 64;   // k of a TILED tile
 constexpr int kBlock = QF_FP8_BLOCK;
+constexpr int64_t kMaxStride = (int64_t)1 << 26;  // elements: 16 rows within 2^31 bytes
 constexpr int kXcds = 8;
+constexpr int kMaxLds = 160 * 1024;
+constexpr int kReadOnce = 2;        // cache policy of a direct-to-LDS copy: read once
+constexpr int kCounterStride = 16;  // a counter a cache line
 constexpr int kTokenPad = 256;  // the token scales' rows are padded to this many tokens
 
 struct Fp8Args {
@@ -35,6 +39,10 @@ struct Fp8Args {
   int64_t ldy;
   int out_f32, vec_out;  // vec_out: 4 values of a row may be stored at once
   int M, N, ksteps, kblocks, ntiles;
+  uint64_t* partial;   // decode, K split: [split][ntiles][2][64 lanes]
+  unsigned* counters;  // a run's arrivals, counter_stride apart; zero between calls
+  int counter_stride;
+  int runs, splits;    // decode
 };
 
 // 4 channels n .. n + 3 of one output row (cnt of them exist), the bias added, rounded once.
@@ -67,108 +75,254 @@ __device__ __forceinline__ void store4(const Fp8Args& a, int m, int n, f32x4_t v
   }
 }
 
+// The hardware hands workgroup i to XCD i % kXcds; consecutive logical indexes share an XCD and its L2.
+__device__ __forceinline__ int xcd_order(int i, int n) {
+  const int xcd = i % kXcds, per = n / kXcds, rem = n % kXcds;
+  return xcd * per + min(xcd, rem) + i / kXcds;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Decode product, M <= 16: bf16 activations, the weights widened to bf16 in registers (exact).
 //
-// A workgroup owns NT tiles of 16 channels, its wavefronts interleave over the blocks of K: wavefront v takes the blocks
-// v, v + W, ..., two 16-byte weight loads a lane and tile a block, DEPTH blocks ahead.  Lane (g, r) holds channel r (or
-// token r) at k 16 g .. 16 g + 15 of each half block, so the fragments need no exchange; the x fragments come from the
-// caches, shared by the NT tiles.  The wavefronts' partial tiles meet in LDS and are added in wavefront order.
+// The grid is (runs of 16-channel tiles, K splits).  A workgroup's W wavefronts interleave over the blocks of its K range:
+// wavefront v takes the blocks v, v + W, ... (S at most) of every tile of the run, holds their x in LDS or registers, and
+// streams its blocks, tile after tile, S of them in flight: TILED weights through registers, each block's reloaded for the
+// next tile as soon as it is multiplied; row-major ones through kRowSlots 2 KiB LDS slots of the wavefront's own, by
+// direct-to-LDS copies of whole lines (a lane's 16-byte piece p of row n comes from piece p ^ ((n >> 1) & 7), which spreads a
+// fragment read's 16 rows over the banks).  No barrier before the sums.  Lane (g, r) holds channel r (or token r) at k
+// 16 g .. 16 g + 15 of each half block, so the fragments need no exchange.  Each wavefront parks its partial tile in LDS;
+// wavefront v then adds the W partials of tiles v, v + W, ... in wavefront order; with a K split the last workgroup of a run
+// adds the splits in split order.
 // ---------------------------------------------------------------------------------------------
-template <int LAYOUT, int NT, int DEPTH>
-__global__ void __launch_bounds__(512) fp8_decode_kernel(const Fp8Args a) {
+constexpr int kRowSlots = 3;
+constexpr int kJoinBatch = 4;
+__host__ __device__ constexpr int decode_ring(int layout, int W) {
+  return layout == QF_LAYOUT_TILED ? 0 : W * kRowSlots * 2048;
+}
+
+template <int LAYOUT, int S, int XL>
+__global__ void __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4)))
+fp8_decode_kernel(const Fp8Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  f32x4_t* part = reinterpret_cast<f32x4_t*>(smem);  // [wavefront][NT][64 lanes]
-  constexpr int RING = DEPTH + 1;
+  __shared__ int last_arrival;
+  constexpr int D = kRowSlots;
+  const int W = blockDim.x / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   const int v = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int W = blockDim.x / kWave;
   const int g = lane >> 4, r = lane & 15;
-  const int tile0 = blockIdx.x * NT;
+  const int split = blockIdx.x / a.runs, run = blockIdx.x - split * a.runs;
+  const int t0 = (int)((int64_t)run * a.ntiles / a.runs);
+  const int nt = (int)((int64_t)(run + 1) * a.ntiles / a.runs) - t0;  // >= 1: no more runs than tiles
+  const int kb0 = (int)((int64_t)split * a.kblocks / a.splits);
+  const int kb1 = (int)((int64_t)(split + 1) * a.kblocks / a.splits);
+  const int mine = kb1 - kb0 > v ? (kb1 - kb0 - v + W - 1) / W : 0;  // at most S
+  uint8_t* const xs = smem + decode_ring(LAYOUT, W) + v * S * XL * 1024;  // [W][S][XL] KiB
+  f32x4_t* const part = reinterpret_cast<f32x4_t*>(smem + decode_ring(LAYOUT, W) + W * S * XL * 1024);  // [nt][W][64 lanes]
 
-  constexpr int kHalf = LAYOUT == QF_LAYOUT_TILED ? kTileN * kStepK : kStepK;  // bytes from a half block to the next
-  const uint8_t* wp[NT];
+  if (mine > 0) {  // uniform
+    // x fragments of the wavefront's blocks.  XL > 0 (up to 4 XL tokens): in LDS for the whole run, a copy fetching 4 rows x
+    // 256 bytes of a block, piece p of row n landing at p ^ n.  XL = 0: in registers, read straight from the caches; columns
+    // past the last token stay zero and cost no requests.
+    u32x4_t xf[XL ? 1 : S][2][2];
+    if constexpr (XL == 0) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int tile = min(tile0 + t, a.ntiles - 1);
-    if constexpr (LAYOUT == QF_LAYOUT_TILED) {
-      wp[t] = a.w + ((int64_t)tile * a.ksteps * kWave + lane) * 16;
-    } else {
-      wp[t] = a.w + (int64_t)min(tile * kTileN + r, a.N - 1) * a.ldw + 16 * g;
-    }
-  }
-  const uint16_t* xp = a.x + (int64_t)min(r, a.M - 1) * a.ldx + 16 * g;
-  const int steps = (a.kblocks - v + W - 1) / W;  // >= 1: the host takes no more wavefronts than blocks
-
-  struct Step {
-    u32x4_t w[NT][2];
-    u32x4_t x[2][2];
-  };
-  Step buf[RING];
-  auto load = [&](int i, Step& b) {
-    const int kb = v + min(i, steps - 1) * W;
-    const int second = 2 * kb + 1 < a.ksteps ? 1 : 0;  // a last half block: its first half again, never used
+      for (int p = 0; p < S; ++p) xf[p][0][0] = xf[p][0][1] = xf[p][1][0] = xf[p][1][1] = u32x4_t{0u, 0u, 0u, 0u};
+      if (r < a.M) {
+        const uint16_t* const xp = a.x + (int64_t)r * a.ldx + 16 * g;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint8_t* p = wp[t] + (int64_t)kb * 2 * kHalf;
-      b.w[t][0] = load_once(p);
-      b.w[t][1] = load_once(p + second * kHalf);
-    }
-    const uint16_t* q = xp + (int64_t)kb * kBlock;
+        for (int p = 0; p < S; ++p)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(q + (h ? second * kStepK : 0));
-      b.x[h][0] = p[0];
-      b.x[h][1] = p[1];
-    }
-  };
-  // the blocks' scales, 64 of this wavefront's steps at a time, one a lane
-  const float* srow = a.scale + (int64_t)(tile0 / (kBlock / kTileN)) * a.kblocks;
-  auto scales = [&](int base) { return srow[min(v + (base + lane) * W, a.kblocks - 1)]; };
-  float sreg = scales(0);
-
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) load(d, buf[d]);
-  f32x4_t acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int base = 0; base < steps; base += RING) {
-#pragma unroll
-    for (int d = 0; d < RING; ++d) {
-      const int i = base + d;
-      load(i + DEPTH, buf[(d + DEPTH) % RING]);
-      __builtin_amdgcn_sched_barrier(0);  // the requests go out ahead of this step's math
-      if (i < steps) {                    // uniform
-        if (i > 0 && (i & (kWave - 1)) == 0) sreg = scales(i);
-        const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sreg), i & (kWave - 1)));
-        const Step& b = buf[d];
-        const bool second = 2 * (v + i * W) + 1 < a.ksteps;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          f32x4_t blk = {0.f, 0.f, 0.f, 0.f};
-          bf16x8_t lo, hi;
-          widen16(b.w[t][0], lo, hi);
-          blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, __builtin_bit_cast(bf16x8_t, b.x[0][0]), blk, 0, 0, 0);
-          blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, __builtin_bit_cast(bf16x8_t, b.x[0][1]), blk, 0, 0, 0);
-          if (second) {
-            widen16(b.w[t][1], lo, hi);
-            blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, __builtin_bit_cast(bf16x8_t, b.x[1][0]), blk, 0, 0, 0);
-            blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, __builtin_bit_cast(bf16x8_t, b.x[1][1]), blk, 0, 0, 0);
+          for (int h = 0; h < 2; ++h) {
+            const int step = min(2 * (kb0 + v + p * W) + h, a.ksteps - 1);
+            const u32x4_t* q = reinterpret_cast<const u32x4_t*>(xp + (int64_t)step * kStepK);
+            xf[p][h][0] = q[0];
+            xf[p][h][1] = q[1];
           }
-          acc[t] += blk * s;
+      }
+    } else {
+      const int row = lane >> 4;
+#pragma unroll
+      for (int p = 0; p < S; ++p) {
+        const int kb = kb0 + v + min(p, mine - 1) * W;
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+          const int n = 4 * i + row, piece = (lane & 15) ^ n;
+          const int piece_in = 2 * kb + 1 < a.ksteps ? piece : piece & 7;  // a last half block: its values twice
+          __builtin_amdgcn_global_load_lds((gptr_t)(a.x + (int64_t)min(n, a.M - 1) * a.ldx + (int64_t)kb * kBlock + piece_in * 8),
+                                           (lptr_t)(xs + (p * XL + i) * 1024), 16, 0, 0);
         }
       }
     }
-  }
+    auto x_of = [&](int p, u32x4_t (&f)[2][2]) {
+      if constexpr (XL == 0) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) part[(v * NT + t) * kWave + lane] = acc[t];
-  __syncthreads();
-  for (int t = v; t < NT; t += W) {
-    f32x4_t sum = part[t * kWave + lane];
-    for (int u = 1; u < W; ++u) sum += part[(u * NT + t) * kWave + lane];
-    const int n = (tile0 + t) * kTileN + 4 * g;
-    if (r < a.M && n < a.N) store4(a, r, n, sum);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) f[h][q] = xf[p][h][q];
+      } else {
+        const int n = r & (4 * XL - 1);  // columns past the last token: any row, never stored
+        const uint32_t base = lds_addr(xs) + p * XL * 1024 + n * 256;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            asm volatile("ds_read_b128 %0, %1" : "=v"(f[h][q]) : "v"(base + (((8 * h + 2 * g + q) ^ n) << 4)));
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0][0]), "+v"(f[0][1]), "+v"(f[1][0]), "+v"(f[1][1]));
+      }
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    float sc[S];
+    auto scales = [&](int t) {  // another block of channels: its scales
+      const float* row = a.scale + (int64_t)((t0 + t) / (kBlock / kTileN)) * a.kblocks + kb0 + v;
+#pragma unroll
+      for (int p = 0; p < S; ++p) sc[p] = row[p < mine ? p * W : 0];
+    };
+    auto whole = [&](int p) { return 2 * (kb0 + v + p * W) + 1 < a.ksteps; };  // or half a block, the last one
+
+    if constexpr (LAYOUT == QF_LAYOUT_TILED) {
+      const uint32_t w_lane = (uint32_t)lane * 16;
+      u32x4_t w[S][2];
+      auto load = [&](int t, int p) {  // (blocks past the range: the last one again, not used)
+        const uint8_t* q = a.w + ((int64_t)(t0 + t) * a.ksteps + 2 * (kb0 + v + min(p, mine - 1) * W)) * 1024;
+        w[p][0] = load_once(q + w_lane);
+        w[p][1] = load_once(q + (whole(min(p, mine - 1)) ? 1024 : 0) + w_lane);
+      };
+#pragma unroll
+      for (int p = 0; p < S; ++p) load(0, p);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (XL > 0) wait_vmcnt<2 * S>();  // x, ahead of the weights
+      for (int t = 0; t < nt; ++t) {
+        if (t == 0 || (t0 + t) % (kBlock / kTileN) == 0) scales(t);
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < S; ++p) {
+          if (p < mine) {
+            u32x4_t x[2][2];
+            x_of(p, x);
+            acc += block_product(w[p], x, whole(p)) * sc[p];
+          }
+          load(min(t + 1, nt - 1), p);
+        }
+        part[(t * W + v) * kWave + lane] = acc;
+      }
+    } else {
+      // The copy cursor: block cp of tile ct, into slot cslot.  Past the last block it goes round the last tile again
+      // (in-bounds re-reads into slots that are read no more), so that every copy is made and counted.
+      uint8_t* const ring = smem + v * D * 2048;
+      const int lrow = lane >> 3, piece = (lane & 7) ^ (lrow >> 1);  // rows 8 .. 15 flip piece bit 2 besides
+      int ct = 0, cp = 0;
+      uint32_t cslot = 0;
+      const uint8_t *row0, *row1;
+      auto enter = [&]() {
+        const int n = (t0 + ct) * kTileN + lrow;
+        row0 = a.w + (int64_t)min(n, a.N - 1) * a.ldw;
+        row1 = a.w + (int64_t)min(n + 8, a.N - 1) * a.ldw;
+      };
+      enter();
+      auto copy = [&]() {
+        const bool both = whole(cp);  // else a last half block: its bytes twice, the second ones not used
+        uint8_t* dst = ring + cslot;
+        const int q0 = both ? piece : piece & 3, q1 = both ? piece ^ 4 : (piece ^ 4) & 3;
+        const int64_t k = (int64_t)(kb0 + v + cp * W) * kBlock;
+        __builtin_amdgcn_global_load_lds((gptr_t)(row0 + k + q0 * 16), (lptr_t)dst, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(row1 + k + q1 * 16), (lptr_t)(dst + 1024), 16, 0, 0);
+        cslot = cslot == (D - 1) * 2048 ? 0 : cslot + 2048;
+        if (++cp == mine) {
+          cp = 0;
+          if (ct < nt - 1) {
+            ++ct;
+            enter();
+          }
+        }
+      };
+#pragma unroll
+      for (int d = 0; d < D; ++d) copy();
+      if constexpr (XL > 0) wait_vmcnt<2 * D>();  // x, ahead of the weights
+      const uint32_t f0 = lds_addr(ring) + r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+      const uint32_t f1 = lds_addr(ring) + r * 128 + (((4 + g) ^ ((r >> 1) & 7)) << 4);
+      uint32_t slot = 0;
+      for (int t = 0; t < nt; ++t) {
+        if (t == 0 || (t0 + t) % (kBlock / kTileN) == 0) scales(t);
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < S; ++p) {
+          if (p < mine) {  // uniform
+            wait_vmcnt<2 * (D - 1)>();  // this block's copies have landed
+            // Read by inline assembly, waits included: before a plain LDS read the compiler may wait for every copy in flight.
+            u32x4_t w[2];
+            asm volatile(
+                "ds_read_b128 %0, %2\n\t"
+                "ds_read_b128 %1, %3\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(w[0]), "=&v"(w[1])
+                : "v"(f0 + slot), "v"(f1 + slot)
+                : "memory");
+            copy();  // the reads have returned: into the slot they read
+            slot = slot == (D - 1) * 2048 ? 0 : slot + 2048;
+            u32x4_t x[2][2];
+            x_of(p, x);
+            acc += block_product(w, x, whole(p)) * sc[p];
+          }
+        }
+        part[(t * W + v) * kWave + lane] = acc;
+      }
+      wait_vmcnt<0>();  // no copy lands once the workgroup's LDS is given back
+    }
+  } else {
+    for (int t = 0; t < nt; ++t) part[(t * W + v) * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  __syncthreads();
+  // a split's partial tile: 64 lanes x 16 bytes, as two planes of 8 bytes a lane
+  auto slot = [&](int split, int t) { return a.partial + ((int64_t)split * a.ntiles + t0 + t) * 2 * kWave + lane; };
+  for (int t = v; t < nt; t += W) {
+    f32x4_t sum = part[t * W * kWave + lane];
+    for (int u = 1; u < W; ++u) sum += part[(t * W + u) * kWave + lane];
+    const int n = (t0 + t) * kTileN + 4 * g;
+    if (r >= a.M) continue;
+    if (a.splits == 1) {
+      if (n < a.N) store4(a, r, n, sum);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        __hip_atomic_store(slot(split, t) + i * kWave, __builtin_bit_cast(uint64_t, f32x2_t{sum[2 * i], sum[2 * i + 1]}),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (a.splits == 1) return;
+  // The splits' sums are in device memory (device-scope stores, waited for) before the run's counter is raised; the last
+  // arrival reads them with device-scope loads issued after its increment returned, and returns the counter to zero.
+  wait_vmcnt<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned prev = __hip_atomic_fetch_add(a.counters + run * a.counter_stride, 1u, __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+    last_arrival = prev == (unsigned)(a.splits - 1);
+  }
+  __syncthreads();
+  if (!last_arrival) return;
+  for (int t = v; t < nt; t += W) {
+    const int n = (t0 + t) * kTileN + 4 * g;
+    if (r < a.M && n < a.N) {
+      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < a.splits; j += kJoinBatch) {  // a batch's loads are all in flight at once
+        f32x2_t q[kJoinBatch][2];
+#pragma unroll
+        for (int k = 0; k < kJoinBatch; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            q[k][i] = __builtin_bit_cast(f32x2_t, __hip_atomic_load(slot(min(j + k, a.splits - 1), t) + i * kWave,
+                                                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+#pragma unroll
+        for (int k = 0; k < kJoinBatch; ++k) {
+          const f32x4_t p = {q[k][0].x, q[k][0].y, q[k][1].x, q[k][1].y};
+          if (j + k < a.splits) sum = j + k == 0 ? p : sum + p;
+        }
+      }
+      store4(a, r, n, sum);
+    }
+  }
+  if (threadIdx.x == 0)
+    __hip_atomic_store(a.counters + run * a.counter_stride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -248,25 +402,6 @@ __global__ void __launch_bounds__(256) quantize_tokens_fp8_kernel(const QuantArg
 // rounding.  The narrower f8 instruction (16x16x32) drops the same and runs at a third of the rate (1.42 against 4.58
 // PFLOP/s); the widened bf16 product of the decode kernel keeps everything, at half of it.
 // ---------------------------------------------------------------------------------------------
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt range");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
-}
-
-// Every wavefront is done with the reads before; the copies that it makes visible are those waited for.
-__device__ __forceinline__ void ring_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" : : : "memory");
-}
-
-// The hardware hands workgroup i to XCD i % kXcds; consecutive logical indexes share an XCD and its L2.
-__device__ __forceinline__ int xcd_order(int i, int n) {
-  const int xcd = i % kXcds, per = n / kXcds, rem = n % kXcds;
-  return xcd * per + min(xcd, rem) + i / kXcds;
-}
-
 template <int FA_, int FB_, int WN_, int WM_, int S_>
 struct Tile {
   static constexpr int FA = FA_, FB = FB_, WN = WN_, WM = WM_, S = S_;
@@ -473,6 +608,7 @@ int check_product(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t ldw,
   if (layout == QF_LAYOUT_ROWMAJOR && N > 1 && ldw < K) return QF_ERR_INVALID_ARG;
   if (K % kStepK || ldx % 8 || !aligned16(x) || !aligned16(w) || (layout == QF_LAYOUT_ROWMAJOR && ldw % 16))
     return QF_ERR_UNSUPPORTED;
+  if (ldx > kMaxStride || (layout == QF_LAYOUT_ROWMAJOR && ldw > kMaxStride)) return QF_ERR_UNSUPPORTED;
   if (N > 0x7fffffff - 255 || K > 0x7fffffff - 255 || M > 0x7fffffff - 255) return QF_ERR_UNSUPPORTED;
   return QF_OK;
 }
@@ -497,18 +633,86 @@ void fill(Fp8Args& a, const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t 
   a.ntiles = (N + kTileN - 1) / kTileN;
 }
 
-template <int LAYOUT, int NT, int DEPTH>
-int launch_decode(const Fp8Args& a, int waves, hipStream_t s) {
-  hipLaunchKernelGGL((fp8_decode_kernel<LAYOUT, NT, DEPTH>), dim3((unsigned)((a.ntiles + NT - 1) / NT)),
-                     dim3((unsigned)(waves * kWave)), (size_t)waves * NT * 1024, s, a);
+// Runs of tiles and splits of K of a decode call.
+constexpr int kMaxRuns = QF_W8A16_COUNTER_BYTES / 4;
+constexpr int kMaxWaves = 16;   // a workgroup's: with at most 128 registers a lane, as many as a CU holds
+constexpr int kDecodeGrid = 256;
+
+struct DecodePlan {
+  int waves, runs, splits, blocks, xl;  // blocks: S
+  size_t lds;
+};
+
+// One workgroup a CU (a second round costs 3.5 us: 272 tiles 11.7 us against 8.3 for 256, K = 5120), so runs as long as that
+// takes, and the cheapest number of splits by what a CU then has to fetch (28 bytes a ns under load) and what joining them
+// costs: 3 us and 0.25 + 0.06 splits a tile of the run.  Splits pay where x is large beside a run's weights.  Measured at M = 16 in us, K
+// = 5120, without a split and with the chosen ones: N = 1280 9.4 -> 7.2, 5120 13.0 -> 12.3, 10240 16.1 (2 splits 17.8);
+// 5120 x 8192 20.4 -> 15.2.  x in LDS (xl) where it fits beside the run's partials, else in registers, 3 blocks a
+// wavefront at most.
+DecodePlan plan_decode(int layout, int M, int ntiles, int kblocks) {
+  DecodePlan best = {};
+  double best_cost = 0;
+  for (int xl : {M <= 4 ? 1 : M <= 8 ? 2 : 4, 0}) {
+    const int most_blocks = xl || layout == QF_LAYOUT_ROWMAJOR ? 5 : 3;
+    const int most = kMaxWaves * most_blocks;
+    const int least = (kblocks + most - 1) / most;
+    for (int splits = least; splits < least + 8 && splits <= kblocks; ++splits) {
+      const int share = (kblocks + splits - 1) / splits;
+      for (int waves : {kMaxWaves, kMaxWaves / 2}) {
+      int S = (share + waves - 1) / waves;
+      if (S == 4) S = 5;
+      if (S > most_blocks) continue;
+      const int W = (share + S - 1) / S;
+      const int fixed = decode_ring(layout, W) + W * S * xl * 1024;
+      const int room = ((int)kMaxLds - 1024 - fixed) / (W * 1024);
+      if (room < 1) continue;
+      const int slots = splits < kDecodeGrid ? kDecodeGrid / splits : 1;
+      const int run = (ntiles + slots - 1) / slots < room ? (ntiles + slots - 1) / slots : room;
+      const int64_t runs = (ntiles + run - 1) / run;
+      const int64_t rounds = (runs * splits + kDecodeGrid - 1) / kDecodeGrid;
+      const double kb = 0.128 * share * (16.0 * run + 2 * M);  // thousand bytes a workgroup
+      const double cost = rounds * (kb / 28 * (W < 12 ? 1.04 : 1) + (xl ? 0 : 0.3 * S)) + 3.5 * (rounds - 1) +
+                          (splits > 1 ? 3.0 + run * (0.25 + 0.06 * splits) : 0);
+      if (best.waves == 0 || cost < best_cost) {
+        best_cost = cost;
+        best = DecodePlan{W, (int)runs, splits, S, xl, (size_t)fixed + (size_t)run * W * 1024};
+      }
+      }
+    }
+  }
+  return best;
+}
+
+template <int LAYOUT, int S, int XL>
+int launch_decode(const Fp8Args& a, const DecodePlan& p, hipStream_t s) {
+  static std::atomic<uint64_t> raised{0};
+  if (!raise_lds(reinterpret_cast<const void*>(&fp8_decode_kernel<LAYOUT, S, XL>), kMaxLds - 512, raised)) return QF_ERR_HIP;
+  hipLaunchKernelGGL((fp8_decode_kernel<LAYOUT, S, XL>), dim3((unsigned)(p.runs * p.splits)), dim3(p.waves * kWave),
+                     p.lds, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
 
+template <int LAYOUT, int XL>
+int decode_by_blocks(const Fp8Args& a, const DecodePlan& p, hipStream_t s) {
+  switch (p.blocks) {
+    case 1: return launch_decode<LAYOUT, 1, XL>(a, p, s);
+    case 2: return launch_decode<LAYOUT, 2, XL>(a, p, s);
+    case 3: return launch_decode<LAYOUT, 3, XL>(a, p, s);
+    case 5:
+      if constexpr (XL > 0 || LAYOUT == QF_LAYOUT_ROWMAJOR) return launch_decode<LAYOUT, 5, XL>(a, p, s);
+      return QF_ERR_UNSUPPORTED;
+    default: return QF_ERR_UNSUPPORTED;
+  }
+}
+
 template <int LAYOUT>
-int decode(const Fp8Args& a, hipStream_t s) {
-  const int waves = a.kblocks < 8 ? a.kblocks : 8;
-  if (a.ntiles >= 1024) return launch_decode<LAYOUT, 2, 3>(a, waves, s);
-  return launch_decode<LAYOUT, 1, 4>(a, waves, s);
+int decode(const Fp8Args& a, const DecodePlan& p, hipStream_t s) {
+  switch (p.xl) {
+    case 0: return decode_by_blocks<LAYOUT, 0>(a, p, s);
+    case 1: return decode_by_blocks<LAYOUT, 1>(a, p, s);
+    case 2: return decode_by_blocks<LAYOUT, 2>(a, p, s);
+    default: return decode_by_blocks<LAYOUT, 4>(a, p, s);
+  }
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -536,15 +740,37 @@ extern "C" {
 
 int qf_block_abi_version(void) { return QF_BLOCK_ABI_VERSION; }
 
+size_t qf_fp8_w8a16_workspace_bytes(int M, int N, int K, int layout) {
+  if (M < 1 || M > QF_FP8_MAX_DECODE_M || N < 1 || K < kStepK || K % kStepK || N > 0x7fffffff - 255 ||
+      (layout != QF_LAYOUT_ROWMAJOR && layout != QF_LAYOUT_TILED))
+    return 0;
+  const int ntiles = (N - 1) / kTileN + 1;
+  const int splits = plan_decode(layout, M, ntiles, (K - 1) / kBlock + 1).splits;
+  return splits == 1 ? 0 : QF_W8A16_COUNTER_BYTES + (size_t)splits * ntiles * 1024;
+}
+
 int qf_fp8_w8a16_gemm(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, int layout, const float* scale,
-                      const uint16_t* bias, void* y, int64_t ldy, int out_dtype, int M, int N, int K, void* stream) {
+                      const uint16_t* bias, void* y, int64_t ldy, int out_dtype, int M, int N, int K, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   const int st = check_product(x, ldx, w, ldw, layout, scale, y, ldy, out_dtype, M, N, K);
   if (st != QF_OK) return st;
   if (M > QF_FP8_MAX_DECODE_M) return QF_ERR_UNSUPPORTED;
   Fp8Args a;
   fill(a, x, ldx, w, ldw, scale, bias, y, ldy, out_dtype, M, N, K);
+  const DecodePlan p = plan_decode(layout, M, a.ntiles, a.kblocks);
+  if (p.waves == 0) return QF_ERR_UNSUPPORTED;
+  if (p.splits > 1) {
+    if (p.runs > kMaxRuns || (int64_t)p.runs * p.splits > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+    if (workspace == nullptr || workspace_bytes < qf_fp8_w8a16_workspace_bytes(M, N, K, layout) || !aligned16(workspace))
+      return QF_ERR_WORKSPACE;
+    a.counters = static_cast<unsigned*>(workspace);
+    a.counter_stride = p.runs * kCounterStride <= kMaxRuns ? kCounterStride : 1;
+    a.partial = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + QF_W8A16_COUNTER_BYTES);
+  }
+  a.runs = p.runs;
+  a.splits = p.splits;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return layout == QF_LAYOUT_TILED ? decode<QF_LAYOUT_TILED>(a, s) : decode<QF_LAYOUT_ROWMAJOR>(a, s);
+  return layout == QF_LAYOUT_TILED ? decode<QF_LAYOUT_TILED>(a, p, s) : decode<QF_LAYOUT_ROWMAJOR>(a, p, s);
 }
 
 int qf_quantize_tokens_fp8(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* xq, int64_t ldq, float* s_a,

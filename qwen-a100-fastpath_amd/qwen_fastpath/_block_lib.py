@@ -28,6 +28,7 @@ ACTS = {"none": 0, "sigmoid": 1}
 EXPORTS = (
     "qf_block_abi_version",
     "qf_fp8_w8a16_gemm",
+    "qf_fp8_w8a16_workspace_bytes",
     "qf_quantize_tokens_fp8",
     "qf_fp8_w8a8_workspace_bytes",
     "qf_fp8_w8a8_linear",
@@ -53,7 +54,8 @@ def load() -> ctypes.CDLL:
     product = [p, i64, p, i64, i32, p, p, p, i64, i32, i32, i32, i32]
     for name, res, args in (
             ("qf_block_abi_version", i32, []),
-            ("qf_fp8_w8a16_gemm", i32, product + [p]),
+            ("qf_fp8_w8a16_workspace_bytes", sz, [i32] * 4),
+            ("qf_fp8_w8a16_gemm", i32, product + [p, sz, p]),
             ("qf_quantize_tokens_fp8", i32, [p, i64, i32, i32, p, i64, p, p]),
             ("qf_fp8_w8a8_workspace_bytes", sz, [i32] * 3),
             ("qf_fp8_w8a8_linear", i32, product + [p, sz, p]),

@@ -15,8 +15,9 @@ from typing import Optional
 import torch
 
 from . import _block_lib as B
-from .w8a16 import ROWMAJOR, TILED, from_tiled, tiled_numel, to_tiled
+from .w8a16 import ROWMAJOR, TILED, _workspace, from_tiled, tiled_numel, to_tiled
 
+_MAX_STRIDE = 1 << 26  # longest row stride the products address
 _BF16, _FP8, _F32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32
 
 
@@ -64,7 +65,7 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     the row stride."""
     M, K = x.shape
     ld = x.stride(0) if M > 1 else K
-    if (x.stride(1) != 1 and K > 1) or x.data_ptr() % 16 or ld % 8 or ld < K:
+    if (x.stride(1) != 1 and K > 1) or x.data_ptr() % 16 or ld % 8 or not K <= ld <= _MAX_STRIDE:
         return x.clone(memory_format=torch.contiguous_format), K
     return x, ld
 
@@ -96,8 +97,8 @@ def _product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Opti
         if N < 1 or (out_features is not None and out_features != N):
             raise ValueError(f"weight has {N} output channels, out_features is {out_features}")
         ldw = w.stride(1) if N > 1 else K
-        if ldw < K or ldw % 16:
-            raise ValueError(f"row-major weight needs a row stride of at least K that is a multiple of 16, got {ldw}")
+        if not K <= ldw <= _MAX_STRIDE or ldw % 16:
+            raise ValueError(f"row-major weight needs a row stride from K to 2^26 that is a multiple of 16, got {ldw}")
     if w.data_ptr() % 16:
         raise ValueError("weight must be 16-byte aligned")
     if w_scale.dim() != 2 or w_scale.shape != fp8_scale_shape(N, K):
@@ -116,7 +117,9 @@ def _product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Opti
     args = (x.data_ptr(), ldx, w.data_ptr(), ldw, layout, w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
             y.data_ptr(), N, 0 if out_dtype is _BF16 else 1, M, N, K)
     if M <= B.MAX_DECODE_M if decode is None else decode:
-        B.call("qf_fp8_w8a16_gemm", dev, *args)
+        nbytes = B.load().qf_fp8_w8a16_workspace_bytes(M, N, K, layout)
+        ws = _workspace(dev, nbytes) if nbytes else None  # K splits' arrival counters: zero between calls
+        B.call("qf_fp8_w8a16_gemm", dev, *args, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     else:
         nbytes = B.load().qf_fp8_w8a8_workspace_bytes(M, N, K)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the caching allocator's: one a call, capture-safe

@@ -25,7 +25,7 @@ def moe_few_tokens(x: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tens
     TILED image (fp8_to_tiled) of the [E * 2 I, H] matrix of each expert's I gate rows, then its I up rows, s13 fp32
     [E, 2 ceil(I / 128), ceil(H / 128)] in that order; w2: the image of [E * H, I], s2 fp32 [E, ceil(H / 128),
     ceil(I / 128)].  H and I multiples of 64; E <= 512, top_k <= min(E, 16).  Activations stay bf16, weights are widened
-    exactly, sums are fp32; the activation is rounded to bf16 before the down product, y once at the end."""
+    exactly, sums are fp32; the activation is kept to 16 bits between the products, y is rounded once at the end."""
     if x.dim() != 2 or x.dtype is not _BF16:
         raise TypeError(f"x must be a 2-D bf16 tensor, got {x.dtype} {tuple(x.shape)}")
     if router_logits.dim() != 2 or (router_logits.dtype is not _F32 and router_logits.dtype is not _BF16):

@@ -48,11 +48,6 @@ def _routing(logits, k, renorm):
     return out
 
 
-def _bf16_range(a, err):
-    """bf16 roundings of the ends of a +- err."""
-    return (a - err).to(F32).to(BF16).double(), (a + err).to(F32).to(BF16).double()
-
-
 def _reference(x, logits, up, down, k, renorm):
     T, Hd = x.shape
     I = down[0][0].shape[1]
@@ -71,13 +66,14 @@ def _reference(x, logits, up, down, k, renorm):
             silu = g * torch.sigmoid(g)
             # the slope of silu is below 1.1; exp, the sum, the division and the product add a few roundings
             err = 1.1 * eg * (u.abs() + eu) + silu.abs() * eu + (silu * u).abs() * (g.abs() + 16) * 2.0 ** -23
-            lo, hi = _bf16_range(silu * u, err)
-            a = (silu * u).to(F32).to(BF16).double()  # inside [lo, hi]: rounding keeps order
+            a = silu * u
             w2 = H.widen(*down[e])
             y[t] += c * (w2 @ a)
-            # where the activation's rounding may fall either way, by as much; the sums; the weight c to 2^-20
-            # (its logits differ by at most 100: 100 * 2^-24 in the exponent, and the sum's and quotient's roundings)
-            bound[t] += c * (w2.abs() @ (hi - lo)) + c * (w2.abs() @ a.abs()) * ((k * I + 16) * H.SUM + 2.0 ** -16)
+            # the activation as two bf16 numbers: what the first leaves (2^-8) is rounded by 2^-8 of itself; the sums, of
+            # both; the weight c (its logits differ by at most 100: 100 * 2^-24 in the exponent, and the sum's and
+            # quotient's roundings: 2^-16 covers them)
+            bound[t] += c * (w2.abs() @ (err + 2.0 ** -16 * a.abs())) + c * (w2.abs() @ a.abs()) * (
+                (2 * k * I + 16) * H.SUM + 2.0 ** -16)
     return y, bound
 
 
