@@ -117,6 +117,20 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
+// A pointer that is the same in every lane, in scalar registers.
+__device__ __forceinline__ const uint8_t* scalar_ptr(const uint8_t* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+  return (const uint8_t*)(((uint64_t)hi << 32) | lo);
+}
+
+// A 32-bit lane offset whose extension to an address is done here: a load then takes a scalar base and this register.
+__device__ __forceinline__ uint32_t here(uint32_t offset) {
+  asm volatile("" : "+v"(offset));
+  return offset;
+}
+
 // Every wavefront is done with the reads before; the copies that it makes visible are those waited for.
 __device__ __forceinline__ void ring_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");

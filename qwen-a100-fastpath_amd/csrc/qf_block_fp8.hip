@@ -414,7 +414,8 @@ struct Tile {
   static constexpr int stage = frags * 2048;
   static constexpr int slot = stage + waves * 256;
   static constexpr int lds = S * slot;
-  static_assert(lds <= 160 * 1024 && waves * FA * FB * 512 <= lds, "LDS");
+  static constexpr int max_kblocks = (kMaxLds - lds) / (4 * WN);
+  static_assert(waves * FA * FB * 512 <= lds && max_kblocks >= 1024, "LDS");
 };
 
 template <int LAYOUT, typename T, int MINW, int MAXW>
@@ -436,46 +437,53 @@ fp8_tile_kernel(const Fp8Args a) {
   // fragment f of the stage: the FA WN weight fragments, then the FB WM activation fragments; channels and tokens past
   // the matrix read its last tile, their outputs are not stored
   constexpr int kHalf = LAYOUT == QF_LAYOUT_TILED ? kTileN * kStepK : kStepK;
+  // fragment's bytes: a scalar base and a 32-bit lane offset (the host bounds 16 rows of row-major weights by 2^31 bytes)
   const uint8_t* src[T::own];
-  int adv[T::own], half[T::own];
+  uint32_t src_lane[T::own];
 #pragma unroll
   for (int j = 0; j < T::own; ++j) {
     const int f = wave * T::own + j;
+    src_lane[j] = (uint32_t)lane * 16;
     if (f < FA * T::WN) {
       const int tile = min(tile0 + f, a.ntiles - 1);
       if constexpr (LAYOUT == QF_LAYOUT_TILED) {
-        src[j] = a.w + ((int64_t)tile * a.ksteps * kWave + lane) * 16;
+        src[j] = a.w + (int64_t)tile * a.ksteps * 1024;
       } else {
-        src[j] = a.w + (int64_t)min(tile * kTileN + r, a.N - 1) * a.ldw + 16 * g;
+        src[j] = a.w + (int64_t)tile * kTileN * a.ldw;
+        src_lane[j] = (uint32_t)min(r, a.N - 1 - tile * kTileN) * (uint32_t)a.ldw + 16 * g;
       }
-      half[j] = kHalf;
     } else {
       const int tile = min((m0 >> 4) + f - FA * T::WN, (a.M - 1) >> 4);
-      src[j] = a.xt + ((int64_t)tile * 2 * a.kblocks * kWave + lane) * 16;
-      half[j] = kTileN * kStepK;
+      src[j] = a.xt + (int64_t)tile * 2 * a.kblocks * 1024;
     }
-    adv[j] = 2 * half[j];
+    src[j] = scalar_ptr(src[j]);
   }
-  const float* ssrc = a.s_tok + m0 + 16 * FB * wm + (lane & (16 * FB - 1));
-  auto copy = [&](int s) {  // stage s (past the last: the last again, into a slot that nothing reads any more)
-    uint8_t* slot = smem + (s % S) * T::slot;
+  const float* const ssrc = a.s_tok + m0 + 16 * FB * wm;
+  const uint32_t s_src_lane = (uint32_t)(lane & (16 * FB - 1)) * 4;
+  // Stage s in own + 1 pieces, a fragment each and the token scales (past the last stage: the last again, into a slot that
+  // nothing reads any more).
+  auto copy_piece = [&](int s, int slot_at, int j) {
+    uint8_t* slot = smem + slot_at * T::slot;
     const int kb = min(s, nsteps - 1);
-    const bool second = 2 * kb + 1 < a.ksteps;
-#pragma unroll
-    for (int j = 0; j < T::own; ++j) {
+    if (j < T::own) {
       const int f = wave * T::own + j;
-      const uint8_t* p = src[j] + (int64_t)kb * adv[j];
+      const int half = f < FA * T::WN ? kHalf : kTileN * kStepK;
+      const uint8_t* p = src[j] + (int64_t)kb * 2 * half;
       // a last half block: the weights' first half again, times the activations' zeros
-      const int h = second || f >= FA * T::WN ? half[j] : 0;
-      __builtin_amdgcn_global_load_lds((gptr_t)p, (lptr_t)(slot + f * 2048), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gptr_t)(p + h), (lptr_t)(slot + f * 2048 + 1024), 16, 0, 0);
+      const uint8_t* q = p + (2 * kb + 1 < a.ksteps || f >= FA * T::WN ? half : 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)(scalar_ptr(p) + here(src_lane[j])), (lptr_t)(slot + f * 2048), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)(scalar_ptr(q) + here(src_lane[j])), (lptr_t)(slot + f * 2048 + 1024), 16, 0, 0);
+    } else {
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(ssrc + (int64_t)kb * a.m_pad);
+      __builtin_amdgcn_global_load_lds((gptr_t)(scalar_ptr(p) + here(s_src_lane)), (lptr_t)(slot + T::stage + wave * 256), 4, 0, 0);
     }
-    __builtin_amdgcn_global_load_lds((gptr_t)(ssrc + (int64_t)kb * a.m_pad), (lptr_t)(slot + T::stage + wave * 256), 4, 0, 0);
   };
   const int n_first = (tile0 + FA * wn) * kTileN;  // this wavefront's first channel
   const float* srow = a.scale + (int64_t)min(n_first / kBlock, (a.N - 1) / kBlock) * a.kblocks;
-  float sreg = srow[min(lane, a.kblocks - 1)];
-  wait_vmcnt<0>();  // here and at each later 64 blocks, not at every use
+  // all of its blocks' scales, in LDS behind the ring (a row of kblocks for each of the WN channel groups)
+  float* const sw = reinterpret_cast<float*>(smem + T::lds) + wn * a.kblocks;
+  for (int k = wm * kWave + lane; k < a.kblocks; k += T::WM * kWave) sw[k] = srow[k];
+  wait_vmcnt<0>();  // the copies below are counted
 
   f32x4_t acc[FA][FB];
 #pragma unroll
@@ -483,40 +491,103 @@ fp8_tile_kernel(const Fp8Args a) {
 #pragma unroll
     for (int j = 0; j < FB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) copy(s);
-
-  for (int s = 0; s < nsteps; ++s) {
-    wait_vmcnt<T::copies*(S - 2)>();
-    ring_barrier();
-    copy(s + S - 1);
-    if (s > 0 && (s & (kWave - 1)) == 0) {
-      sreg = srow[min(s + lane, a.kblocks - 1)];
-      wait_vmcnt<0>();
-    }
-    const float sb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sreg), s & (kWave - 1)));
-    const uint8_t* slot = smem + (s % S) * T::slot;
-    auto frag = [&](int f) {
-      const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(slot + f * 2048 + lane * 16);
-      const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(slot + f * 2048 + 1024 + lane * 16);
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    i32x8_t B[FB];
-    float sc[FB];
+  for (int s = 0; s < S - 1; ++s)
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-      B[j] = frag(FA * T::WN + FB * wm + j);
-      sc[j] = *reinterpret_cast<const float*>(slot + T::stage + wave * 256 + (16 * j + r) * 4) * sb;
-    }
+    for (int j = 0; j <= T::own; ++j) copy_piece(s, s, j);
+
+  // LDS reads are issued by inline assembly and waited for by count (before a plain read's use the compiler waits for all of
+  // LDS while copies are in flight); their registers are tied to the waits, so nothing uses them before.
+  const uint32_t lane16 = (uint32_t)lane * 16, r4 = (uint32_t)r * 4;
+  const uint32_t a_at = lds_addr(smem) + FA * wn * 2048;
+  const uint32_t b_at = lds_addr(smem) + (FA * T::WN + FB * wm) * 2048;
+  const uint32_t s_at = lds_addr(smem) + T::stage + wave * 256;
+  const uint32_t w_at = lds_addr(sw);
+  auto read_frag = [](uint32_t at) {
+    i32x4_t lo, hi;
+    asm volatile("ds_read_b128 %0, %1" : "=v"(lo) : "v"(at));
+    asm volatile("ds_read_b128 %0, %1 offset:1024" : "=v"(hi) : "v"(at));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto read_tokens = [&](int s, uint32_t slot, i32x8_t (&B)[FB], float (&sc)[FB], float& w) {  // fragments, both scales
+    asm volatile("ds_read_b32 %0, %1" : "=v"(w) : "v"(w_at + 4 * min(s, nsteps - 1)));
+#pragma unroll
+    for (int j = 0; j < FB; ++j) asm volatile("ds_read_b32 %0, %1" : "=v"(sc[j]) : "v"(here(r4) + (s_at + slot + 64 * j)));
+#pragma unroll
+    for (int j = 0; j < FB; ++j) B[j] = read_frag(here(lane16) + (b_at + slot + j * 2048));
+  };
+  auto tie = [](i32x8_t (&B)[FB], float (&sc)[FB], float& w) {
+    asm volatile("" : "+v"(w));
+#pragma unroll
+    for (int j = 0; j < FB; ++j) asm volatile("" : "+v"(B[j]), "+v"(sc[j]));
+  };
+  // Products wait one row of fragments in t before they are scaled and added, so that the additions run beside the next
+  // row's matrix instructions; each weight fragment is read a row ahead, the next stage's first ones ahead of the last row.
+  // No branch in a stage: the compiler would move additions across it and keep every product alive.
+  // The copies of the stage that refills the slot of stage s - 1 go out between the rows of stage s.
+  constexpr int per_row = (T::own + FA - 1) / (FA - 1);  // pieces: own + 1 over FA - 1 rows
+  f32x4_t t[FB];
+#pragma unroll
+  for (int j = 0; j < FB; ++j) t[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  i32x8_t A[2], B0[FB], B1[FB];
+  float s0[FB], s1[FB], w;
+  int at = 0, free_at = S - 1;  // ring slots of stage s, and of the one before it
+  // (Bn, scn): the stage before (its scales), then the next
+  auto step = [&](int s, i32x8_t (&B)[FB], float (&sc)[FB], i32x8_t (&Bn)[FB], float (&scn)[FB]) {
+    const int next_at = at + 1 == S ? 0 : at + 1;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
-      const i32x8_t A = frag(FA * wn + i);
+      if (i == 1) {
+#pragma unroll
+        for (int j = 0; j < FB; ++j) sc[j] *= w;
+      }
+      if (i + 1 < FA) {
+        A[(i + 1) & 1] = read_frag(here(lane16) + (a_at + (uint32_t)at * T::slot + (i + 1) * 2048));
+        asm volatile("s_waitcnt lgkmcnt(2)" : "+v"(A[i & 1]) : : "memory");
+        if (i == 0) tie(B, sc, w);
+      } else {  // (past the last stage: a stage that is copied again, not used)
+        wait_vmcnt<T::copies*(S - 2)>();
+        ring_barrier();  // stage s + 1 has landed, and nothing reads stage s any more
+        asm volatile("" : "+v"(A[i & 1]));
+        read_tokens(s + 1, (uint32_t)next_at * T::slot, Bn, scn, w);
+        A[(i + 1) & 1] = read_frag(here(lane16) + (a_at + (uint32_t)next_at * T::slot));
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < FB; ++j) {
-        const f32x4_t blk =
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-        acc[i][j] += blk * sc[j];
+        acc[(i + FA - 1) % FA][j] += t[j] * (i == 0 ? scn[j] : sc[j]);
+        t[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A[i & 1], B[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i + 1 < FA) {
+#pragma unroll
+        for (int j = i * per_row; j < (i + 1) * per_row && j <= T::own; ++j) copy_piece(s + S - 1, free_at, j);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    free_at = at;
+    at = next_at;
+  };
+  static_assert(FA % 2 == 0, "the weight fragments' two buffers alternate through a stage");
+#pragma unroll
+  for (int j = 0; j < FB; ++j) s1[j] = 0.f;
+  wait_vmcnt<T::copies*(S - 2)>();
+  ring_barrier();
+  read_tokens(0, 0, B0, s0, w);
+  A[0] = read_frag(here(lane16) + a_at);
+  int s = 0;
+  for (; s + 1 < nsteps; s += 2) {
+    step(s, B0, s0, B1, s1);
+    step(s + 1, B1, s1, B0, s0);
+  }
+  const bool odd = s < nsteps;
+  if (odd) step(s, B0, s0, B1, s1);
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(A[0]), "+v"(A[1]) : : "memory");  // the reads past the last stage have returned
+  tie(B0, s0, w);
+  tie(B1, s1, w);
+#pragma unroll
+  for (int j = 0; j < FB; ++j) {
+    const float even_s = s1[j], odd_s = s0[j];
+    acc[FA - 1][j] += t[j] * (odd ? odd_s : even_s);
   }
   wait_vmcnt<0>();  // the last copies have landed before LDS is reused or released
 
@@ -582,10 +653,10 @@ typedef Tile<2, 4, 4, 1, 3> SmallTile;  // 128 x 64
 template <int LAYOUT, typename T, int MINW, int MAXW>
 int launch_tile(const Fp8Args& a, hipStream_t s) {
   static std::atomic<uint64_t> raised{0};
-  if (!raise_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), T::lds, raised)) return QF_ERR_HIP;
+  if (!raise_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), kMaxLds, raised)) return QF_ERR_HIP;
   const int64_t grid = (int64_t)((a.N + T::channels - 1) / T::channels) * ((a.M + T::tokens - 1) / T::tokens);
-  if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), dim3((unsigned)grid), dim3(T::waves * kWave), T::lds, s, a);
+  if (grid > 0x7fffffff || a.kblocks > T::max_kblocks) return QF_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), dim3((unsigned)grid), dim3(T::waves * kWave), T::lds + T::WN * a.kblocks * 4, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
 
