@@ -39,10 +39,10 @@ struct Fp8Args {
   int64_t ldy;
   int out_f32, vec_out;  // vec_out: 4 values of a row may be stored at once
   int M, N, ksteps, kblocks, ntiles;
-  uint64_t* partial;   // decode, K split: [split][ntiles][2][64 lanes]
-  unsigned* counters;  // a run's arrivals, counter_stride apart; zero between calls
+  uint64_t* partial;   // K split: decode [split][ntiles][2][64 lanes], else [tile][split][wavefront][FA][FB][2][64 lanes]
+  unsigned* counters;  // arrivals of a run (counter_stride apart, zero between calls) or a tile (zeroed by the quantiser)
   int counter_stride;
-  int runs, splits;    // decode
+  int runs, splits;    // runs: decode
 };
 
 // 4 channels n .. n + 3 of one output row (cnt of them exist), the bias added, rounded once.
@@ -338,12 +338,16 @@ struct QuantArgs {
   float* s;
   int m_pad;
   int M, ksteps, kblocks;
+  unsigned* counters;  // the product's arrival counters, zeroed here
+  int n_counters;
 };
 
 constexpr int kQuantBlocks = 4;  // blocks of 128 a workgroup
 
 template <bool TILED>
 __global__ void __launch_bounds__(256) quantize_tokens_fp8_kernel(const QuantArgs a) {
+  if (TILED && blockIdx.x == 0 && blockIdx.y == 0)
+    for (int c = threadIdx.x; c < a.n_counters; c += 256) a.counters[c] = 0;
   const int i = threadIdx.x & 15;
   const int m = blockIdx.x * 16 + threadIdx.x / 16;
   const int mr = min(m, a.M - 1);
@@ -428,11 +432,13 @@ fp8_tile_kernel(const Fp8Args a) {
   const int wn = wave % T::WN, wm = wave / T::WN;
   const int g = lane >> 4, r = lane & 15;
   const int mblocks = (a.M + T::tokens - 1) / T::tokens;
-  const int l = xcd_order(blockIdx.x, gridDim.x);
-  const int nb = l / mblocks, mb = l - nb * mblocks;
+  const int place = xcd_order(blockIdx.x, gridDim.x);
+  const int tile = place / a.splits, split = place - tile * a.splits;
+  const int nb = tile / mblocks, mb = tile - nb * mblocks;
   const int tile0 = nb * (T::channels / 16);
   const int m0 = mb * T::tokens;
-  const int nsteps = a.kblocks;
+  const int k0 = (int)((int64_t)split * a.kblocks / a.splits);  // this workgroup's blocks of K
+  const int nsteps = (int)((int64_t)(split + 1) * a.kblocks / a.splits) - k0;
 
   // fragment f of the stage: the FA WN weight fragments, then the FB WM activation fragments; channels and tokens past
   // the matrix read its last tile, their outputs are not stored
@@ -445,16 +451,16 @@ fp8_tile_kernel(const Fp8Args a) {
     const int f = wave * T::own + j;
     src_lane[j] = (uint32_t)lane * 16;
     if (f < FA * T::WN) {
-      const int tile = min(tile0 + f, a.ntiles - 1);
+      const int t = min(tile0 + f, a.ntiles - 1);
       if constexpr (LAYOUT == QF_LAYOUT_TILED) {
-        src[j] = a.w + (int64_t)tile * a.ksteps * 1024;
+        src[j] = a.w + (int64_t)t * a.ksteps * 1024;
       } else {
-        src[j] = a.w + (int64_t)tile * kTileN * a.ldw;
-        src_lane[j] = (uint32_t)min(r, a.N - 1 - tile * kTileN) * (uint32_t)a.ldw + 16 * g;
+        src[j] = a.w + (int64_t)t * kTileN * a.ldw;
+        src_lane[j] = (uint32_t)min(r, a.N - 1 - t * kTileN) * (uint32_t)a.ldw + 16 * g;
       }
     } else {
-      const int tile = min((m0 >> 4) + f - FA * T::WN, (a.M - 1) >> 4);
-      src[j] = a.xt + (int64_t)tile * 2 * a.kblocks * 1024;
+      const int t = min((m0 >> 4) + f - FA * T::WN, (a.M - 1) >> 4);
+      src[j] = a.xt + (int64_t)t * 2 * a.kblocks * 1024;
     }
     src[j] = scalar_ptr(src[j]);
   }
@@ -464,7 +470,7 @@ fp8_tile_kernel(const Fp8Args a) {
   // nothing reads any more).
   auto copy_piece = [&](int s, int slot_at, int j) {
     uint8_t* slot = smem + slot_at * T::slot;
-    const int kb = min(s, nsteps - 1);
+    const int kb = k0 + min(s, nsteps - 1);
     if (j < T::own) {
       const int f = wave * T::own + j;
       const int half = f < FA * T::WN ? kHalf : kTileN * kStepK;
@@ -479,10 +485,10 @@ fp8_tile_kernel(const Fp8Args a) {
     }
   };
   const int n_first = (tile0 + FA * wn) * kTileN;  // this wavefront's first channel
-  const float* srow = a.scale + (int64_t)min(n_first / kBlock, (a.N - 1) / kBlock) * a.kblocks;
-  // all of its blocks' scales, in LDS behind the ring (a row of kblocks for each of the WN channel groups)
-  float* const sw = reinterpret_cast<float*>(smem + T::lds) + wn * a.kblocks;
-  for (int k = wm * kWave + lane; k < a.kblocks; k += T::WM * kWave) sw[k] = srow[k];
+  const float* srow = a.scale + (int64_t)min(n_first / kBlock, (a.N - 1) / kBlock) * a.kblocks + k0;
+  // all of its blocks' scales, in LDS behind the ring (a row for each of the WN channel groups)
+  float* const sw = reinterpret_cast<float*>(smem + T::lds) + wn * nsteps;
+  for (int k = wm * kWave + lane; k < nsteps; k += T::WM * kWave) sw[k] = srow[k];
   wait_vmcnt<0>();  // the copies below are counted
 
   f32x4_t acc[FA][FB];
@@ -591,6 +597,49 @@ fp8_tile_kernel(const Fp8Args a) {
   }
   wait_vmcnt<0>();  // the last copies have landed before LDS is reused or released
 
+  if (a.splits > 1) {
+    // The splits of a tile meet through the workspace: each leaves its sums, lane for lane, by device-scope stores and waits
+    // for them; one thread counts the arrival; the last one to arrive reads the others' by device-scope loads, issued after its
+    // increment returned, and adds all in split order.
+    auto slot = [&](int split, int i, int j) {
+      return a.partial + ((((int64_t)tile * a.splits + split) * T::waves + wave) * (FA * FB) + i * FB + j) * 2 * kWave + lane;
+    };
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          __hip_atomic_store(slot(split, i, j) + h * kWave, __builtin_bit_cast(uint64_t, f32x2_t{acc[i][j][2 * h], acc[i][j][2 * h + 1]}),
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    wait_vmcnt<0>();
+    __syncthreads();
+    int* const last = reinterpret_cast<int*>(smem);
+    if (threadIdx.x == 0)
+      *last = __hip_atomic_fetch_add(a.counters + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+              (unsigned)(a.splits - 1);
+    __syncthreads();
+    if (!*last) return;
+    __syncthreads();  // before LDS is written again
+    for (int o = 0; o < a.splits; ++o) {
+#pragma unroll
+      for (int i = 0; i < FA; ++i) {
+        f32x4_t p[FB];
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f32x2_t v = __builtin_bit_cast(f32x2_t, __hip_atomic_load(slot(o, i, j) + h * kWave, __ATOMIC_RELAXED,
+                                                                            __HIP_MEMORY_SCOPE_AGENT));
+            p[j][2 * h] = v.x;
+            p[j][2 * h + 1] = v.y;
+          }
+#pragma unroll
+        for (int j = 0; j < FB; ++j) acc[i][j] = o == 0 ? p[j] : acc[i][j] + p[j];
+      }
+    }
+  }
+
   // Lane (g, r) holds channels 4 g .. 4 g + 3 of a tile, token r.
   if (!a.out_f32 && a.vec_out && a.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0) {
     // each wavefront's block through its own LDS (16-byte chunk c of token t at c ^ (t % NC)): whole row pieces are stored
@@ -649,25 +698,106 @@ fp8_tile_kernel(const Fp8Args a) {
 typedef Tile<8, 4, 2, 4, 2> BigTile;    // 256 channels x 256 tokens
 typedef Tile<4, 2, 2, 4, 4> MidTile;    // 128 x 128
 typedef Tile<2, 4, 4, 1, 3> SmallTile;  // 128 x 64
+typedef Tile<2, 2, 2, 2, 4> TinyTile;   // 64 x 64
 
 template <int LAYOUT, typename T, int MINW, int MAXW>
 int launch_tile(const Fp8Args& a, hipStream_t s) {
   static std::atomic<uint64_t> raised{0};
   if (!raise_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), kMaxLds, raised)) return QF_ERR_HIP;
-  const int64_t grid = (int64_t)((a.N + T::channels - 1) / T::channels) * ((a.M + T::tokens - 1) / T::tokens);
-  if (grid > 0x7fffffff || a.kblocks > T::max_kblocks) return QF_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), dim3((unsigned)grid), dim3(T::waves * kWave), T::lds + T::WN * a.kblocks * 4, s, a);
+  const int64_t grid = (int64_t)((a.N + T::channels - 1) / T::channels) * ((a.M + T::tokens - 1) / T::tokens) * a.splits;
+  const int share = (a.kblocks + a.splits - 1) / a.splits;
+  if (grid > 0x7fffffff || share > T::max_kblocks) return QF_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), dim3((unsigned)grid), dim3(T::waves * kWave),
+                     T::lds + T::WN * share * 4, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
 
+// The tile shapes' launch figures: us a block of K takes one workgroup a CU and two (0: LDS holds one), and what joining
+// s splits adds, join + s * more (a tile's last arrival reads the others' sums).  Measured over M = 17 to 2048, N = 2000 to
+// 34816, K = 2048 to 8192; the estimates below are within 15% of the times there, but for weights that come from HBM once.
+struct TileFigures {
+  int channels, tokens;
+  double step, step2, join, more;
+};
+enum TileKind { kBig, kMid, kSmall, kTiny, kKinds };
+constexpr TileFigures kFigures[kKinds] = {
+    {256, 256, 1.70, 0, 6.0, 5.0}, {128, 128, 0.57, 0, 2.5, 2.2}, {128, 64, 0.48, 0.85, 1.2, 0.8}, {64, 64, 0.31, 0.50, 1.0, 0.5}};
+constexpr int kCus = 256;
+constexpr double kLaunch = 4.0;  // us
+
+// One launch over N channels, and where main_n > 0 one of whole rounds of 256 x 256 tiles over the first main_n before it.
+struct TilePlan {
+  int kind, splits, main_n;
+  double cost;
+};
+
+int64_t tiles_of(int kind, int M, int N) {
+  const TileFigures& f = kFigures[kind];
+  return (int64_t)((N - 1) / f.channels + 1) * ((M - 1) / f.tokens + 1);
+}
+
+TilePlan plan_single(int M, int N, int kblocks) {
+  TilePlan best = {kTiny, 1, 0, 0};
+  for (int kind = 0; kind < kKinds; ++kind) {
+    const TileFigures& f = kFigures[kind];
+    const int64_t tiles = tiles_of(kind, M, N);
+    for (int splits = 1; splits <= 4 && splits <= kblocks && (splits == 1 || tiles * splits <= kCus); ++splits) {
+      const int64_t wgs = tiles * splits;
+      const int steps = (kblocks + splits - 1) / splits;
+      const double round = wgs > kCus && f.step2 > 0 ? ((wgs + 2 * kCus - 1) / (2 * kCus)) * f.step2 : ((wgs + kCus - 1) / kCus) * f.step;
+      const double cost = kLaunch + round * steps + (splits > 1 ? f.join + splits * f.more : 0);
+      if (best.cost == 0 || cost < best.cost) best = TilePlan{kind, splits, 0, cost};
+    }
+  }
+  return best;
+}
+
+// Past whole rounds of 256 x 256 tiles the channels left over may take a second launch of smaller ones (2048 x 34816 x
+// 5120: 1088 tiles, 4.25 rounds).
+TilePlan plan_tiles(int M, int N, int kblocks) {
+  TilePlan best = plan_single(M, N, kblocks);
+  const TileFigures& f = kFigures[kBig];
+  const int mblocks = (M - 1) / f.tokens + 1;
+  const int64_t rounds = tiles_of(kBig, M, N) / kCus;
+  const int64_t main_n = rounds * kCus / mblocks * f.channels;
+  if (main_n > 0 && main_n < N) {
+    TilePlan tail = plan_single(M, N - (int)main_n, kblocks);
+    tail.cost += kLaunch + rounds * f.step * kblocks;
+    tail.main_n = (int)main_n;
+    if (tail.cost < best.cost) best = tail;
+  }
+  return best;
+}
+
 template <int LAYOUT>
-int launch_w8a8(const Fp8Args& a, hipStream_t s) {
-  auto blocks = [&](int channels, int tokens) {
-    return (int64_t)((a.N + channels - 1) / channels) * ((a.M + tokens - 1) / tokens);
-  };
-  if (a.M > 128 && blocks(256, 256) >= 200) return launch_tile<LAYOUT, BigTile, 2, 2>(a, s);
-  if (a.M > 64 && blocks(128, 128) >= 200) return launch_tile<LAYOUT, MidTile, 2, 2>(a, s);
-  return launch_tile<LAYOUT, SmallTile, 1, 2>(a, s);
+int launch_kind(const Fp8Args& a, int kind, hipStream_t s) {
+  switch (kind) {
+    case kBig: return launch_tile<LAYOUT, BigTile, 2, 2>(a, s);
+    case kMid: return launch_tile<LAYOUT, MidTile, 2, 2>(a, s);
+    case kSmall: return launch_tile<LAYOUT, SmallTile, 1, 2>(a, s);
+    default: return launch_tile<LAYOUT, TinyTile, 1, 2>(a, s);
+  }
+}
+
+template <int LAYOUT>
+int launch_w8a8(Fp8Args a, const TilePlan& p, hipStream_t s) {
+  if (p.main_n > 0) {
+    Fp8Args m = a;
+    m.N = p.main_n;
+    m.ntiles = p.main_n / kTileN;
+    m.splits = 1;
+    const int st = launch_kind<LAYOUT>(m, kBig, s);
+    if (st != QF_OK) return st;
+    // the channels from main_n (a multiple of 256) on
+    a.w += LAYOUT == QF_LAYOUT_TILED ? (int64_t)m.ntiles * a.ksteps * 1024 : (int64_t)p.main_n * a.ldw;
+    a.scale += (int64_t)(p.main_n / kBlock) * a.kblocks;
+    if (a.bias != nullptr) a.bias += p.main_n;
+    a.y = static_cast<uint8_t*>(a.y) + (int64_t)p.main_n * (a.out_f32 ? 4 : 2);
+    a.N -= p.main_n;
+    a.ntiles -= m.ntiles;
+  }
+  a.splits = p.splits;
+  return launch_kind<LAYOUT>(a, p.kind, s);
 }
 
 int check_product(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, int layout, const float* scale,
@@ -790,16 +920,21 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct W8a8Plan {
   int m_pad, kblocks;
-  size_t scales, image, total;  // offsets
+  TilePlan tiles;
+  int64_t n_tiles;
+  size_t image, counters, partial, total;  // offsets in the workspace; the token scales first
 };
 
 int plan_w8a8(int M, int N, int K, W8a8Plan* p) {
   if (M < 1 || N < 1 || K < 1 || K % kStepK || M > 0x7fffffff - 255) return QF_ERR_UNSUPPORTED;
   p->kblocks = (K + kBlock - 1) / kBlock;
   p->m_pad = (M + kTokenPad - 1) / kTokenPad * kTokenPad;
-  p->scales = 0;
+  p->tiles = plan_tiles(M, N, p->kblocks);
+  p->n_tiles = p->tiles.splits > 1 ? tiles_of(p->tiles.kind, M, N - p->tiles.main_n) : 0;
   p->image = round256((size_t)p->kblocks * p->m_pad * 4);
-  p->total = p->image + (size_t)((M + 15) / 16) * 16 * p->kblocks * kBlock;
+  p->counters = p->image + round256((size_t)((M + 15) / 16) * 16 * p->kblocks * kBlock);
+  p->partial = p->counters + round256((size_t)p->n_tiles * 4);
+  p->total = p->partial + (size_t)p->n_tiles * p->tiles.splits * kFigures[p->tiles.kind].channels * kFigures[p->tiles.kind].tokens * 4;
   return QF_OK;
 }
 
@@ -852,7 +987,7 @@ int qf_quantize_tokens_fp8(const uint16_t* x, int64_t ldx, int M, int K, uint8_t
     return QF_ERR_UNSUPPORTED;
   const int kblocks = (K + kBlock - 1) / kBlock;
   if (kblocks > 65535 * kQuantBlocks) return QF_ERR_UNSUPPORTED;
-  const QuantArgs q = {x, ldx, xq, ldq, s_a, 0, M, K / kStepK, kblocks};
+  const QuantArgs q = {x, ldx, xq, ldq, s_a, 0, M, K / kStepK, kblocks, nullptr, 0};
   hipLaunchKernelGGL(quantize_tokens_fp8_kernel<false>, dim3((unsigned)((M + 15) / 16), (unsigned)((kblocks + kQuantBlocks - 1) / kQuantBlocks)),
                      dim3(256), 0, static_cast<hipStream_t>(stream), q);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
@@ -876,15 +1011,17 @@ int qf_fp8_w8a8_linear(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t
   Fp8Args a;
   fill(a, x, ldx, w, ldw, scale, bias, y, ldy, out_dtype, M, N, K);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.s_tok = reinterpret_cast<const float*>(ws + p.scales);
+  a.s_tok = reinterpret_cast<const float*>(ws);
   a.xt = ws + p.image;
   a.m_pad = p.m_pad;
+  a.counters = reinterpret_cast<unsigned*>(ws + p.counters);
+  a.partial = reinterpret_cast<uint64_t*>(ws + p.partial);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const QuantArgs q = {x, ldx, ws + p.image, 0, reinterpret_cast<float*>(ws + p.scales), p.m_pad, M, a.ksteps, a.kblocks};
+  const QuantArgs q = {x, ldx, ws + p.image, 0, reinterpret_cast<float*>(ws), p.m_pad, M, a.ksteps, a.kblocks, a.counters, (int)p.n_tiles};
   hipLaunchKernelGGL(quantize_tokens_fp8_kernel<true>, dim3((unsigned)((M + 15) / 16), (unsigned)((a.kblocks + kQuantBlocks - 1) / kQuantBlocks)),
                      dim3(256), 0, s, q);
   if (hipGetLastError() != hipSuccess) return QF_ERR_HIP;
-  return layout == QF_LAYOUT_TILED ? launch_w8a8<QF_LAYOUT_TILED>(a, s) : launch_w8a8<QF_LAYOUT_ROWMAJOR>(a, s);
+  return layout == QF_LAYOUT_TILED ? launch_w8a8<QF_LAYOUT_TILED>(a, p.tiles, s) : launch_w8a8<QF_LAYOUT_ROWMAJOR>(a, p.tiles, s);
 }
 
 }  // extern "C"
