@@ -530,7 +530,7 @@ fp8_tile_kernel(const Fp8Args a) {
   // row's matrix instructions; each weight fragment is read a row ahead, the next stage's first ones ahead of the last row.
   // No branch in a stage: the compiler would move additions across it and keep every product alive.
   // The copies of the stage that refills the slot of stage s - 1 go out between the rows of stage s.
-  constexpr int per_row = (T::own + FA - 1) / (FA - 1);  // pieces: own + 1 over FA - 1 rows
+  constexpr int per_row = S == 2 ? 2 : (T::own + FA - 1) / (FA - 1);  // pieces: own + 1 over FA - 1 rows; early with one stage ahead
   f32x4_t t[FB];
 #pragma unroll
   for (int j = 0; j < FB; ++j) t[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
