@@ -6,6 +6,8 @@
 //
 // A block's products meet in an MFMA accumulator that starts at zero, and the scaled block is added to the running fp32
 // sum with one multiply-add a value.
+#include <type_traits>
+
 #include "qf_block_common.h"
 
 namespace qfb {
@@ -191,7 +193,7 @@ fp8_decode_kernel(const Fp8Args a) {
       for (int p = 0; p < S; ++p) load(0, p);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (XL > 0) wait_vmcnt<2 * S>();  // x, ahead of the weights
-      for (int t = 0; t < nt; ++t) {
+      auto tile = [&](int t, auto reload) {
         if (t == 0 || (t0 + t) % (kBlock / kTileN) == 0) scales(t);
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -201,10 +203,12 @@ fp8_decode_kernel(const Fp8Args a) {
             x_of(p, x);
             acc += block_product(w[p], x, whole(p)) * sc[p];
           }
-          load(min(t + 1, nt - 1), p);
+          if constexpr (decltype(reload)::value) load(t + 1, p);
         }
         part[(t * W + v) * kWave + lane] = acc;
-      }
+      };
+      for (int t = 0; t + 1 < nt; ++t) tile(t, std::true_type());
+      tile(nt - 1, std::false_type());
     } else {
       // The copy cursor: block cp of tile ct, into slot cslot.  Past the last block it goes round the last tile again
       // (in-bounds re-reads into slots that are read no more), so that every copy is made and counted.
