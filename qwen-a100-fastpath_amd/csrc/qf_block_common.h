@@ -138,14 +138,15 @@ __device__ __forceinline__ void ring_barrier() {
   asm volatile("" : : : "memory");
 }
 
-// A block of K of one weight tile times its token fragments, from zero.
+// A block of K of one weight tile times its token fragments, from zero.  `second` (the block has its second half) is the same
+// in all lanes; matrix instructions run whatever the lane mask is, so the branch has to be a scalar one.
 __device__ __forceinline__ f32x4_t block_product(const u32x4_t (&w)[2], const u32x4_t (&x)[2][2], bool second) {
   f32x4_t blk = {0.f, 0.f, 0.f, 0.f};
   bf16x8_t lo, hi;
   widen16(w[0], lo, hi);
   blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, __builtin_bit_cast(bf16x8_t, x[0][0]), blk, 0, 0, 0);
   blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, __builtin_bit_cast(bf16x8_t, x[0][1]), blk, 0, 0, 0);
-  if (second) {
+  if (__builtin_amdgcn_readfirstlane(second)) {
     widen16(w[1], lo, hi);
     blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, __builtin_bit_cast(bf16x8_t, x[1][0]), blk, 0, 0, 0);
     blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, __builtin_bit_cast(bf16x8_t, x[1][1]), blk, 0, 0, 0);

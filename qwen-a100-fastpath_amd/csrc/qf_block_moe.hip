@@ -4,14 +4,21 @@
 //   a_e = silu(Wgate_e x) * (Wup_e x),   y[t] = sum over the chosen experts e of c[t, e] * W2_e a_e
 //
 // 1. moe_up_kernel: every workgroup works the routing out for itself (a few thousand cycles, no launch and no trip through
-//    memory between), then takes (chosen expert, 16 gate rows with their 16 up rows) items in turn; workgroup 0
-//    leaves the routing for the second launch.
-// 2. moe_down_kernel: a workgroup owns 16 output channels; its wavefronts share out the (expert, block of I) units, the
-//    columns of the accumulator are the tokens, and a unit is weighed by its block's scale times c[t, e].
+//    memory between), then streams a run of (chosen expert, 16 gate rows with their 16 up rows) items, the wavefronts sharing
+//    out the blocks of H; workgroup 0 leaves the routing for the second launch.
+// 2. moe_down_kernel: a workgroup owns 32 output channels and a part of the (expert, block of I) units, its wavefronts share
+//    these out; the columns of the accumulator are the tokens, and a unit is weighed by its block's scale times c[t, e].  The
+//    last of a channel group's workgroups to arrive adds their sums, in split order.
 // An expert's weights are read once for all its tokens.  Products are exact (weights widened to bf16 in registers), sums
 // fp32 in a fixed order.  Between the launches an activation is the sum of two bf16 numbers (16 bits of it are kept): one
 // bf16 alone put 2^-9 of noise into every a_e, half as much again as the output's own rounding (2.6e-3 against 1.7e-3 from
 // the exact result); the second product costs no weight bytes.  Bound by the memory rate over the chosen experts' weights.
+//
+// Measured, H 2048, I 768, 8 experts a token: 1 token (38 MB of weights) 10.8 + 7.1 us; 16 tokens of 128 experts (about 390
+// MB) 48 + 28 us, 5.2 TB/s.  The second launch took 61 us with 16 output channels a workgroup, 16 wavefronts and all units
+// (the activations' 1 KiB a token and unit, read again for every 16 channels, were the larger part of its loads); with 32
+// channels and the units split it is 28 with 8 wavefronts, 32 with 6, 30 with 4 and two workgroups a CU, 28 with 48 channels
+// (8 against 7 at one token) and 38 with 64.
 #include "qf_block_common.h"
 
 namespace qfb {
@@ -21,17 +28,16 @@ constexpr int kStepK = 64;
 constexpr int kBlock = QF_FP8_BLOCK;
 constexpr int kMaxT = QF_FP8_MAX_DECODE_M;
 constexpr int kMaxPairs = kMaxT * QF_MOE_MAX_TOP_K;          // (token, chosen expert) pairs, so chosen experts too
-constexpr int kPerLane = QF_MOE_MAX_EXPERTS / kWave;         // experts a lane in the routing
-constexpr int kMoeWaves = 8;
-constexpr int kDownWaves = 16;
-constexpr int kUpDepth = 2;    // blocks of H a wavefront requests ahead
-constexpr int kDownDepth = 3;  // units a wavefront requests ahead; odd: the activations' two buffers alternate with the ring
-static_assert(kDownDepth % 2 == 1, "an even ring");
+constexpr int kUpWaves = 8;
+constexpr int kDownGrid = 256;  // workgroups of the second launch where it splits: one a CU
+constexpr int kDownWaves = 8;
+constexpr int kDownTiles = 2;  // tiles of 16 output channels a workgroup
 
 // What the first launch leaves for the second.
 struct Routing {
   int active;                       // chosen experts
   int pad[3];
+  unsigned arrivals[kDownGrid / 2];  // of the second launch's splits, a group of tiles each; zeroed by the first
   uint16_t expert[kMaxPairs];       // in ascending order
   int16_t pair[kMaxPairs][kMaxT];   // row of a_e of (chosen expert, token), -1: not routed
   float weight[kMaxPairs][kMaxT];   // c, 0 where not routed
@@ -50,6 +56,8 @@ struct MoeArgs {
   uint16_t* y;
   int64_t ldy;
   Routing* routing;
+  uint64_t* partial;  // [split][tile][2][64 lanes]
+  int splits;
   uint16_t* a;  // [pairs][2][I]: the activations, each as the sum of two bf16 numbers
   int T, E, k, H, I, renormalize;
   int h_steps, h_blocks, i_steps, i_blocks;
@@ -76,7 +84,8 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return k == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// The routing of all tokens into LDS (every thread of the workgroup; ends with a barrier).
+// The routing of all tokens into LDS (every thread of the workgroup; ends with a barrier), for up to 64 kPerLane experts.
+template <int kPerLane>
 __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -171,16 +180,18 @@ __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kMoeWaves* kWave) __attribute__((amdgpu_waves_per_eu(4))) moe_up_kernel(const MoeArgs a) {
+template <int kPerLane>
+__global__ void __launch_bounds__(kUpWaves* kWave) __attribute__((amdgpu_waves_per_eu(4))) moe_up_kernel(const MoeArgs a) {
   __shared__ RoutingLds s;
-  __shared__ f32x4_t part[2][kMoeWaves][2][kWave];
+  __shared__ f32x4_t part[2][kUpWaves][2][kWave];
   const int lane = threadIdx.x & (kWave - 1);
   const int v = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, r = lane & 15;
-  route(a, s);
+  route<kPerLane>(a, s);
   if (blockIdx.x == 0) {
     const int active = s.active;
     if (threadIdx.x == 0) a.routing->active = active;
+    if (threadIdx.x < kDownGrid / 2) a.routing->arrivals[threadIdx.x] = 0;
     for (int i = threadIdx.x; i < active; i += blockDim.x) a.routing->expert[i] = s.expert[i];
     for (int i = threadIdx.x; i < active * kMaxT; i += blockDim.x) {
       const int at = i / kMaxT, t = i % kMaxT, e = s.expert[at];
@@ -192,20 +203,21 @@ __global__ void __launch_bounds__(kMoeWaves* kWave) __attribute__((amdgpu_waves_
       a.routing->pair[at][t] = in ? (int16_t)(s.first[at] + __builtin_popcount(s.tokens[e] & ((1u << t) - 1))) : (int16_t)-1;
     }
   }
-  // this workgroup's run of (chosen expert, 16 gate rows and their up rows) items, as one stream of blocks of H
+  // This workgroup's run of (chosen expert, 16 gate rows and their up rows) items, as one stream of chunks of two blocks of
+  // H a wavefront; a chunk's registers are loaded again for the next one as soon as they are multiplied.  (A wavefront without
+  // a block in a chunk reads one line and multiplies nothing.)
   const int row_tiles = a.I / kTileN;
   const int items = __builtin_amdgcn_readfirstlane(s.active) * row_tiles;
   const int first_item = (int)((int64_t)blockIdx.x * items / gridDim.x);
   const int n_items = (int)((int64_t)(blockIdx.x + 1) * items / gridDim.x) - first_item;
-  const int steps = (a.h_blocks - v + kMoeWaves - 1) / kMoeWaves;  // of this wavefront in an item, maybe none
-  const int total = n_items * steps;
+  const int chunks = (a.h_blocks + 2 * kUpWaves - 1) / (2 * kUpWaves);  // of an item
+  if (n_items == 0) return;
   struct Step {
     u32x4_t gate[2], up[2], x[2][2];
     float s_gate, s_up;
   };
-  Step buf[kUpDepth + 1];
-  const uint32_t w_lane = (uint32_t)lane * 16;
-  int pi = first_item, pj = 0;  // the next request
+  Step buf[2];
+  int pi = first_item, pj = 0;  // the next chunk to load
   const uint8_t* p_gate;
   const float* p_scale;
   uint32_t x_lane;
@@ -218,48 +230,49 @@ __global__ void __launch_bounds__(kMoeWaves* kWave) __attribute__((amdgpu_waves_
     p_gate = a.w13 + (e * 2 * row_tiles + j) * a.h_steps * (kWave * 16);
     p_scale = a.s13 + (e * 2 * a.i_blocks + j * kTileN / kBlock) * a.h_blocks;
   };
-  auto load = [&](Step& b) {
-    const int kb = v + pj * kMoeWaves;
+  auto block = [&](int j, int p) { return v + (2 * j + p) * kUpWaves; };
+  auto load = [&](int j, int p, Step& b) {
+    const bool in = block(j, p) < a.h_blocks;
+    const int kb = in ? block(j, p) : 0;
     const int half = 2 * kb + 1 < a.h_steps ? 1 : 0;  // a last half block: its first half again, not used
-    const uint8_t* p = p_gate + (int64_t)kb * 2048;
-    const uint8_t* q = p + (int64_t)row_tiles * a.h_steps * (kWave * 16);
-    b.gate[0] = load_once(p + w_lane);
-    b.gate[1] = load_once(p + half * 1024 + w_lane);
+    const uint32_t w_lane = in ? (uint32_t)lane * 16 : 0u, x_at = in ? x_lane : 0u;
+    const uint8_t* w = p_gate + (int64_t)kb * 2048;
+    const uint8_t* q = w + (int64_t)row_tiles * a.h_steps * (kWave * 16);
+    b.gate[0] = load_once(w + w_lane);
+    b.gate[1] = load_once(w + half * 1024 + w_lane);
     b.up[0] = load_once(q + w_lane);
     b.up[1] = load_once(q + half * 1024 + w_lane);
     const uint8_t* xp = reinterpret_cast<const uint8_t*>(a.x + (int64_t)kb * kBlock);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const u32x4_t* c = reinterpret_cast<const u32x4_t*>(xp + (h ? half * 2 * kStepK : 0) + x_lane);
+      const u32x4_t* c = reinterpret_cast<const u32x4_t*>(xp + (h ? half * 2 * kStepK : 0) + x_at);
       b.x[h][0] = c[0];
       b.x[h][1] = c[1];
     }
     b.s_gate = p_scale[kb];
     b.s_up = p_scale[(int64_t)a.i_blocks * a.h_blocks + kb];
-    if (++pj == steps) {
-      if (pi + 1 < first_item + n_items) {
-        enter(++pi);
-        pj = 0;
-      } else {
-        pj = steps - 1;
-      }
+  };
+  auto advance = [&]() {
+    if (++pj == chunks) {
+      pj = 0;
+      enter(++pi);
     }
   };
   // The wavefronts' partial tiles meet in LDS (two buffers, one barrier an item); one wavefront, another one each time, adds
   // them in wavefront order while the others stream on.
   f32x4_t acc_gate = {0.f, 0.f, 0.f, 0.f}, acc_up = acc_gate;
   auto leave = [&](int i) {
-    f32x4_t(&slot)[kMoeWaves][2][kWave] = part[i & 1];
+    f32x4_t(&slot)[kUpWaves][2][kWave] = part[i & 1];
     slot[v][0][lane] = acc_gate;
     slot[v][1][lane] = acc_up;
     acc_gate = acc_up = f32x4_t{0.f, 0.f, 0.f, 0.f};
     ring_barrier();
-    if (v != i % kMoeWaves) return;
+    if (v != i % kUpWaves) return;
     const int item = first_item + i, at = item / row_tiles, j = item - at * row_tiles;
     const int first = s.first[at];
     if (r >= s.first[at + 1] - first) return;
     f32x4_t gate = slot[0][0][lane], up = slot[0][1][lane];
-    for (int u = 1; u < kMoeWaves; ++u) {
+    for (int u = 1; u < kUpWaves; ++u) {
       gate += slot[u][0][lane];
       up += slot[u][1][lane];
     }
@@ -275,43 +288,49 @@ __global__ void __launch_bounds__(kMoeWaves* kWave) __attribute__((amdgpu_waves_
     *reinterpret_cast<u32x2_t*>(row) = u32x2_t{pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3])};
     *reinterpret_cast<u32x2_t*>(row + a.I) = u32x2_t{pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3])};
   };
-  if (n_items == 0) return;
-  if (steps == 0) {  // fewer blocks of H than wavefronts: this one has only its place in the sums
-    for (int i = 0; i < n_items; ++i) leave(i);
-    return;
-  }
   enter(pi);
-#pragma unroll
-  for (int d = 0; d < kUpDepth; ++d) load(buf[d]);
+  load(0, 0, buf[0]);
+  load(0, 1, buf[1]);
   int ci = 0, cj = 0;
-  for (int base = 0; base < total; base += kUpDepth + 1) {
+  const int total = n_items * chunks;
+  for (int n = 0; n + 1 < total; ++n) {
+    advance();
 #pragma unroll
-    for (int d = 0; d <= kUpDepth; ++d) {
-      load(buf[(d + kUpDepth) % (kUpDepth + 1)]);
-      __builtin_amdgcn_sched_barrier(0);  // the requests go out ahead of this step's math
-      if (base + d < total) {             // uniform
-        const Step& b = buf[d];
-        const bool second = 2 * (v + cj * kMoeWaves) + 1 < a.h_steps;
-        acc_gate += block_product(b.gate, b.x, second) * b.s_gate;
-        acc_up += block_product(b.up, b.x, second) * b.s_up;
-        if (++cj == steps) {
-          leave(ci++);
-          cj = 0;
-        }
+    for (int p = 0; p < 2; ++p) {
+      if (block(cj, p) < a.h_blocks) {  // uniform
+        const bool second = 2 * block(cj, p) + 1 < a.h_steps;
+        acc_gate += block_product(buf[p].gate, buf[p].x, second) * buf[p].s_gate;
+        acc_up += block_product(buf[p].up, buf[p].x, second) * buf[p].s_up;
       }
+      load(pj, p, buf[p]);
+    }
+    if (++cj == chunks) {
+      leave(ci++);
+      cj = 0;
     }
   }
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    if (block(cj, p) < a.h_blocks) {
+      const bool second = 2 * block(cj, p) + 1 < a.h_steps;
+      acc_gate += block_product(buf[p].gate, buf[p].x, second) * buf[p].s_gate;
+      acc_up += block_product(buf[p].up, buf[p].x, second) * buf[p].s_up;
+    }
+  }
+  leave(ci);
 }
 
+// The grid is (groups of kDownTiles tiles, splits of the units).
 __global__ void __launch_bounds__(kDownWaves* kWave) moe_down_kernel(const MoeArgs a) {
   __shared__ int16_t pair[kMaxPairs][kMaxT];
   __shared__ float weight[kMaxPairs][kMaxT];
   __shared__ uint16_t expert[kMaxPairs];
-  __shared__ f32x4_t part[kDownWaves][kWave];
+  __shared__ f32x4_t part[kDownWaves][kDownTiles][kWave];
+  __shared__ int last_arrival;
   const int lane = threadIdx.x & (kWave - 1);
   const int v = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, r = lane & 15;
-  const int nt = blockIdx.x;
+  const int h_tiles = a.H / kTileN, nt = blockIdx.x * kDownTiles;
   const int active = a.routing->active;
   for (int i = threadIdx.x; i < active * kMaxT; i += blockDim.x) {
     (&pair[0][0])[i] = (&a.routing->pair[0][0])[i];
@@ -319,84 +338,126 @@ __global__ void __launch_bounds__(kDownWaves* kWave) moe_down_kernel(const MoeAr
   }
   for (int i = threadIdx.x; i < active; i += blockDim.x) expert[i] = a.routing->expert[i];
   __syncthreads();
-  // (chosen expert, block of I) units, interleaved over the wavefronts; weights kDownDepth units ahead, activations one
+  // this split's (chosen expert, block of I) units, interleaved over the wavefronts, two of a wavefront's in flight
   const int units = active * a.i_blocks;
-  const int total = units > v ? (units - v + kDownWaves - 1) / kDownWaves : 0;
-  const int h_tiles = a.H / kTileN;
-  const int64_t h_blocks = a.h_blocks;
-  const uint32_t w_lane = (uint32_t)lane * 16;
-  struct Weights {
-    u32x4_t w[2];
-    float s;
+  const int u0 = (int)((int64_t)blockIdx.y * units / a.splits), u1 = (int)((int64_t)(blockIdx.y + 1) * units / a.splits);
+  const int total = u1 - u0 > v ? (u1 - u0 - v + kDownWaves - 1) / kDownWaves : 0;
+  struct Unit {
+    u32x4_t w[kDownTiles][2], hi[2][2], lo[2][2];
+    float s[kDownTiles];
+    bool in, second;
   };
-  struct Acts {
-    u32x4_t hi[2][2], lo[2][2];
-    float c;
-    bool in;
-  };
-  Weights wb[kDownDepth + 1];
-  Acts xb[2];
-  auto load_w = [&](int i, Weights& b) {
-    const int u = v + min(i, total - 1) * kDownWaves;
+  Unit buf[2];
+  auto load = [&](int i, Unit& b) {
+    const bool some = i < total;
+    const int u = some ? u0 + v + i * kDownWaves : u0 + v;
     const int at = u / a.i_blocks, kb = u - at * a.i_blocks;
     const int64_t e = __builtin_amdgcn_readfirstlane(expert[at]);
-    const int half = 2 * kb + 1 < a.i_steps ? 1 : 0;
-    const uint8_t* p = a.w2 + ((e * h_tiles + nt) * a.i_steps + 2 * kb) * (kWave * 16);
-    b.w[0] = load_once(p + w_lane);
-    b.w[1] = load_once(p + half * 1024 + w_lane);
-    b.s = a.s2[(e * h_blocks + nt * kTileN / kBlock) * a.i_blocks + kb];
-  };
-  auto load_x = [&](int i, Acts& b) {
-    const int u = v + min(i, total - 1) * kDownWaves;
-    const int at = u / a.i_blocks, kb = u - at * a.i_blocks;
-    const int half = 2 * kb + 1 < a.i_steps ? 1 : 0;
-    const int p = pair[at][r];
-    b.c = weight[at][r];
+    b.second = 2 * kb + 1 < a.i_steps;
+    const int half = b.second ? 1 : 0;
+    const uint32_t w_lane = some ? (uint32_t)lane * 16 : 0u;
+    const int p = some ? pair[at][r] : -1;
     b.in = p >= 0;
+    const float c = weight[at][r];
+#pragma unroll
+    for (int t = 0; t < kDownTiles; ++t) {
+      const int tile = min(nt + t, h_tiles - 1);
+      const uint8_t* q = a.w2 + ((e * h_tiles + tile) * a.i_steps + 2 * kb) * (kWave * 16);
+      b.w[t][0] = load_once(q + w_lane);
+      b.w[t][1] = load_once(q + half * 1024 + w_lane);
+      b.s[t] = a.s2[(e * a.h_blocks + tile * kTileN / kBlock) * a.i_blocks + kb] * c;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        b.hi[h][q] = b.lo[h][q] = u32x4_t{0u, 0u, 0u, 0u};  // a token that is not routed here: zeros, whatever `a` holds
-        if (b.in) {
-          const uint16_t* c = a.a + (int64_t)p * 2 * a.I + kb * kBlock + (h ? half * kStepK : 0) + 16 * g + 8 * q;
-          b.hi[h][q] = *reinterpret_cast<const u32x4_t*>(c);
-          b.lo[h][q] = *reinterpret_cast<const u32x4_t*>(c + a.I);
+      for (int q = 0; q < 2; ++q) b.hi[h][q] = b.lo[h][q] = u32x4_t{0u, 0u, 0u, 0u};
+    if (b.in) {  // a token that is not routed here: zeros, whatever `a` holds
+      const uint16_t* c = a.a + (int64_t)p * 2 * a.I + kb * kBlock + 16 * g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          b.hi[h][q] = *reinterpret_cast<const u32x4_t*>(c + (h ? half * kStepK : 0) + 8 * q);
+          b.lo[h][q] = *reinterpret_cast<const u32x4_t*>(c + a.I + (h ? half * kStepK : 0) + 8 * q);
         }
-      }
+    }
   };
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  f32x4_t acc[kDownTiles];
+#pragma unroll
+  for (int t = 0; t < kDownTiles; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto use = [&](const Unit& b) {
+#pragma unroll
+    for (int t = 0; t < kDownTiles; ++t) {
+      const f32x4_t add = (block_product(b.w[t], b.hi, b.second) + block_product(b.w[t], b.lo, b.second)) * b.s[t];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] += b.in ? add[e] : 0.f;  // NaN weights of an expert reach its own tokens only
+    }
+  };
   if (total > 0) {
+    load(0, buf[0]);
+    load(1, buf[1]);
+    int i = 0;
+    for (; i + 2 < total; i += 2) {
+      use(buf[0]);
+      load(i + 2, buf[0]);
+      use(buf[1]);
+      load(i + 3, buf[1]);
+    }
+    use(buf[0]);
+    if (i + 1 < total) use(buf[1]);
+  }
 #pragma unroll
-    for (int d = 0; d < kDownDepth; ++d) load_w(d, wb[d]);
-    load_x(0, xb[0]);
-    for (int base = 0; base < total; base += kDownDepth + 1) {
+  for (int t = 0; t < kDownTiles; ++t) part[v][t][lane] = acc[t];
+  __syncthreads();
+  auto store = [&](int tile, f32x4_t sum) {
+    *reinterpret_cast<u32x2_t*>(a.y + (int64_t)r * a.ldy + tile * kTileN + 4 * g) =
+        u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
+  };
+  const bool mine = v < kDownTiles && nt + v < h_tiles && r < a.T;  // wavefront t adds tile t up
+  auto slot = [&](int split) { return a.partial + ((int64_t)split * h_tiles + nt + v) * 2 * kWave + lane; };
+  if (mine) {
+    f32x4_t sum = part[0][v][lane];
+    for (int u = 1; u < kDownWaves; ++u) sum += part[u][v][lane];
+    if (a.splits == 1) {
+      store(nt + v, sum);
+    } else {
 #pragma unroll
-      for (int d = 0; d <= kDownDepth; ++d) {
-        const int i = base + d;
-        load_w(i + kDownDepth, wb[(d + kDownDepth) % (kDownDepth + 1)]);
-        load_x(i + 1, xb[(d + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (i < total) {  // uniform
-          const Weights& b = wb[d];
-          const Acts& x = xb[d & 1];
-          const bool second = 2 * ((v + i * kDownWaves) % a.i_blocks) + 1 < a.i_steps;
-          const f32x4_t add = (block_product(b.w, x.hi, second) + block_product(b.w, x.lo, second)) * (b.s * x.c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += x.in ? add[e] : 0.f;  // NaN weights of an expert reach its own tokens only
-        }
-      }
+      for (int h = 0; h < 2; ++h)
+        __hip_atomic_store(slot(blockIdx.y) + h * kWave, __builtin_bit_cast(uint64_t, f32x2_t{sum[2 * h], sum[2 * h + 1]}),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
-  part[v][lane] = acc;
+  if (a.splits == 1) return;
+  // The splits' sums are in device memory (device-scope stores, waited for) before the group's arrival is counted; the last
+  // one reads them with device-scope loads issued after its increment returned, and adds them in split order.
+  wait_vmcnt<0>();
   __syncthreads();
-  if (v == 0 && r < a.T) {
-    f32x4_t sum = part[0][lane];
-    for (int u = 1; u < kDownWaves; ++u) sum += part[u][lane];
-    *reinterpret_cast<u32x2_t*>(a.y + (int64_t)r * a.ldy + nt * kTileN + 4 * g) =
-        u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
+  if (threadIdx.x == 0)
+    last_arrival = __hip_atomic_fetch_add(&a.routing->arrivals[blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                   (unsigned)(a.splits - 1);
+  __syncthreads();
+  if (!last_arrival || !mine) return;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < a.splits; j += 4) {  // a batch's loads are all in flight at once
+    f32x2_t q[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        q[k][h] = __builtin_bit_cast(f32x2_t, __hip_atomic_load(slot(min(j + k, a.splits - 1)) + h * kWave, __ATOMIC_RELAXED,
+                                                                __HIP_MEMORY_SCOPE_AGENT));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x4_t p = {q[k][0].x, q[k][0].y, q[k][1].x, q[k][1].y};
+      if (j + k < a.splits) sum = j + k == 0 ? p : sum + p;
+    }
   }
+  store(nt + v, sum);
 }
+
+// Splits of the second launch: one workgroup a CU where the tile groups alone are fewer.
+int down_groups(int H) { return (H / kTileN + kDownTiles - 1) / kDownTiles; }
+int down_splits(int H) { return down_groups(H) <= kDownGrid / 2 ? kDownGrid / down_groups(H) : 1; }
 
 bool moe_sizes_ok(int T, int E, int top_k, int H, int I) {
   return T >= 1 && T <= kMaxT && E >= 1 && E <= QF_MOE_MAX_EXPERTS && top_k >= 1 && top_k <= QF_MOE_MAX_TOP_K &&
@@ -404,6 +465,7 @@ bool moe_sizes_ok(int T, int E, int top_k, int H, int I) {
 }
 
 constexpr size_t kRoutingBytes = (sizeof(Routing) + 255) / 256 * 256;
+size_t partial_bytes(int H) { return down_splits(H) > 1 ? (size_t)down_splits(H) * (H / kTileN) * 1024 : 0; }
 
 }  // namespace qfb
 
@@ -413,7 +475,7 @@ extern "C" {
 
 size_t qf_moe_few_workspace_bytes(int T, int E, int top_k, int H, int I) {
   if (!moe_sizes_ok(T, E, top_k, H, I)) return 0;
-  return kRoutingBytes + ((size_t)T * top_k * I * 4 + 255) / 256 * 256;
+  return kRoutingBytes + partial_bytes(H) + ((size_t)T * top_k * I * 4 + 255) / 256 * 256;
 }
 
 int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_t ldl, int logits_f32, const uint8_t* w13,
@@ -439,7 +501,9 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
   a.y = y;
   a.ldy = ldy;
   a.routing = static_cast<Routing*>(workspace);
-  a.a = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + kRoutingBytes);
+  a.partial = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + kRoutingBytes);
+  a.splits = down_splits(H);
+  a.a = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + kRoutingBytes + partial_bytes(H));
   a.T = T;
   a.E = E;
   a.k = top_k;
@@ -454,9 +518,11 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
   const int64_t chosen = (int64_t)T * top_k < E ? (int64_t)T * top_k : E;
   const int64_t items = chosen * (I / kTileN);
   const unsigned grid = (unsigned)(items < 512 ? items : 512);
-  hipLaunchKernelGGL(moe_up_kernel, dim3(grid), dim3(kMoeWaves * kWave), 0, s, a);
+  const auto up = E <= kWave ? &moe_up_kernel<1> : E <= 2 * kWave ? &moe_up_kernel<2> : E <= 4 * kWave ? &moe_up_kernel<4>
+                                                                                             : &moe_up_kernel<8>;
+  hipLaunchKernelGGL(up, dim3(grid), dim3(kUpWaves * kWave), 0, s, a);
   if (hipGetLastError() != hipSuccess) return QF_ERR_HIP;
-  hipLaunchKernelGGL(moe_down_kernel, dim3((unsigned)(H / kTileN)), dim3(kDownWaves * kWave), 0, s, a);
+  hipLaunchKernelGGL(moe_down_kernel, dim3((unsigned)down_groups(H), (unsigned)a.splits), dim3(kDownWaves * kWave), 0, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
 

@@ -99,6 +99,13 @@ def test_sizes(qf, T, E, k, Hd, I, renorm):
     _check(qf, T, E, k, Hd, I, renorm, F32 if renorm else BF16, seed=T + E)
 
 
+# output channels in one group of workgroups, in two splits, in none; an odd last tile; many units
+@pytest.mark.parametrize("T,E,k,Hd,I", [(2, 3, 2, 4096, 64), (2, 3, 2, 4160, 64), (3, 4, 2, 8192, 192), (16, 40, 8, 2688, 448),
+                                        (9, 20, 16, 64, 1344)])
+def test_splits_of_the_second_product(qf, T, E, k, Hd, I):
+    _check(qf, T, E, k, Hd, I, True, seed=Hd)
+
+
 def test_every_token_count(qf):
     g = H.gen(11)
     up, down = _layer(g, 12, 128, 128)
