@@ -72,25 +72,25 @@ def load() -> ctypes.CDLL:
     return L
 
 
-def same_gpu(*tensors) -> torch.device:
-    """The GPU that every tensor handed to the library lives on: a host pointer, or another device's, reaching a kernel
-    faults the device."""
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise TypeError(f"expected a GPU tensor, got one on {dev}")
-    for t in tensors[1:]:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}: all must be on one GPU")
-    return dev
+def same_gpu(first: torch.Tensor, *others) -> int:
+    """Index of the GPU that every tensor handed to the library lives on: a host pointer, or another device's, reaching a
+    kernel faults the device."""
+    if not first.is_cuda:
+        raise TypeError(f"expected a GPU tensor, got one on {first.device}")
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on {first.device} and {t.device}: all must be on one GPU")
+    return index
 
 
-def call(name: str, device: torch.device, *args) -> None:
-    """Run an entry point on torch's current stream of `device` (its last argument), whatever the current device is."""
+def call(name: str, index: int, *args) -> None:
+    """Run an entry point on torch's current stream of GPU `index` (its last argument), whatever the current device is."""
     fn = getattr(_lib or load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         raise QFError(rc, name)

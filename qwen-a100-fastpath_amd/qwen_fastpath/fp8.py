@@ -53,8 +53,8 @@ def quantize_tokens_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if K < 64 or K % 64:
         raise ValueError(f"K must be a multiple of 64, got {K}")
     x, ldx = _rows(x)
-    q = torch.empty((M, K), dtype=_FP8, device=dev)
-    s = torch.empty((M, -(-K // B.BLOCK)), dtype=_F32, device=dev)
+    q = x.new_empty((M, K), dtype=_FP8)
+    s = x.new_empty((M, -(-K // B.BLOCK)), dtype=_F32)
     if M:
         B.call("qf_quantize_tokens_fp8", dev, x.data_ptr(), ldx, M, K, q.data_ptr(), K, s.data_ptr())
     return q, s
@@ -110,7 +110,7 @@ def _product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Opti
             raise TypeError(f"bias must be bf16 [{N}], got {bias.dtype} {list(bias.shape)}")
         if not bias.is_contiguous():
             bias = bias.contiguous()
-    y = torch.empty((M, N), dtype=out_dtype, device=dev)
+    y = x.new_empty((M, N), dtype=out_dtype)
     if M == 0:
         return y
     x, ldx = _rows(x)
@@ -118,11 +118,11 @@ def _product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Opti
             y.data_ptr(), N, 0 if out_dtype is _BF16 else 1, M, N, K)
     if M <= B.MAX_DECODE_M if decode is None else decode:
         nbytes = B.load().qf_fp8_w8a16_workspace_bytes(M, N, K, layout)
-        ws = _workspace(dev, nbytes) if nbytes else None  # K splits' arrival counters: zero between calls
+        ws = _workspace(x.device, nbytes) if nbytes else None  # K splits' arrival counters: zero between calls
         B.call("qf_fp8_w8a16_gemm", dev, *args, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     else:
         nbytes = B.load().qf_fp8_w8a8_workspace_bytes(M, N, K)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the caching allocator's: one a call, capture-safe
+        ws = x.new_empty(nbytes, dtype=torch.uint8)  # the caching allocator's: one a call, capture-safe
         B.call("qf_fp8_w8a8_linear", dev, *args, ws.data_ptr(), nbytes)
     return y
 

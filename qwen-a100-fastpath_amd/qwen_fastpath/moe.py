@@ -55,7 +55,7 @@ def moe_few_tokens(x: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tens
         raise ValueError(f"s13 and s2 must be {[E, 2 * nb, kb]} and {[E, kb, nb]}, got {list(s13.shape)} and {list(s2.shape)}")
     if w13.data_ptr() % 16 or w2.data_ptr() % 16:
         raise ValueError("w13 and w2 must be 16-byte aligned")
-    y = torch.empty((T, H), dtype=_BF16, device=dev)
+    y = x.new_empty((T, H))
     if T == 0:
         return y
     if not s13.is_contiguous():
@@ -66,7 +66,7 @@ def moe_few_tokens(x: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tens
     if router_logits.stride(1) != 1 or (T > 1 and router_logits.stride(0) < E):
         router_logits = router_logits.clone(memory_format=torch.contiguous_format)
     nbytes = B.load().qf_moe_few_workspace_bytes(T, E, top_k, H, I)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the caching allocator's: one a call, capture-safe
+    ws = x.new_empty(nbytes, dtype=torch.uint8)  # the caching allocator's: one a call, capture-safe
     B.call("qf_moe_few_tokens", dev, x.data_ptr(), ldx, router_logits.data_ptr(),
            router_logits.stride(0) if T > 1 else E, router_logits.dtype is _F32, w13.data_ptr(), s13.data_ptr(),
            w2.data_ptr(), s2.data_ptr(), y.data_ptr(), H, T, E, top_k, H, I, bool(renormalize), ws.data_ptr(), nbytes)

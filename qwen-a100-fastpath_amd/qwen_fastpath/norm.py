@@ -17,7 +17,8 @@ _BF16, _F32 = torch.bfloat16, torch.float32
 
 def _fit(t: torch.Tensor, align: int) -> bool:
     """Rows the kernel can address: unit column stride, 16-byte aligned, a row stride that is a multiple of `align`."""
-    return t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or t.stride(0) % align == 0)
+    rows, unit = t.stride()
+    return unit == 1 and t.data_ptr() % 16 == 0 and (rows % align == 0 or t.shape[0] == 1)
 
 
 def _weight(w: Optional[torch.Tensor], N: int, name: str) -> Optional[torch.Tensor]:
@@ -32,7 +33,7 @@ def _weight(w: Optional[torch.Tensor], N: int, name: str) -> Optional[torch.Tens
 
 def _output(out: Optional[torch.Tensor], like: torch.Tensor, M: int, N: int, align: int, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty((M, N), dtype=like.dtype, device=like.device)
+        return torch.empty_like(like) if like.is_contiguous() else like.new_empty((M, N))
     if out.dtype != like.dtype or tuple(out.shape) != (M, N) or out.device != like.device or not _fit(out, align) or (
             M > 1 and out.stride(0) < N):
         raise ValueError(f"{name} must be a {like.dtype} [{M}, {N}] tensor on {like.device} with unit column stride, 16-byte "

@@ -114,7 +114,7 @@ _WS_MIN = 8 << 20
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     dev = device.index if device.index is not None else torch.cuda.current_device()
-    handle = torch.cuda.current_stream(device).cuda_stream
+    handle = torch._C._cuda_getCurrentRawStream(dev)
     if torch.cuda.is_current_stream_capturing():
         cid = L.capture_id(handle)
         entry = _capture_ws.get((dev, handle))
