@@ -66,6 +66,20 @@ def test_quantiser_bits(qf, M, K):
     assert torch.equal(q.cpu().view(torch.uint8) , qr.view(torch.uint8))
 
 
+def test_quantiser_rounds_as_the_division(qf):
+    """Every sign, exponent and significand against maxima of all kinds: bit for bit, signed zeros among them."""
+    g = H.gen(9)
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF16)
+    x = x[x.isfinite()][:65024].view(508, 128).clone()       # blocks of like magnitude
+    y = x.flatten()[torch.randperm(65024, generator=g)].view(508, 128)  # and of unlike
+    z = (H.rows(g, 508, 128).float() * 2.0 ** torch.randint(-126, 100, (508, 1), generator=g)).to(BF16)
+    x = torch.cat([x, y, z], 1)
+    q, s = qf.quantize_tokens_fp8(x.cuda())
+    qr, sr = H.quantize(x)
+    assert torch.equal(s.cpu(), sr)
+    assert torch.equal(q.cpu().view(torch.uint8), qr.view(torch.uint8))
+
+
 def test_quantiser_tiny_and_not_finite(qf):
     x = torch.zeros(4, 256)
     x[0, :8] = torch.tensor([1, -2, 3, -4, 5, 100, 333, 127.]) * 2.0 ** -133  # subnormal in bf16
