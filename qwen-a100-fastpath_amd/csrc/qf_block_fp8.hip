@@ -95,7 +95,7 @@ __device__ __forceinline__ int xcd_order(int i, int n) {
 // wavefront v then adds the W partials of tiles v, v + W, ... in wavefront order; with a K split the last workgroup of a run
 // adds the splits in split order.
 // ---------------------------------------------------------------------------------------------
-constexpr int kRowSlots = 3;
+constexpr int kRowSlots = 2;
 constexpr int kJoinBatch = 4;
 __host__ __device__ constexpr int decode_ring(int layout, int W) {
   return layout == QF_LAYOUT_TILED ? 0 : W * kRowSlots * 2048;

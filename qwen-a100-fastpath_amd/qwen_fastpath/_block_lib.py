@@ -6,6 +6,7 @@ library is missing, every GPU entry point raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -70,6 +71,12 @@ def load() -> ctypes.CDLL:
         raise ImportError(f"{LIB_PATH}: ABI version {v}, expected {ABI_VERSION}")
     _lib = L
     return L
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(name: str, *sizes: int) -> int:
+    """A call's workspace by its sizes (which settle it): asked of the library once."""
+    return getattr(load(), name)(*sizes)
 
 
 def same_gpu(first: torch.Tensor, *others) -> int:

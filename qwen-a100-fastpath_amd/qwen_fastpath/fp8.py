@@ -117,11 +117,11 @@ def _product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Opti
     args = (x.data_ptr(), ldx, w.data_ptr(), ldw, layout, w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
             y.data_ptr(), N, 0 if out_dtype is _BF16 else 1, M, N, K)
     if M <= B.MAX_DECODE_M if decode is None else decode:
-        nbytes = B.load().qf_fp8_w8a16_workspace_bytes(M, N, K, layout)
+        nbytes = B.workspace_bytes("qf_fp8_w8a16_workspace_bytes", M, N, K, layout)
         ws = _workspace(x.device, nbytes) if nbytes else None  # K splits' arrival counters: zero between calls
         B.call("qf_fp8_w8a16_gemm", dev, *args, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     else:
-        nbytes = B.load().qf_fp8_w8a8_workspace_bytes(M, N, K)
+        nbytes = B.workspace_bytes("qf_fp8_w8a8_workspace_bytes", M, N, K)
         ws = x.new_empty(nbytes, dtype=torch.uint8)  # the caching allocator's: one a call, capture-safe
         B.call("qf_fp8_w8a8_linear", dev, *args, ws.data_ptr(), nbytes)
     return y

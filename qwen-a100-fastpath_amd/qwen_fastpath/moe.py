@@ -65,7 +65,7 @@ def moe_few_tokens(x: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tens
     x, ldx = _rows(x)
     if router_logits.stride(1) != 1 or (T > 1 and router_logits.stride(0) < E):
         router_logits = router_logits.clone(memory_format=torch.contiguous_format)
-    nbytes = B.load().qf_moe_few_workspace_bytes(T, E, top_k, H, I)
+    nbytes = B.workspace_bytes("qf_moe_few_workspace_bytes", T, E, top_k, H, I)
     ws = x.new_empty(nbytes, dtype=torch.uint8)  # the caching allocator's: one a call, capture-safe
     B.call("qf_moe_few_tokens", dev, x.data_ptr(), ldx, router_logits.data_ptr(),
            router_logits.stride(0) if T > 1 else E, router_logits.dtype is _F32, w13.data_ptr(), s13.data_ptr(),
