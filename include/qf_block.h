@@ -34,6 +34,8 @@ extern "C" {
 #define QF_FP8_BLOCK 128
 /* Largest M of qf_fp8_w8a16_gemm and T of qf_moe_few_tokens. */
 #define QF_FP8_MAX_DECODE_M 16
+/* Longest K of qf_fp8_w8a8_linear. */
+#define QF_FP8_MAX_W8A8_K 262144
 /* Longest row of qf_block_norm_rows. */
 #define QF_BLOCK_NORM_MAX_N 32768
 /* Most experts, and experts a token, of qf_moe_few_tokens. */
@@ -49,7 +51,8 @@ int qf_block_abi_version(void);
 /* y[m, n] = sum over blocks of scale[n / 128, kb] * sum_{k in kb} x[m, k] * q[n, k] (+ bias[n]): x bf16 [M, K] (row
  * stride ldx), w e4m3, scale fp32 [ceil(N / 128), ceil(K / 128)] contiguous, bias bf16 [N] or NULL, y bf16 or fp32
  * [M, N] (row stride ldy).  1 <= M <= 16.  Products are exact, sums fp32, y is rounded once.  x and w 16-byte aligned,
- * ldx % 8 == 0, row-major ldw % 16 == 0, both at most 2^26, else QF_ERR_UNSUPPORTED. */
+ * ldx % 8 == 0, row-major ldw % 16 == 0, both at most 2^26, else QF_ERR_UNSUPPORTED.  (Where K is split, one arrival counter
+ * serves several tiles of 16 channels; QF_W8A16_COUNTER_BYTES of them reach past a million channels.) */
 int qf_fp8_w8a16_gemm(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, int layout, const float* scale,
                       const uint16_t* bias, void* y, int64_t ldy, int out_dtype, int M, int N, int K, void* workspace,
                       size_t workspace_bytes, void* stream);
@@ -70,7 +73,7 @@ int qf_quantize_tokens_fp8(const uint16_t* x, int64_t ldx, int M, int K, uint8_t
 size_t qf_fp8_w8a8_workspace_bytes(int M, int N, int K);
 
 /* y[m, n] = sum over blocks of s_a[m, kb] * scale[n / 128, kb] * sum_{k in kb} xq[m, k] * q[n, k] (+ bias[n]), with xq and
- * s_a those of qf_quantize_tokens_fp8.  Any M >= 1; the rest as qf_fp8_w8a16_gemm.  The workspace needs no clearing and is
+ * s_a those of qf_quantize_tokens_fp8.  1 <= M < 2^28, K <= QF_FP8_MAX_W8A8_K; the rest as qf_fp8_w8a16_gemm.  The workspace needs no clearing and is
  * free again when the last launch ends; calls that may run at the same time need distinct ones (16-byte aligned). */
 int qf_fp8_w8a8_linear(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, int layout, const float* scale,
                        const uint16_t* bias, void* y, int64_t ldy, int out_dtype, int M, int N, int K,

@@ -170,6 +170,9 @@ inline bool raise_lds(const void* fn, int bytes, std::atomic<uint64_t>& raised) 
   return true;
 }
 
+// A launch's threads along x: below 2^32.
+inline bool grid_fits(int64_t groups, int threads) { return groups * threads <= 0xffffffffll; }
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace qfb

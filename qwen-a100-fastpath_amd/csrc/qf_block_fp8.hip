@@ -433,8 +433,8 @@ struct Tile {
   static constexpr int stage = frags * 2048;
   static constexpr int slot = stage + waves * 256;
   static constexpr int lds = S * slot;
-  static constexpr int max_kblocks = (kMaxLds - lds) / (4 * WN);
-  static_assert(waves * FA * FB * 512 <= lds && max_kblocks >= 1024, "LDS");
+  static constexpr int max_kblocks = (kMaxLds - lds) / (4 * WN);  // the weight scales stand behind the ring
+  static_assert(waves * FA * FB * 512 <= lds && max_kblocks >= QF_FP8_MAX_W8A8_K / kBlock, "LDS");
 };
 
 template <int LAYOUT, typename T, int MINW, int MAXW>
@@ -721,7 +721,7 @@ int launch_tile(const Fp8Args& a, hipStream_t s) {
   if (!raise_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), kMaxLds, raised)) return QF_ERR_HIP;
   const int64_t grid = (int64_t)((a.N + T::channels - 1) / T::channels) * ((a.M + T::tokens - 1) / T::tokens) * a.splits;
   const int share = (a.kblocks + a.splits - 1) / a.splits;
-  if (grid > 0x7fffffff || share > T::max_kblocks) return QF_ERR_UNSUPPORTED;
+  if (!grid_fits(grid, T::waves * kWave)) return QF_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((fp8_tile_kernel<LAYOUT, T, MINW, MAXW>), dim3((unsigned)grid), dim3(T::waves * kWave),
                      T::lds + T::WN * share * 4, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
@@ -875,24 +875,24 @@ DecodePlan plan_decode(int layout, int M, int ntiles, int kblocks) {
     for (int splits = least; splits < least + 8 && splits <= kblocks; ++splits) {
       const int share = (kblocks + splits - 1) / splits;
       for (int waves : {kMaxWaves, kMaxWaves / 2}) {
-      int S = (share + waves - 1) / waves;
-      if (S == 4) S = 5;
-      if (S > most_blocks) continue;
-      const int W = (share + S - 1) / S;
-      const int fixed = decode_ring(layout, W) + W * S * xl * 1024;
-      const int room = ((int)kMaxLds - 1024 - fixed) / (W * 1024);
-      if (room < 1) continue;
-      const int slots = splits < kDecodeGrid ? kDecodeGrid / splits : 1;
-      const int run = (ntiles + slots - 1) / slots < room ? (ntiles + slots - 1) / slots : room;
-      const int64_t runs = (ntiles + run - 1) / run;
-      const int64_t rounds = (runs * splits + kDecodeGrid - 1) / kDecodeGrid;
-      const double kb = 0.128 * share * (16.0 * run + 2 * M);  // thousand bytes a workgroup
-      const double cost = rounds * (kb / 28 * (W < 12 ? 1.04 : 1) + (xl ? 0 : 0.3 * S)) + 3.5 * (rounds - 1) +
-                          (splits > 1 ? 3.0 + run * (0.25 + 0.06 * splits) : 0);
-      if (best.waves == 0 || cost < best_cost) {
-        best_cost = cost;
-        best = DecodePlan{W, (int)runs, splits, S, xl, (size_t)fixed + (size_t)run * W * 1024};
-      }
+        int S = (share + waves - 1) / waves;
+        if (S == 4) S = 5;
+        if (S > most_blocks) continue;
+        const int W = (share + S - 1) / S;
+        const int fixed = decode_ring(layout, W) + W * S * xl * 1024;
+        const int room = ((int)kMaxLds - 1024 - fixed) / (W * 1024);
+        if (room < 1) continue;
+        const int slots = splits < kDecodeGrid ? kDecodeGrid / splits : 1;
+        const int run = (ntiles + slots - 1) / slots < room ? (ntiles + slots - 1) / slots : room;
+        const int64_t runs = (ntiles + run - 1) / run;
+        const int64_t rounds = (runs * splits + kDecodeGrid - 1) / kDecodeGrid;
+        const double kb = 0.128 * share * (16.0 * run + 2 * M);  // thousand bytes a workgroup
+        const double cost = rounds * (kb / 28 * (W < 12 ? 1.04 : 1) + (xl ? 0 : 0.3 * S)) + 3.5 * (rounds - 1) +
+                            (splits > 1 ? 3.0 + run * (0.25 + 0.06 * splits) : 0);
+        if (best.waves == 0 || cost < best_cost) {
+          best_cost = cost;
+          best = DecodePlan{W, (int)runs, splits, S, xl, (size_t)fixed + (size_t)run * W * 1024};
+        }
       }
     }
   }
@@ -941,7 +941,9 @@ struct W8a8Plan {
 };
 
 int plan_w8a8(int M, int N, int K, W8a8Plan* p) {
-  if (M < 1 || N < 1 || K < 1 || K % kStepK || M > 0x7fffffff - 255) return QF_ERR_UNSUPPORTED;
+  if (M < 1 || N < 1 || K < 1 || K % kStepK || K > QF_FP8_MAX_W8A8_K || N > 0x7fffffff - 255 || M > 0x7fffffff - 255 ||
+      !grid_fits((M + 15) / 16, 256))
+    return QF_ERR_UNSUPPORTED;
   p->kblocks = (K + kBlock - 1) / kBlock;
   p->m_pad = (M + kTokenPad - 1) / kTokenPad * kTokenPad;
   p->tiles = plan_tiles(M, N, p->kblocks);
@@ -1001,7 +1003,7 @@ int qf_quantize_tokens_fp8(const uint16_t* x, int64_t ldx, int M, int K, uint8_t
   if (K % kStepK || ldx % 8 || ldq % 8 || !aligned16(x) || ((uintptr_t)xq & 7) || M > 0x7fffffff - 255)
     return QF_ERR_UNSUPPORTED;
   const int kblocks = (K + kBlock - 1) / kBlock;
-  if (kblocks > 65535 * kQuantBlocks) return QF_ERR_UNSUPPORTED;
+  if (kblocks > 65535 * kQuantBlocks || !grid_fits((M + 15) / 16, 256)) return QF_ERR_UNSUPPORTED;
   const QuantArgs q = {x, ldx, xq, ldq, s_a, 0, M, K / kStepK, kblocks, nullptr, 0};
   hipLaunchKernelGGL(quantize_tokens_fp8_kernel<false>, dim3((unsigned)((M + 15) / 16), (unsigned)((kblocks + kQuantBlocks - 1) / kQuantBlocks)),
                      dim3(256), 0, static_cast<hipStream_t>(stream), q);
@@ -1021,7 +1023,6 @@ int qf_fp8_w8a8_linear(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t
   W8a8Plan p;
   st = plan_w8a8(M, N, K, &p);
   if (st != QF_OK) return st;
-  if (p.kblocks > 65535 * kQuantBlocks) return QF_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < p.total || !aligned16(workspace)) return QF_ERR_WORKSPACE;
   Fp8Args a;
   fill(a, x, ldx, w, ldw, scale, bias, y, ldy, out_dtype, M, N, K);

@@ -35,7 +35,8 @@ __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
 }
 
-// Sum over a row's threads (their shares of the mean: the squares' sum itself may overflow where the mean does not): groups of L lanes, or (L = 0) the whole workgroup.
+// Sum over a row's threads (their shares of the mean: the squares' sum itself may overflow where the mean does not):
+// groups of L lanes, or (L = 0) the whole workgroup.
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float* exchange) {
   if constexpr (L > 0) return group_sum<L>(v);
@@ -159,12 +160,14 @@ __global__ void __launch_bounds__(L > 0 ? 256 : 1024) block_norm_kernel(const No
 }
 
 template <int L, int P>
-void launch_norm(bool wide, unsigned grid, unsigned threads, hipStream_t s, const NormArgs& a) {
+int launch_norm(bool wide, unsigned grid, unsigned threads, hipStream_t s, const NormArgs& a) {
+  if (!grid_fits(grid, (int)threads)) return QF_ERR_UNSUPPORTED;
   if (wide) {
     hipLaunchKernelGGL((block_norm_kernel<L, P, true>), dim3(grid), dim3(threads), 0, s, a);
   } else {
     hipLaunchKernelGGL((block_norm_kernel<L, P, false>), dim3(grid), dim3(threads), 0, s, a);
   }
+  return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
 
 }  // namespace qfb
@@ -211,20 +214,11 @@ extern "C" int qf_block_norm_rows(const uint16_t* x, int64_t ldx, const void* re
   a.inv_n = 1.f / (float)N;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool wide = residual_f32 != 0;
-  if (a.pieces <= 16) {
-    launch_norm<16, 1>(wide, (unsigned)((M + 15) / 16), 256, s, a);
-  } else if (a.pieces <= 64) {
-    launch_norm<64, 1>(wide, (unsigned)((M + 3) / 4), 256, s, a);
-  } else {
-    const int P = a.pieces <= 1024 ? 1 : a.pieces <= 2048 ? 2 : 4;
-    const unsigned threads = (unsigned)(((a.pieces + P - 1) / P + kWave - 1) / kWave * kWave);
-    if (P == 1) {
-      launch_norm<0, 1>(wide, (unsigned)M, threads, s, a);
-    } else if (P == 2) {
-      launch_norm<0, 2>(wide, (unsigned)M, threads, s, a);
-    } else {
-      launch_norm<0, 4>(wide, (unsigned)M, threads, s, a);
-    }
-  }
-  return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
+  if (a.pieces <= 16) return launch_norm<16, 1>(wide, (unsigned)((M + 15ll) / 16), 256, s, a);
+  if (a.pieces <= 64) return launch_norm<64, 1>(wide, (unsigned)((M + 3ll) / 4), 256, s, a);
+  const int P = a.pieces <= 1024 ? 1 : a.pieces <= 2048 ? 2 : 4;
+  const unsigned threads = (unsigned)(((a.pieces + P - 1) / P + kWave - 1) / kWave * kWave);
+  if (P == 1) return launch_norm<0, 1>(wide, (unsigned)M, threads, s, a);
+  if (P == 2) return launch_norm<0, 2>(wide, (unsigned)M, threads, s, a);
+  return launch_norm<0, 4>(wide, (unsigned)M, threads, s, a);
 }

@@ -150,7 +150,8 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     ``torch.ops.qwen_fastpath.qf_fp8_linear`` is the same call as one opaque op for torch.compile."""
     if x.dim() == 2:
         return _product(x, w, w_scale, bias, _BF16, out_features, None)
-    return _product(x.reshape(-1, x.shape[-1]), w, w_scale, bias, _BF16, out_features, None).view(*x.shape[:-1], -1)
+    y = _product(x.reshape(-1, x.shape[-1]), w, w_scale, bias, _BF16, out_features, None)
+    return y.view(*x.shape[:-1], y.shape[1])
 
 
 @torch.library.custom_op("qwen_fastpath::qf_fp8_linear", mutates_args=(), device_types="cuda")

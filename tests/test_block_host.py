@@ -61,6 +61,19 @@ def test_product_limits():
         assert B.load().qf_fp8_w8a8_workspace_bytes(M, N, K) == 0
 
 
+def test_sizes_past_a_launch():
+    """Grids of 2^32 threads and more, and rows of activations whose scales outgrow a workgroup, are refused."""
+    w8a8 = B.load().qf_fp8_w8a8_workspace_bytes
+    assert w8a8(2 ** 28 - 16, 16, 64) > 0 and w8a8(2 ** 28, 16, 64) == 0
+    assert w8a8(32, 16, 2 ** 18) > 0 and w8a8(32, 16, 2 ** 18 + 64) == 0
+    assert _product(True, M=2 ** 28, nbytes=1 << 62) == UNSUPPORTED
+    assert _product(True, K=2 ** 18 + 64, ldx=2 ** 18 + 64, ldw=2 ** 18 + 64, nbytes=1 << 62) == UNSUPPORTED
+    assert B.load().qf_quantize_tokens_fp8(P, 64, 2 ** 28, 64, P, 64, P, None) == UNSUPPORTED
+    for M, N in ((2 ** 22, 8192), (2 ** 26, 512), (2 ** 28, 128), (2 ** 31 - 1, 8)):
+        assert B.load().qf_block_norm_rows(P, N, P, N, 0, None, None, 0.0, None, 0, 0, 0, 1.0, 1e-6, M, N, P, N, P, N,
+                                           None) == UNSUPPORTED
+
+
 @pytest.mark.parametrize("kw,want", [
     (dict(x=None), INVALID), (dict(xq=None), INVALID), (dict(s=None), INVALID), (dict(M=0), INVALID),
     (dict(ldx=64), INVALID), (dict(ldq=64), INVALID), (dict(K=72), UNSUPPORTED), (dict(ldx=132), UNSUPPORTED),

@@ -105,6 +105,23 @@ def test_w8a8(qf, M, N, K, tiled, out):
     _check(qf, M, N, K, tiled, M % 2 == 1, out, True, seed=M + N)
 
 
+# a whole round of the largest tiles, tokens that end inside one; whole rounds and a second launch for the channels behind
+@pytest.mark.parametrize("tiled", [True, False])
+@pytest.mark.parametrize("M,N,K", [(1000, 16384, 320), (260, 33000, 2624)])
+def test_w8a8_wide(qf, M, N, K, tiled):
+    g = H.gen(N)
+    q, s = H.weight(g, N, K)
+    x, bias = H.rows(g, M, K), torch.randn(N, generator=g).to(BF16)
+    w = qf.fp8_to_tiled(q.cuda().t()) if tiled else q.cuda().t()
+    y = qf.fp8_w8a8_mm(x.cuda(), w, s.cuda(), bias=bias.cuda(), out_features=N).cpu()
+    rows = torch.tensor([0, 255, 256, M // 2, M - 1])
+    for b in (0, N // 256, 255, N // 128 - 1, (N - 1) // 128):  # channels of these blocks
+        b = min(b, (N - 1) // 128)
+        at = slice(128 * b, min(128 * b + 128, N))
+        ref, bound = H.product(x[rows], q[at], s[b:b + 1], bias[at], True)
+        H.within(y[rows][:, at], ref, bound, H.BF16)
+
+
 def test_linear_picks_by_rows_and_keeps_leading_dims(qf):
     g = H.gen(5)
     q, s = H.weight(g, 200, 256)
@@ -115,6 +132,8 @@ def test_linear_picks_by_rows_and_keeps_leading_dims(qf):
     assert torch.equal(qf.fp8_linear(x.view(2, 3, 4, 256), w, s), qf.fp8_linear(x, w, s).view(2, 3, 4, 200))
     assert torch.equal(torch.ops.qwen_fastpath.qf_fp8_linear(x, w, s), qf.fp8_linear(x, w, s))
     assert qf.fp8_linear(x[:0], w, s).shape == (0, 200)
+    assert qf.fp8_linear(x[:0].view(2, 0, 256), w, s).shape == (2, 0, 200)
+    assert torch.equal(qf.fp8_linear(x[0], w, s), qf.fp8_linear(x[:1], w, s)[0])
 
 
 @pytest.mark.parametrize("M", [5, 40, 300])
