@@ -1,7 +1,8 @@
-"""ctypes binding of libqf_block.so, the C ABI declared in include/qf_block.h.
+"""ctypes binding of libqf_block.so, the C ABI declared in include/qf_block.h, and the extension module that makes a
+call in its plain form without the steps in Python (csrc/qf_block_call.cpp).
 
-Built in-tree by qwen-a100-fastpath_amd/csrc/Makefile next to this file.  There is no fallback implementation: if the
-library is missing, every GPU entry point raises.
+Both are built in-tree by qwen-a100-fastpath_amd/csrc/Makefile next to this file.  There is no fallback implementation: if
+one is missing, every GPU entry point raises.
 """
 from __future__ import annotations
 
@@ -39,6 +40,7 @@ EXPORTS = (
 )
 
 _lib: ctypes.CDLL | None = None
+_plain = None
 
 
 def load() -> ctypes.CDLL:
@@ -71,6 +73,22 @@ def load() -> ctypes.CDLL:
         raise ImportError(f"{LIB_PATH}: ABI version {v}, expected {ABI_VERSION}")
     _lib = L
     return L
+
+
+def plain():
+    """(module, device, stream): the extension, whose functions return None where a call is not in the plain form, and what
+    they take, the current device with torch's current stream on it."""
+    global _plain
+    if _plain is None:
+        load()
+        try:
+            from . import _qf_block_call
+        except ImportError as e:
+            raise ImportError("qwen_fastpath._qf_block_call cannot be loaded: build it with `make -C "
+                              f"qwen-a100-fastpath_amd/csrc` (or __graft_entry__.build()): {e}") from e
+        _plain = _qf_block_call
+    device = torch._C._cuda_getDevice()
+    return _plain, device, torch._C._cuda_getCurrentRawStream(device)
 
 
 @functools.lru_cache(maxsize=4096)

@@ -70,8 +70,18 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x, ld
 
 
+def _split_workspace(x: torch.Tensor, nbytes: int) -> torch.Tensor:
+    return _workspace(x.device, nbytes)
+
+
 def _product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor], out_dtype,
              out_features: Optional[int], decode: Optional[bool]) -> torch.Tensor:
+    if x.is_cuda and (out_dtype is _BF16 or out_dtype is _F32):
+        plain, device, stream = B.plain()
+        y = plain.product(x, w, w_scale, bias, out_dtype is _F32, -1 if out_features is None else max(int(out_features), 0),
+                          -1 if decode is None else decode, _split_workspace, device, stream)
+        if y is not None:
+            return y
     if x.dim() != 2 or x.dtype is not _BF16:
         raise TypeError(f"x must be a 2-D bf16 tensor, got {x.dtype} {tuple(x.shape)}")
     if w.dtype is not _FP8 or w_scale.dtype is not _F32:

@@ -26,6 +26,11 @@ def moe_few_tokens(x: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tens
     [E, 2 ceil(I / 128), ceil(H / 128)] in that order; w2: the image of [E * H, I], s2 fp32 [E, ceil(H / 128),
     ceil(I / 128)].  H and I multiples of 64; E <= 512, top_k <= min(E, 16).  Activations stay bf16, weights are widened
     exactly, sums are fp32; the activation is kept to 16 bits between the products, y is rounded once at the end."""
+    if x.is_cuda:
+        plain, device, stream = B.plain()
+        y = plain.moe(x, router_logits, w13, s13, w2, s2, int(top_k), renormalize, device, stream)
+        if y is not None:
+            return y
     if x.dim() != 2 or x.dtype is not _BF16:
         raise TypeError(f"x must be a 2-D bf16 tensor, got {x.dtype} {tuple(x.shape)}")
     if router_logits.dim() != 2 or (router_logits.dtype is not _F32 and router_logits.dtype is not _BF16):

@@ -55,6 +55,12 @@ def block_norm_rows(x: torch.Tensor, residual: torch.Tensor, post_weight: Option
     one); gate bf16 [N] (a channel's), [M, 1] (a token's) or [M, N], gate_act "none" or "sigmoid".  All arithmetic is fp32;
     y is rounded once to the residual's type, h, from y before that rounding, once to bf16.  y may be given as the residual and
     h as x (in place); outputs must not overlap the inputs otherwise.  N % 8 == 0, N <= 32768."""
+    act = B.ACTS.get(gate_act)
+    if x.is_cuda and y is None and h is None and act is not None:
+        plain, device, stream = B.plain()
+        yh = plain.norm(x, residual, post_weight, pre_weight, gate, act, alpha, eps, weight_offset, device, stream)
+        if yh is not None:
+            return yh
     if x.dim() != 2 or x.dtype is not _BF16:
         raise TypeError(f"x must be a 2-D bf16 tensor, got {x.dtype} {tuple(x.shape)}")
     wide = residual.dtype is _F32
@@ -65,7 +71,6 @@ def block_norm_rows(x: torch.Tensor, residual: torch.Tensor, post_weight: Option
     M, N = x.shape
     if N < 8 or N % 8 or N > B.NORM_MAX_N:
         raise ValueError(f"N must be a multiple of 8 up to {B.NORM_MAX_N}, got {N}")
-    act = B.ACTS.get(gate_act)
     if act is None:
         raise ValueError(f"gate_act must be one of {sorted(B.ACTS)}, got {gate_act!r}")
     if not eps >= 0:

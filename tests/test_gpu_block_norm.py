@@ -155,3 +155,35 @@ def test_graph_replays(qf):
         torch.cuda.synchronize()
         assert torch.equal(y, ref[0]) and torch.equal(h, ref[1])
     assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+
+
+def test_plain_calls_agree_with_the_long_way(qf, monkeypatch):
+    import qwen_fastpath._qf_block_call as plain
+    g = H.gen(5)
+    x, r = torch.randn(9, 520, generator=g).to(BF16).cuda(), torch.randn(9, 520, generator=g).cuda()
+    w = torch.randn(520, generator=g).to(BF16).cuda()
+    calls = [lambda r=r, gate=gate, act=act: qf.block_norm_rows(x, r, w, None, gate, act, 0.5, 1e-5, 1.0)
+             for r in (r, r.to(BF16)) for gate in (None, w, x[:, :1], x) for act in ("none", "sigmoid")]
+    took = []
+    real = plain.norm
+    monkeypatch.setattr(plain, "norm", lambda *a: took.append(real(*a)) or took[-1])
+    short = [f() for f in calls]
+    assert len(took) == len(calls) and all(t is not None for t in took)
+    monkeypatch.setattr(plain, "norm", lambda *a: None)
+    for a, f in zip(short, calls):
+        b = f()
+        assert a[0].dtype == b[0].dtype and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_wrong_calls_on_the_gpu(qf):
+    x = torch.zeros(4, 64, dtype=BF16, device="cuda")
+    for f in (lambda: qf.block_norm_rows(x.half(), x), lambda: qf.block_norm_rows(x, x.half()), lambda: qf.block_norm_rows(x, x, x[0].float()),
+              lambda: qf.block_norm_rows(x, x, None, x[0, :32]), lambda: qf.block_norm_rows(x, x, gate=x[0].float())):
+        with pytest.raises(TypeError):
+            f()
+    for f in (lambda: qf.block_norm_rows(x, x[:3]), lambda: qf.block_norm_rows(x[:, :60].contiguous(), x[:, :60].contiguous()),
+              lambda: qf.block_norm_rows(x, x, gate=x[:, :2]), lambda: qf.block_norm_rows(x, x, gate=x[0, :4]),
+              lambda: qf.block_norm_rows(x, x, gate_act="silu"), lambda: qf.block_norm_rows(x, x, eps=-1.0),
+              lambda: qf.block_norm_rows(x, x.cpu())):
+        with pytest.raises(ValueError):
+            f()

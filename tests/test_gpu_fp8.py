@@ -136,6 +136,44 @@ def test_linear_picks_by_rows_and_keeps_leading_dims(qf):
     assert torch.equal(qf.fp8_linear(x[0], w, s), qf.fp8_linear(x[:1], w, s)[0])
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 200, 256), (16, 64, 8192), (40, 130, 320)])
+def test_plain_calls_agree_with_the_long_way(qf, monkeypatch, M, N, K):
+    import qwen_fastpath._qf_block_call as plain
+    g = H.gen(M)
+    q, s = H.weight(g, N, K)
+    x, w, s, bias = H.rows(g, M, K).cuda(), q.cuda().t(), s.cuda(), torch.randn(N, generator=g).to(BF16).cuda()
+    image = qf.fp8_to_tiled(w)
+    calls = [lambda: qf.fp8_linear(x, w, s), lambda: qf.fp8_linear(x, image, s, bias, N), lambda: qf.fp8_w8a8_mm(x, w, s, F32),
+             lambda: qf.fp8_w8a8_mm(x, image, s, bias=bias, out_features=N)]
+    took = []
+    real = plain.product
+    monkeypatch.setattr(plain, "product", lambda *a: took.append(real(*a)) or took[-1])
+    short = [f() for f in calls]
+    assert len(took) == len(calls) and all(t is not None for t in took)
+    monkeypatch.setattr(plain, "product", lambda *a: None)
+    for a, f in zip(short, calls):
+        b = f()
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_wrong_calls_on_the_gpu(qf):
+    g = H.gen(0)
+    q, s = H.weight(g, 200, 256)
+    x, w, s = H.rows(g, 24, 256).cuda(), q.cuda().t(), s.cuda()
+    image, bias = qf.fp8_to_tiled(w), torch.zeros(200, dtype=BF16, device="cuda")
+    for f in (lambda: qf.fp8_w8a8_mm(x, w, s, torch.float16), lambda: qf.fp8_linear(x.half(), w, s), lambda: qf.fp8_linear(x, w, s.half()),
+              lambda: qf.fp8_linear(x, w.view(torch.uint8), s), lambda: qf.fp8_linear(x, w, s, bias.float()),
+              lambda: qf.fp8_linear(x, w, s, bias[:199])):
+        with pytest.raises(TypeError):
+            f()
+    for f in (lambda: qf.fp8_linear(x, image, s, None, -1), lambda: qf.fp8_linear(x, image, s, None, 0), lambda: qf.fp8_linear(x, image, s, None, 192),
+              lambda: qf.fp8_linear(x, w, s, None, 199), lambda: qf.fp8_linear(x, w, s[:, :1]), lambda: qf.fp8_linear(x[:, :192], w, s),
+              lambda: qf.fp8_linear(x, w, s.cpu()), lambda: qf.fp8_linear(x, w.cpu(), s), lambda: qf.fp8_w8a16_mm(x, w, s),
+              lambda: qf.fp8_linear(x[:, :100].contiguous(), w[:100], s)):
+        with pytest.raises(ValueError):
+            f()
+
+
 @pytest.mark.parametrize("M", [5, 40, 300])
 def test_strided_and_unaligned_inputs(qf, M):
     g = H.gen(M)

@@ -106,6 +106,38 @@ def test_splits_of_the_second_product(qf, T, E, k, Hd, I):
     _check(qf, T, E, k, Hd, I, True, seed=Hd)
 
 
+def test_plain_calls_agree_with_the_long_way(qf, monkeypatch):
+    import qwen_fastpath._qf_block_call as plain
+    g = H.gen(2)
+    w = _on(qf, *_layer(g, 5, 128, 192))
+    x, logits = torch.randn(7, 128, generator=g).to(BF16).cuda(), torch.randn(7, 5, generator=g).cuda()
+    calls = [lambda T=T, l=l, n=n: qf.moe_few_tokens(x[:T], l[:T], *w, 3, n) for T in (1, 7) for l in (logits, logits.to(BF16)) for n in (True, False)]
+    took = []
+    real = plain.moe
+    monkeypatch.setattr(plain, "moe", lambda *a: took.append(real(*a)) or took[-1])
+    short = [f() for f in calls]
+    assert len(took) == len(calls) and all(t is not None for t in took)
+    monkeypatch.setattr(plain, "moe", lambda *a: None)
+    assert all(torch.equal(a, f()) for a, f in zip(short, calls))
+
+
+def test_wrong_calls_on_the_gpu(qf):
+    g = H.gen(2)
+    w13, s13, w2, s2 = _on(qf, *_layer(g, 5, 128, 192))
+    x, logits = torch.zeros(7, 128, dtype=BF16, device="cuda"), torch.zeros(7, 5, device="cuda")
+    for f in (lambda: qf.moe_few_tokens(x.half(), logits, w13, s13, w2, s2, 2), lambda: qf.moe_few_tokens(x, logits.half(), w13, s13, w2, s2, 2),
+              lambda: qf.moe_few_tokens(x, logits, w13, s13.half(), w2, s2, 2)):
+        with pytest.raises(TypeError):
+            f()
+    for f in (lambda: qf.moe_few_tokens(x, logits[:6], w13, s13, w2, s2, 2), lambda: qf.moe_few_tokens(x, logits, w13, s13, w2, s2, 0),
+              lambda: qf.moe_few_tokens(x, logits, w13, s13, w2, s2, 6), lambda: qf.moe_few_tokens(x, logits[:, :4], w13, s13, w2, s2, 2),
+              lambda: qf.moe_few_tokens(x, logits, w13, s13[:, :2], w2, s2, 2), lambda: qf.moe_few_tokens(x, logits, w13[:-1], s13, w2, s2, 2),
+              lambda: qf.moe_few_tokens(x, logits, w13, s13, w2, s2.cpu(), 2),
+              lambda: qf.moe_few_tokens(torch.cat([x, x, x]), torch.cat([logits, logits, logits]), w13, s13, w2, s2, 2)):
+        with pytest.raises(ValueError):
+            f()
+
+
 def test_every_token_count(qf):
     g = H.gen(11)
     up, down = _layer(g, 12, 128, 128)
