@@ -5,7 +5,7 @@
 //
 // 1. moe_up_kernel: every workgroup works the routing out for itself (a few thousand cycles, no launch and no trip through
 //    memory between), then streams a run of (chosen expert, 16 gate rows with their 16 up rows) items, the wavefronts sharing
-//    out the blocks of H; workgroup 0 leaves the routing for the second launch.
+//    out the blocks of H, two in flight each; workgroup 0 leaves the routing for the second launch.
 // 2. moe_down_kernel: a workgroup owns 32 output channels and a part of the (expert, block of I) units, its wavefronts share
 //    these out; the columns of the accumulator are the tokens, and a unit is weighed by its block's scale times c[t, e].  The
 //    last of a channel group's workgroups to arrive adds their sums, in split order.
@@ -28,7 +28,7 @@ constexpr int kStepK = 64;
 constexpr int kBlock = QF_FP8_BLOCK;
 constexpr int kMaxT = QF_FP8_MAX_DECODE_M;
 constexpr int kMaxPairs = kMaxT * QF_MOE_MAX_TOP_K;          // (token, chosen expert) pairs, so chosen experts too
-constexpr int kUpWaves = 8;
+constexpr int kMaxUpWaves = 16;
 constexpr int kDownGrid = 256;  // workgroups of the second launch where it splits: one a CU
 constexpr int kDownWaves = 8;
 constexpr int kDownTiles = 2;  // tiles of 16 output channels a workgroup
@@ -181,9 +181,11 @@ __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
 }
 
 template <int kPerLane>
-__global__ void __launch_bounds__(kUpWaves* kWave) __attribute__((amdgpu_waves_per_eu(4))) moe_up_kernel(const MoeArgs a) {
+__global__ void __launch_bounds__(kMaxUpWaves* kWave) __attribute__((amdgpu_waves_per_eu(4))) moe_up_kernel(const MoeArgs a) {
   __shared__ RoutingLds s;
-  __shared__ f32x4_t part[2][kUpWaves][2][kWave];
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int W = blockDim.x / kWave;
+  f32x4_t* const part = reinterpret_cast<f32x4_t*>(smem);  // [2][W][2][64 lanes]
   const int lane = threadIdx.x & (kWave - 1);
   const int v = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, r = lane & 15;
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kUpWaves* kWave) __attribute__((amdgpu_waves_p
   const int items = __builtin_amdgcn_readfirstlane(s.active) * row_tiles;
   const int first_item = (int)((int64_t)blockIdx.x * items / gridDim.x);
   const int n_items = (int)((int64_t)(blockIdx.x + 1) * items / gridDim.x) - first_item;
-  const int chunks = (a.h_blocks + 2 * kUpWaves - 1) / (2 * kUpWaves);  // of an item
+  const int chunks = (a.h_blocks + 2 * W - 1) / (2 * W);  // of an item
   if (n_items == 0) return;
   struct Step {
     u32x4_t gate[2], up[2], x[2][2];
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(kUpWaves* kWave) __attribute__((amdgpu_waves_p
     p_gate = a.w13 + (e * 2 * row_tiles + j) * a.h_steps * (kWave * 16);
     p_scale = a.s13 + (e * 2 * a.i_blocks + j * kTileN / kBlock) * a.h_blocks;
   };
-  auto block = [&](int j, int p) { return v + (2 * j + p) * kUpWaves; };
+  auto block = [&](int j, int p) { return v + (2 * j + p) * W; };
   auto load = [&](int j, int p, Step& b) {
     const bool in = block(j, p) < a.h_blocks;
     const int kb = in ? block(j, p) : 0;
@@ -262,19 +264,19 @@ __global__ void __launch_bounds__(kUpWaves* kWave) __attribute__((amdgpu_waves_p
   // them in wavefront order while the others stream on.
   f32x4_t acc_gate = {0.f, 0.f, 0.f, 0.f}, acc_up = acc_gate;
   auto leave = [&](int i) {
-    f32x4_t(&slot)[kUpWaves][2][kWave] = part[i & 1];
-    slot[v][0][lane] = acc_gate;
-    slot[v][1][lane] = acc_up;
+    f32x4_t* const slot = part + (i & 1) * W * 2 * kWave + lane;
+    slot[2 * v * kWave] = acc_gate;
+    slot[(2 * v + 1) * kWave] = acc_up;
     acc_gate = acc_up = f32x4_t{0.f, 0.f, 0.f, 0.f};
     ring_barrier();
-    if (v != i % kUpWaves) return;
+    if (v != i % W) return;
     const int item = first_item + i, at = item / row_tiles, j = item - at * row_tiles;
     const int first = s.first[at];
     if (r >= s.first[at + 1] - first) return;
-    f32x4_t gate = slot[0][0][lane], up = slot[0][1][lane];
-    for (int u = 1; u < kUpWaves; ++u) {
-      gate += slot[u][0][lane];
-      up += slot[u][1][lane];
+    f32x4_t gate = slot[0], up = slot[kWave];
+    for (int u = 1; u < W; ++u) {
+      gate += slot[2 * u * kWave];
+      up += slot[(2 * u + 1) * kWave];
     }
     // the activation as two bf16 parts, the rounded value and what the rounding left
     float hi[4], lo[4];
@@ -455,6 +457,17 @@ __global__ void __launch_bounds__(kDownWaves* kWave) moe_down_kernel(const MoeAr
   store(nt + v, sum);
 }
 
+// Wavefronts of the first launch's workgroups, each with two blocks of H in flight: the fewest passes over an item's blocks,
+// evenly filled.  17 blocks (H 2112, 7 tokens): 27 us with 9 wavefronts and one workgroup a CU, 32 with 8 in two passes and
+// two workgroups; 16 blocks: 48 with 8, 50 with 9 or 4, 60 with 5.
+constexpr int kCus = 256;
+constexpr int kSimdWaves = 4;  // of this kernel, by its registers; a workgroup's wavefronts go round the 4 SIMDs
+int up_waves(int h_blocks) {
+  const int passes = (h_blocks + 2 * kMaxUpWaves - 1) / (2 * kMaxUpWaves);
+  const int waves = (h_blocks + 2 * passes - 1) / (2 * passes);
+  return waves < 4 ? 4 : waves;
+}
+
 // Splits of the second launch: one workgroup a CU where the tile groups alone are fewer.
 int down_groups(int H) { return (H / kTileN + kDownTiles - 1) / kDownTiles; }
 int down_splits(int H) { return down_groups(H) <= kDownGrid / 2 ? kDownGrid / down_groups(H) : 1; }
@@ -517,10 +530,11 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t chosen = (int64_t)T * top_k < E ? (int64_t)T * top_k : E;
   const int64_t items = chosen * (I / kTileN);
-  const unsigned grid = (unsigned)(items < 512 ? items : 512);
+  const int waves = up_waves(a.h_blocks), resident = kCus * (kSimdWaves / ((waves + 3) / 4));
+  const unsigned grid = (unsigned)(items < resident ? items : resident);
   const auto up = E <= kWave ? &moe_up_kernel<1> : E <= 2 * kWave ? &moe_up_kernel<2> : E <= 4 * kWave ? &moe_up_kernel<4>
                                                                                              : &moe_up_kernel<8>;
-  hipLaunchKernelGGL(up, dim3(grid), dim3(kUpWaves * kWave), 0, s, a);
+  hipLaunchKernelGGL(up, dim3(grid), dim3(waves * kWave), waves * 4096, s, a);
   if (hipGetLastError() != hipSuccess) return QF_ERR_HIP;
   hipLaunchKernelGGL(moe_down_kernel, dim3((unsigned)down_groups(H), (unsigned)a.splits), dim3(kDownWaves * kWave), 0, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
