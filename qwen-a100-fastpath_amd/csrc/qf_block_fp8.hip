@@ -94,6 +94,11 @@ __device__ __forceinline__ int xcd_order(int i, int n) {
 // 16 g .. 16 g + 15 of each half block, so the fragments need no exchange.  Each wavefront parks its partial tile in LDS;
 // wavefront v then adds the W partials of tiles v, v + W, ... in wavefront order; with a K split the last workgroup of a run
 // adds the splits in split order.
+//
+// Bound by the weights' bytes: 5 x 34816 x 5120 30.4 us (5.9 TB/s), 1 x 5120 x 5120 8.6, 16 x 5120 x 17408 19.2 (row-major
+// 21).  A request behind a run's last tile cost 0.5 us there and 1.6 at 34816 channels.  Row-major slots a wavefront, 5 x
+// 34816 x 5120: 2 35.7 us, 3 36.8, 4 40.2.  The nontemporal hint: TILED 30.4 us, 32 without it where the weights do not stand
+// in the last-level cache; row-major copies with it 5% faster there and 20% slower where they do.
 // ---------------------------------------------------------------------------------------------
 constexpr int kRowSlots = 2;
 constexpr int kJoinBatch = 4;
@@ -420,6 +425,12 @@ __global__ void __launch_bounds__(256) quantize_tokens_fp8_kernel(const QuantArg
 // that is 1.5e-5 to 3.6e-5 of a result's size (normal values, K = 128 to 5120), a hundredth of an e4m3 activation's own
 // rounding.  The narrower f8 instruction (16x16x32) drops the same and runs at a third of the rate (1.42 against 4.58
 // PFLOP/s); the widened bf16 product of the decode kernel keeps everything, at half of it.
+//
+// Measured: 2048 x 32768 x 5120 (four rounds of 256 x 256) 315 to 330 us, 2.1 PFLOP/s, the matrix cores half busy at 2.2
+// GHz.  Without its copies (in a copy of the kernel, for timing) a round takes 57 us instead of 82; 256 x 128 tiles with two
+// stages ahead, all of a stage's copies at once, activations stored block by block, or weights read ahead into L2 change
+// nothing or cost time.  128 x 128 tiles reach 1.9 PFLOP/s: the LDS traffic of a step (96 KiB read, 32 written) is 0.47 of its
+// 0.57 us; 4 wavefronts of 64 x 64 read 64 KiB and take 0.7, as one wavefront a SIMD hides nothing.
 // ---------------------------------------------------------------------------------------------
 template <int FA_, int FB_, int WN_, int WM_, int S_>
 struct Tile {

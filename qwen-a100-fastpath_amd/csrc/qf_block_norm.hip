@@ -7,7 +7,8 @@
 // One pass: a row's values are read once into registers, 16 bytes a lane and piece, the two sums of squares meet by DPP
 // (and through LDS where a row spans wavefronts), and y (before its rounding) feeds the second norm from registers.  All
 // arithmetic is fp32 in a fixed order, each output rounded once.  Bound by memory: 8 bytes a value with a bf16 residual,
-// 12 with fp32, 2 more with a gate a value.
+// 12 with fp32, 2 more with a gate a value.  Measured: 2048 x 5120, fp32 residual, 24 us (5.2 TB/s, a large copy's rate);
+// 8191 x 2568 with a gate a value 35 us (6.0 TB/s); one row of 5120 3.0 us, a launch and three trips to memory and LDS.
 #include "qf_block_common.h"
 
 namespace qfb {
@@ -214,8 +215,11 @@ extern "C" int qf_block_norm_rows(const uint16_t* x, int64_t ldx, const void* re
   a.inv_n = 1.f / (float)N;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool wide = residual_f32 != 0;
+  // Rows of one piece a lane: 8192 rows in us, against a workgroup a row: N = 64 3.5 (5.7), 128 3.6 (5.8), 256 4.7 (6.3).
+  // Longer rows want the workgroup: 512 values 8.1 (32 lanes with two pieces 8.7, a wavefront 9.1), one row of them 2.0 (2.8
+  // with two pieces).  A thread takes 2 or 4 pieces only where 1024 threads do not reach.
   if (a.pieces <= 16) return launch_norm<16, 1>(wide, (unsigned)((M + 15ll) / 16), 256, s, a);
-  if (a.pieces <= 64) return launch_norm<64, 1>(wide, (unsigned)((M + 3ll) / 4), 256, s, a);
+  if (a.pieces <= 32) return launch_norm<32, 1>(wide, (unsigned)((M + 7ll) / 8), 256, s, a);
   const int P = a.pieces <= 1024 ? 1 : a.pieces <= 2048 ? 2 : 4;
   const unsigned threads = (unsigned)(((a.pieces + P - 1) / P + kWave - 1) / kWave * kWave);
   if (P == 1) return launch_norm<0, 1>(wide, (unsigned)M, threads, s, a);
