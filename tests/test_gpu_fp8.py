@@ -49,6 +49,25 @@ def test_decode(qf, M, N, K, tiled, out):
     _check(qf, M, N, K, tiled, M % 2 == 1, out, False, seed=M + N)
 
 
+# each form of the kernel (blocks a wavefront, x in LDS for up to 4, 8 and 16 tokens or in registers) with and without K splits
+@pytest.mark.parametrize("tiled", [True, False])
+@pytest.mark.parametrize("M,N,K", [
+    (15, 16672, 1920), (15, 4144, 7680), (4, 16, 5248), (8, 16, 3968), (15, 16, 2560), (9, 1376, 3968), (9, 8352, 3968),
+    (9, 16, 46336), (1, 16, 2176), (1, 16, 18688), (5, 16, 2176), (5, 16, 18688), (9, 16, 2176), (9, 16, 21248), (9, 2112, 4736),
+    (9, 16, 50304), (1, 16, 4224), (1, 16, 50304), (5, 16, 4224), (5, 288, 50304), (9, 4144, 2944), (9, 608, 25088), (5, 2736, 6528),
+    (9, 480, 50304), (1, 16, 6272), (1, 1040, 18688), (5, 1376, 6272), (5, 416, 50304), (9, 16, 3200), (9, 16, 34944),
+    (9, 4144, 3968), (12, 16, 15104), (9, 1040, 27264), (9, 21328, 2048)])
+def test_decode_forms(qf, M, N, K, tiled):
+    g = H.gen(K)
+    q, s = H.weight(g, N, K)
+    x, bias = H.rows(g, M, K), torch.randn(N, generator=g).to(BF16)
+    y = qf.fp8_w8a16_mm(x.cuda(), _weight_on(qf, q, tiled), s.cuda(), F32, bias.cuda(), N).cpu()
+    for b in {0, (N - 1) // 256, (N - 1) // 128}:  # channels of these blocks
+        at = slice(128 * b, min(128 * b + 128, N))
+        ref, bound = H.product(x, q[at], s[b:b + 1], bias[at], False)
+        H.within(y[:, at], ref, bound, H.F32)
+
+
 @pytest.mark.parametrize("M", range(1, 17))
 def test_decode_every_width(qf, M):
     _check(qf, M, 272, 640, M % 2 == 0, False, BF16, False, seed=M)
