@@ -125,8 +125,11 @@ def test_w8a8(qf, M, N, K, tiled, out):
 
 
 # a whole round of the largest tiles, tokens that end inside one; whole rounds and a second launch for the channels behind
+# (of each smaller tile); each tile with K splits
 @pytest.mark.parametrize("tiled", [True, False])
-@pytest.mark.parametrize("M,N,K", [(1000, 16384, 320), (260, 33000, 2624)])
+@pytest.mark.parametrize("M,N,K", [
+    (1000, 16384, 320), (260, 33000, 2624), (2917, 11832, 512), (2917, 5834, 768), (2751, 6068, 640), (2309, 2096, 7424),
+    (2178, 1862, 4864), (1286, 912, 4864), (852, 1157, 4224), (904, 663, 11648), (904, 663, 5632), (598, 777, 3456), (532, 588, 9600)])
 def test_w8a8_wide(qf, M, N, K, tiled):
     g = H.gen(N)
     q, s = H.weight(g, N, K)
@@ -134,8 +137,7 @@ def test_w8a8_wide(qf, M, N, K, tiled):
     w = qf.fp8_to_tiled(q.cuda().t()) if tiled else q.cuda().t()
     y = qf.fp8_w8a8_mm(x.cuda(), w, s.cuda(), bias=bias.cuda(), out_features=N).cpu()
     rows = torch.tensor([0, 255, 256, M // 2, M - 1])
-    for b in (0, N // 256, 255, N // 128 - 1, (N - 1) // 128):  # channels of these blocks
-        b = min(b, (N - 1) // 128)
+    for b in {min(b, (N - 1) // 128) for b in (0, N // 256, 31, 255, N // 128 - 1, N // 128)}:  # channels of these blocks
         at = slice(128 * b, min(128 * b + 128, N))
         ref, bound = H.product(x[rows], q[at], s[b:b + 1], bias[at], True)
         H.within(y[rows][:, at], ref, bound, H.BF16)
