@@ -71,7 +71,7 @@ __device__ __forceinline__ float group_max(float v) {  // NaN only where every v
   return v;
 }
 
-// Inclusive scan of sums, and the maximum in lane 63, over the wavefront's 64 lanes (every lane active).
+// Inclusive scan of sums over the wavefront's 64 lanes (every lane active).
 __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
@@ -81,14 +81,19 @@ __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: rows 0, 1 into 2, 3
   return v;
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
+// Maximum over groups of 16 or all 64 lanes, the same in each lane of a group.
+template <int L>
+__device__ __forceinline__ uint32_t group_max_u32(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));
+  if constexpr (L == 64) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));  // rows 1 and 3 with the rows before
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));  // rows 2 and 3 with row 1
+    v = (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
+  }
+  return v;
 }
 
 // 16 e4m3 values (a lane's bytes of a weight fragment) as two fragments of 8 bf16; exact (v_cvt_scalef32_pk_bf16_fp8).

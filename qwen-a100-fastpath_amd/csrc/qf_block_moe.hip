@@ -4,8 +4,8 @@
 //   a_e = silu(Wgate_e x) * (Wup_e x),   y[t] = sum over the chosen experts e of c[t, e] * W2_e a_e
 //
 // 1. moe_up_kernel: every workgroup works the routing out for itself (a few thousand cycles, no launch and no trip through
-//    memory between), then streams a run of (chosen expert, 16 gate rows with their 16 up rows) items, the wavefronts sharing
-//    out the blocks of H, two in flight each; workgroup 0 leaves the routing for the second launch.
+//    memory between).  Workgroup 0 leaves it for the second launch; the others each stream a run of (chosen expert, 16 gate
+//    rows with their 16 up rows) items, the wavefronts sharing out the blocks of H, two in flight each.
 // 2. moe_down_kernel: a workgroup owns 32 output channels and a part of the (expert, block of I) units, its wavefronts share
 //    these out; the columns of the accumulator are the tokens, and a unit is weighed by its block's scale times c[t, e].  The
 //    last of a channel group's workgroups to arrive adds their sums, in split order.
@@ -71,6 +71,7 @@ struct RoutingLds {
   uint8_t token[kMaxPairs];             // of a pair
   int16_t id[kMaxT][QF_MOE_MAX_TOP_K];  // -1: not routed
   float weight[kMaxT][QF_MOE_MAX_TOP_K];
+  float pair_weight[kMaxPairs];
   int active;
 };
 
@@ -84,8 +85,9 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return k == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// The routing of all tokens into LDS (every thread of the workgroup; ends with a barrier), for up to 64 kPerLane experts.
-template <int kPerLane>
+// The routing of all tokens into LDS (every thread of the workgroup; ends with a barrier): L lanes a token, each with up to
+// kPerLane experts, one chosen expert a round.
+template <int L, int kPerLane>
 __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -93,26 +95,26 @@ __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
   const int per = (a.E + kWave - 1) / kWave;
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) s.tokens[e] = 0;
   __syncthreads();
-  for (int t = wave; t < a.T; t += waves) {
-    uint32_t key[kPerLane];  // of experts lane * per .. + per - 1; 0: none, or taken
+  const int i = lane & (L - 1), share = (a.E + L - 1) / L;
+  for (int t0 = wave * (kWave / L); t0 < a.T; t0 += waves * (kWave / L)) {
+    const int t = t0 + lane / L;  // past the last token: the last one's values, not kept
+    uint32_t key[kPerLane];       // of experts i * share .. + share - 1; 0: none, or taken
+    const int64_t row = (int64_t)min(t, a.T - 1) * a.ldl;
 #pragma unroll
     for (int p = 0; p < kPerLane; ++p) {
-      const int e = lane * per + p;
+      const int e = i * share + p;
       key[p] = 0;
-      if (p < per && e < a.E) {
-        const int64_t at = t * a.ldl + e;
-        key[p] = order_key(a.logits_f32 ? static_cast<const float*>(a.logits)[at]
-                                        : bf16_f32(static_cast<const uint16_t*>(a.logits)[at]));
-      }
+      if (p < share && e < a.E)
+        key[p] = order_key(a.logits_f32 ? static_cast<const float*>(a.logits)[row + e]
+                                        : bf16_f32(static_cast<const uint16_t*>(a.logits)[row + e]));
     }
     float sum = 0.f;  // of the whole softmax's terms, relative to the largest
     uint32_t mine = 0, top = 0;
-    int id = 0;
     for (int j = 0; j < a.k; ++j) {
       uint32_t best = 0;
 #pragma unroll
       for (int p = 0; p < kPerLane; ++p) best = max(best, key[p]);
-      const uint32_t m = wave_max_u32(best);
+      const uint32_t m = group_max_u32<L>(best);
       if (j == 0) {
         top = m;
         if (!a.renormalize) {
@@ -120,30 +122,34 @@ __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
 #pragma unroll
           for (int p = 0; p < kPerLane; ++p)
             if (key[p] != 0) sum += expf(key_value(key[p]) - f);
-          sum = group_sum<64>(sum);
+          sum = group_sum<L>(sum);
         }
       }
-      const int from = __builtin_ctzll(__ballot(best == m));  // the first lane that has it: the lowest experts
-      int at = 0;
+      // the first lane that has it, and its first one: the lowest expert
+      const uint64_t have = __ballot(best == m);
+      const int from = L == kWave ? __builtin_ctzll(have) : __builtin_ctz((uint32_t)(have >> (lane & ~(L - 1))) & 0xffffu);
+      if (i == from) {
+        int at = 0;
 #pragma unroll
-      for (int p = kPerLane - 1; p >= 0; --p) at = key[p] == m ? p : at;
-      at = __builtin_amdgcn_readlane(at, from);
+        for (int p = kPerLane - 1; p >= 0; --p) at = key[p] == m ? p : at;
 #pragma unroll
-      for (int p = 0; p < kPerLane; ++p)
-        if (lane == from && p == at) key[p] = 0;
-      if (lane == j) {
-        mine = m;
-        id = from * per + at;
+        for (int p = 0; p < kPerLane; ++p)
+          if (p == at) key[p] = 0;
+        if (t < a.T) s.id[t][j] = (int16_t)(i * share + at);
       }
+      if (i == j) mine = m;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the ids that other lanes wrote
     const float f = key_value(top);
-    float c = lane < a.k ? expf(key_value(mine) - f) : 0.f;
-    if (a.renormalize) sum = group_sum<64>(c);
+    float c = i < a.k ? expf(key_value(mine) - f) : 0.f;
+    if (a.renormalize) sum = group_sum<L>(c);
     c = f == -__builtin_inff() ? 0.f : c / sum;
-    if (lane < a.k) {
-      s.id[t][lane] = c != 0.f ? (int16_t)id : (int16_t)-1;
-      s.weight[t][lane] = c;
-      if (c != 0.f) atomicOr(&s.tokens[id], 1u << t);
+    if (i < a.k && t < a.T) {
+      s.weight[t][i] = c;
+      if (c != 0.f)
+        atomicOr(&s.tokens[s.id[t][i]], 1u << t);
+      else
+        s.id[t][i] = -1;
     }
   }
   __syncthreads();
@@ -175,12 +181,15 @@ __device__ __forceinline__ void route(const MoeArgs& a, RoutingLds& s) {
   __syncthreads();
   for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x) {
     const int t = i / a.k, id = s.id[t][i % a.k];
-    if (id >= 0) s.token[s.first[s.place[id]] + __builtin_popcount(s.tokens[id] & ((1u << t) - 1))] = (uint8_t)t;
+    if (id < 0) continue;
+    const int pair = s.first[s.place[id]] + __builtin_popcount(s.tokens[id] & ((1u << t) - 1));
+    s.token[pair] = (uint8_t)t;
+    s.pair_weight[pair] = s.weight[t][i % a.k];
   }
   __syncthreads();
 }
 
-template <int kPerLane>
+template <int L, int kPerLane>
 __global__ void __launch_bounds__(kMaxUpWaves* kWave) __attribute__((amdgpu_waves_per_eu(4))) moe_up_kernel(const MoeArgs a) {
   __shared__ RoutingLds s;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -189,29 +198,30 @@ __global__ void __launch_bounds__(kMaxUpWaves* kWave) __attribute__((amdgpu_wave
   const int lane = threadIdx.x & (kWave - 1);
   const int v = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, r = lane & 15;
-  route<kPerLane>(a, s);
-  if (blockIdx.x == 0) {
+  route<L, kPerLane>(a, s);
+  if (blockIdx.x == 0) {  // leaves the routing for the second launch; the other workgroups share out the items
     const int active = s.active;
     if (threadIdx.x == 0) a.routing->active = active;
     if (threadIdx.x < kDownGrid / 2) a.routing->arrivals[threadIdx.x] = 0;
     for (int i = threadIdx.x; i < active; i += blockDim.x) a.routing->expert[i] = s.expert[i];
     for (int i = threadIdx.x; i < active * kMaxT; i += blockDim.x) {
-      const int at = i / kMaxT, t = i % kMaxT, e = s.expert[at];
-      const bool in = s.tokens[e] >> t & 1;
-      float c = 0.f;
-      if (in)
-        for (int j = 0; j < a.k; ++j) c = s.id[t][j] == e ? s.weight[t][j] : c;
-      a.routing->weight[at][t] = c;
-      a.routing->pair[at][t] = in ? (int16_t)(s.first[at] + __builtin_popcount(s.tokens[e] & ((1u << t) - 1))) : (int16_t)-1;
+      const int at = i / kMaxT, t = i % kMaxT;
+      const uint32_t tokens = s.tokens[s.expert[at]];
+      const int pair = s.first[at] + __builtin_popcount(tokens & ((1u << t) - 1));
+      const bool in = tokens >> t & 1;
+      a.routing->pair[at][t] = in ? (int16_t)pair : (int16_t)-1;
+      a.routing->weight[at][t] = in ? s.pair_weight[pair] : 0.f;
     }
+    return;
   }
   // This workgroup's run of (chosen expert, 16 gate rows and their up rows) items, as one stream of chunks of two blocks of
   // H a wavefront; a chunk's registers are loaded again for the next one as soon as they are multiplied.  (A wavefront without
   // a block in a chunk reads one line and multiplies nothing.)
   const int row_tiles = a.I / kTileN;
   const int items = __builtin_amdgcn_readfirstlane(s.active) * row_tiles;
-  const int first_item = (int)((int64_t)blockIdx.x * items / gridDim.x);
-  const int n_items = (int)((int64_t)(blockIdx.x + 1) * items / gridDim.x) - first_item;
+  const int share = gridDim.x - 1, place = blockIdx.x - 1;
+  const int first_item = (int)((int64_t)place * items / share);
+  const int n_items = (int)((int64_t)(place + 1) * items / share) - first_item;
   const int chunks = (a.h_blocks + 2 * W - 1) / (2 * W);  // of an item
   if (n_items == 0) return;
   struct Step {
@@ -468,9 +478,15 @@ int up_waves(int h_blocks) {
   return waves < 4 ? 4 : waves;
 }
 
-// Splits of the second launch: one workgroup a CU where the tile groups alone are fewer.
+// Splits of the second launch: one workgroup a CU where the tile groups alone are fewer, and a unit a wavefront at least, as
+// joining them takes about 2 us (H 512: 4 units 4.2 us, 7.0 in 16 splits; 16 units 5.7 and 7.9; H 1024: 30 units 7.4 in
+// one, 6.4 in 2 or 8).
 int down_groups(int H) { return (H / kTileN + kDownTiles - 1) / kDownTiles; }
-int down_splits(int H) { return down_groups(H) <= kDownGrid / 2 ? kDownGrid / down_groups(H) : 1; }
+int down_splits(int T, int E, int top_k, int H, int I) {
+  const int64_t chosen = T * top_k < E ? T * top_k : E, units = chosen * ((I + kBlock - 1) / kBlock);  // at most
+  const int64_t splits = down_groups(H) <= kDownGrid / 2 ? kDownGrid / down_groups(H) : 1;
+  return (int)(units / kDownWaves < 1 ? 1 : units / kDownWaves < splits ? units / kDownWaves : splits);
+}
 
 bool moe_sizes_ok(int T, int E, int top_k, int H, int I) {
   return T >= 1 && T <= kMaxT && E >= 1 && E <= QF_MOE_MAX_EXPERTS && top_k >= 1 && top_k <= QF_MOE_MAX_TOP_K &&
@@ -478,7 +494,7 @@ bool moe_sizes_ok(int T, int E, int top_k, int H, int I) {
 }
 
 constexpr size_t kRoutingBytes = (sizeof(Routing) + 255) / 256 * 256;
-size_t partial_bytes(int H) { return down_splits(H) > 1 ? (size_t)down_splits(H) * (H / kTileN) * 1024 : 0; }
+size_t partial_bytes(int splits, int H) { return splits > 1 ? (size_t)splits * (H / kTileN) * 1024 : 0; }
 
 }  // namespace qfb
 
@@ -488,7 +504,7 @@ extern "C" {
 
 size_t qf_moe_few_workspace_bytes(int T, int E, int top_k, int H, int I) {
   if (!moe_sizes_ok(T, E, top_k, H, I)) return 0;
-  return kRoutingBytes + partial_bytes(H) + ((size_t)T * top_k * I * 4 + 255) / 256 * 256;
+  return kRoutingBytes + partial_bytes(down_splits(T, E, top_k, H, I), H) + ((size_t)T * top_k * I * 4 + 255) / 256 * 256;
 }
 
 int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_t ldl, int logits_f32, const uint8_t* w13,
@@ -515,8 +531,8 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
   a.ldy = ldy;
   a.routing = static_cast<Routing*>(workspace);
   a.partial = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + kRoutingBytes);
-  a.splits = down_splits(H);
-  a.a = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + kRoutingBytes + partial_bytes(H));
+  a.splits = down_splits(T, E, top_k, H, I);
+  a.a = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + kRoutingBytes + partial_bytes(a.splits, H));
   a.T = T;
   a.E = E;
   a.k = top_k;
@@ -531,10 +547,12 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
   const int64_t chosen = (int64_t)T * top_k < E ? (int64_t)T * top_k : E;
   const int64_t items = chosen * (I / kTileN);
   const int waves = up_waves(a.h_blocks), resident = kCus * (kSimdWaves / ((waves + 3) / 4));
-  const unsigned grid = (unsigned)(items < resident ? items : resident);
-  // the routing's registers by the experts a lane holds (60 experts: 27.2 us, 27.6 with the 256 experts' form)
-  const auto up = E <= kWave ? &moe_up_kernel<1> : E <= 2 * kWave ? &moe_up_kernel<2> : E <= 4 * kWave ? &moe_up_kernel<4>
-                                                                                             : &moe_up_kernel<8>;
+  const unsigned grid = (unsigned)(items < resident - 1 ? items + 1 : resident);
+  // Routing: a wavefront a token where there are as many, else 16 lanes a token, so that 4 tokens share a round's latency (16
+  // tokens, 8 of 16 experts, H 512, I 128: 9.8 -> 6.8 us; 16 lanes for one token: +0.5 us).
+  const auto up = T > waves && E <= 64 ? &moe_up_kernel<16, 4> : T > waves && E <= 128 ? &moe_up_kernel<16, 8>
+                  : E <= 64 ? &moe_up_kernel<64, 1> : E <= 128 ? &moe_up_kernel<64, 2> : E <= 256 ? &moe_up_kernel<64, 4>
+                                                                                             : &moe_up_kernel<64, 8>;
   hipLaunchKernelGGL(up, dim3(grid), dim3(waves * kWave), waves * 4096, s, a);
   if (hipGetLastError() != hipSuccess) return QF_ERR_HIP;
   hipLaunchKernelGGL(moe_down_kernel, dim3((unsigned)down_groups(H), (unsigned)a.splits), dim3(kDownWaves * kWave), 0, s, a);
