@@ -14,7 +14,7 @@
 // bf16 alone put 2^-9 of noise into every a_e, half as much again as the output's own rounding (2.6e-3 against 1.7e-3 from
 // the exact result); the second product costs no weight bytes.  Bound by the memory rate over the chosen experts' weights.
 //
-// Measured, H 2048, I 768, 8 experts a token: 1 token (38 MB of weights) 10.2 + 7.1 us; 16 tokens of 128 experts (about 390
+// Measured, H 2048, I 768, 8 experts a token: 1 token (38 MB of weights) 10.8 + 7.1 us; 16 tokens of 128 experts (about 390
 // MB) 48 + 28 us, 5.2 TB/s.  The second launch took 61 us with 16 output channels a workgroup, 16 wavefronts and all units
 // (the activations' 1 KiB a token and unit, read again for every 16 channels, were the larger part of its loads); with 32
 // channels and the units split it is 28 with 8 wavefronts, 32 with 6, 30 with 4 and two workgroups a CU, 28 with 48 channels

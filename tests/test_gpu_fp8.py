@@ -228,7 +228,7 @@ def test_not_finite_values_stay_in_their_rows_and_channels(qf, M):
     assert torch.equal(torch.isnan(y), nan)
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 2500, 1088), (77, 2500, 2112), (300, 512, 1024)])
+@pytest.mark.parametrize("M,N,K", [(5, 2500, 1088), (9, 16, 18688), (16, 2560, 4352), (77, 2500, 2112), (300, 512, 1024), (852, 1157, 4224)])
 def test_graph_replays_and_repeats_bitwise(qf, M, N, K):
     g = H.gen(M)
     q, s = H.weight(g, N, K)
@@ -249,6 +249,35 @@ def test_graph_replays_and_repeats_bitwise(qf, M, N, K):
         assert torch.equal(qf.fp8_linear(v, w, s, out_features=N), ref)  # the program's own work between replays
         torch.cuda.synchronize()
         assert torch.equal(y, ref) and torch.equal(z, ref)
+
+
+@pytest.mark.parametrize("M", [16, 60])
+def test_two_graphs_at_once(qf, M):
+    """Graphs captured on one stream, their K splits' workspaces their own: replayed on two streams, eager calls beside."""
+    g = H.gen(M)
+    q, s = H.weight(g, 1200, 4352)
+    w, s = _weight_on(qf, q, True), s.cuda()
+    xs = [H.rows(g, M, 4352).cuda() for _ in range(3)]
+    want = [qf.fp8_linear(x, w, s, out_features=1200) for x in xs]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    for x in xs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(qf.fp8_linear(x, w, s, out_features=1200))
+        graphs.append(graph)
+    sides = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for y in outs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for side, graph in zip(sides, graphs):
+            with torch.cuda.stream(side):
+                graph.replay()
+        eager = qf.fp8_linear(xs[2], w, s, out_features=1200)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
 
 
 def test_calls_on_two_streams_at_once(qf):

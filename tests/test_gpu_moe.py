@@ -138,6 +138,33 @@ def test_wrong_calls_on_the_gpu(qf):
             f()
 
 
+def test_two_graphs_at_once(qf):
+    g = H.gen(6)
+    w = _on(qf, *_layer(g, 9, 512, 384))
+    xs = [torch.randn(16, 512, generator=g).to(BF16).cuda() for _ in range(3)]
+    logits = torch.randn(16, 9, generator=g).cuda()
+    want = [qf.moe_few_tokens(x, logits, *w, 3) for x in xs]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    for x in xs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(qf.moe_few_tokens(x, logits, *w, 3))
+        graphs.append(graph)
+    sides = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for y in outs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for side, graph in zip(sides, graphs):
+            with torch.cuda.stream(side):
+                graph.replay()
+        eager = qf.moe_few_tokens(xs[2], logits, *w, 3)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
+
+
 def test_every_token_count(qf):
     g = H.gen(11)
     up, down = _layer(g, 12, 128, 128)
