@@ -63,8 +63,9 @@ int qf_fp8_w8a16_gemm(const uint16_t* x, int64_t ldx, const uint8_t* w, int64_t 
 size_t qf_fp8_w8a16_workspace_bytes(int M, int N, int K, int layout);
 
 /* xq[m, k] = e4m3(x[m, k] / s_a[m, kb]), s_a[m, kb] = max_{k in kb} |x[m, k]| / 448 in fp32, both roundings to nearest
- * even; a block of zeros has scale 0 and values 0, a block that holds an infinity or NaN gives NaN there.  x bf16 [M, K] (row
- * stride ldx), xq e4m3 [M, K] (row stride ldq, a multiple of 8, 8-byte aligned), s_a fp32 [M, ceil(K / 128)] contiguous.  K % 64 == 0. */
+ * even; a block of zeros has scale 0 and values 0, a block that holds an infinity or NaN gives NaN there.  x bf16 [M, K]
+ * (row stride ldx), xq e4m3 [M, K] (row stride ldq, a multiple of 8, 8-byte aligned), s_a fp32 [M, ceil(K / 128)]
+ * contiguous.  K % 64 == 0. */
 int qf_quantize_tokens_fp8(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* xq, int64_t ldq, float* s_a,
                            void* stream);
 

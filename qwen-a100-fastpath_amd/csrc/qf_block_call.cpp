@@ -3,10 +3,10 @@
 // A call of one token takes the GPU 3 to 10 us and took the host 10 to 18: checks and address arithmetic in Python, a
 // ctypes call of twenty arguments, an allocation or two through torch's Python bindings.  These functions check the same
 // things on the tensors themselves, allocate through ATen and call the C ABI: a product of one row 9.0 -> 5.1 us on the host,
-// the norms of one row 9.5 -> 4.9 us (a launch is 3 of them).  A function returns None, before it has done anything, wherever something is not in
-// the plain form (a stride or alignment that needs a copy, another device or type, a tensor subclass, nothing to do, an
-// argument that is wrong); the caller in Python then takes the call from the start, with its copies and its errors.  A
-// status other than QF_OK also ends there.
+// the norms of one row 9.5 -> 4.9 us (a launch is 3 of them).  A function returns None, before it has launched anything,
+// wherever something is not in the plain form (a stride or alignment that needs a copy, another device or type, a tensor
+// subclass, nothing to do, an argument that is wrong); the caller in Python then takes the call from the start, with its
+// copies and its errors.  A status other than QF_OK also ends there.
 //
 // `device` and `stream` are the current device and torch's current stream on it.
 #include <Python.h>
@@ -71,7 +71,8 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       w->scalar_type() != at::kFloat8_e4m3fn || scale->scalar_type() != at::kFloat)
     Py_RETURN_NONE;
   const int64_t M = x->size(0), K = x->size(1);
-  if (M < 1 || M > kIntMax || K < 64 || K % 64 || K > kIntMax || ldx < K || ldx > kMaxStride || !aligned(w->data_ptr())) Py_RETURN_NONE;
+  if (M < 1 || M > kIntMax || K < 64 || K % 64 || K > kIntMax || ldx < K || ldx > kMaxStride || !aligned(w->data_ptr()))
+    Py_RETURN_NONE;
   int layout = QF_LAYOUT_TILED;
   if (w->dim() == 1) {
     N = named < 0 ? w->numel() / K : named;

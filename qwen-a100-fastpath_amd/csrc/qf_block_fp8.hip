@@ -872,8 +872,8 @@ struct DecodePlan {
 
 // One workgroup a CU (a second round costs 3.5 us: 272 tiles 11.7 us against 8.3 for 256, K = 5120), so runs as long as that
 // takes, and the cheapest number of splits by what a CU then has to fetch (28 bytes a ns under load) and what joining them
-// costs: 3 us and 0.25 + 0.06 splits a tile of the run.  Splits pay where x is large beside a run's weights.  Measured at M = 16 in us, K
-// = 5120, without a split and with the chosen ones: N = 1280 9.4 -> 7.2, 5120 13.0 -> 12.3, 10240 16.1 (2 splits 17.8);
+// costs: 3 us and 0.25 + 0.06 splits a tile of the run.  Splits pay where x is large beside a run's weights.  Measured at M
+// = 16 in us, K = 5120, without a split and with the chosen ones: N = 1280 9.4 -> 7.2, 5120 13.0 -> 12.3, 10240 16.1 (2 splits 17.8);
 // 5120 x 8192 20.4 -> 15.2.  x in LDS (xl) where it fits beside the run's partials, else in registers, 3 blocks a
 // wavefront at most.
 DecodePlan plan_decode(int layout, int M, int ntiles, int kblocks) {

@@ -514,7 +514,9 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
     return QF_ERR_INVALID_ARG;
   if (T < 1 || E < 1 || top_k < 1 || H < 1 || I < 1 || (T > 1 && (ldx < H || ldl < E || ldy < H))) return QF_ERR_INVALID_ARG;
   if (!moe_sizes_ok(T, E, top_k, H, I)) return QF_ERR_UNSUPPORTED;
-  if (ldx > ((int64_t)1 << 26) || ldx % 8 || ldy % 4 || !aligned16(x) || !aligned16(w13) || !aligned16(w2) || ((uintptr_t)y & 7)) return QF_ERR_UNSUPPORTED;
+  if (ldx > ((int64_t)1 << 26) || ldx % 8 || ldy % 4 || !aligned16(x) || !aligned16(w13) || !aligned16(w2) ||
+      ((uintptr_t)y & 7))
+    return QF_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < qf_moe_few_workspace_bytes(T, E, top_k, H, I) || !aligned16(workspace))
     return QF_ERR_WORKSPACE;
   MoeArgs a;
