@@ -36,8 +36,7 @@ __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
 }
 
-// Sum over a row's threads (their shares of the mean: the squares' sum itself may overflow where the mean does not):
-// groups of L lanes, or (L = 0) the whole workgroup.
+// Sum over a row's threads of their shares of the mean: groups of L lanes, or (L = 0) the whole workgroup.
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float* exchange) {
   if constexpr (L > 0) return group_sum<L>(v);
@@ -49,6 +48,34 @@ __device__ __forceinline__ float row_sum(float v, float* exchange) {
   v = 0.f;
   for (int w = 0; w < waves; ++w) v += exchange[w];
   return v;
+}
+
+// A row's mean square, of the P pieces of 8 values of a thread that piece(i, f) gives.  A thread's squares may overflow where
+// the mean does not: such a row's are taken again, of the values' 2^-8 (exact but for what vanishes beside them), which
+// keeps rows of up to 2^15 values in range.  The branch is uniform over the wavefront, and over the workgroup where rows span
+// wavefronts (its threads add the same sums in the same order); the other rows of a wavefront keep their own mean.
+template <int L, int P, typename F>
+__device__ __forceinline__ float mean_square(float inv_n, float* exchange, F piece) {
+  static_assert(QF_BLOCK_NORM_MAX_N <= 1 << 15, "2^-16 of a row's squares stays below their mean");
+  float f[8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    piece(i, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += f[e] * f[e];
+  }
+  const float mean = row_sum<L>(sum * inv_n, exchange);
+  if (__builtin_expect(!__any(!(mean < __builtin_inff())), 1)) return mean;
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    piece(i, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += (f[e] * 0x1p-8f) * (f[e] * 0x1p-8f);
+  }
+  if constexpr (L == 0) __syncthreads();  // the first sums have been read
+  const float again = row_sum<L>(sum * (inv_n * 0x1p16f), exchange);
+  return mean < __builtin_inff() ? mean : again;
 }
 
 // L lanes a row with 256 / L rows a workgroup (L > 0), or a workgroup a row (L = 0); P pieces of 8 values a thread.
@@ -87,19 +114,11 @@ __global__ void __launch_bounds__(L > 0 ? 256 : 1024) block_norm_kernel(const No
   }
 
   if (a.w_post != nullptr) {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      float f[8];
-      unpack8(xv[i], f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += f[e] * f[e];
-    }
-    row_gate *= 1.f / sqrtf(row_sum<L>(sum * a.inv_n, exchange[0]) + a.eps);
+    const float mean = mean_square<L, P>(a.inv_n, exchange[0], [&](int i, float(&f)[8]) { unpack8(xv[i], f); });
+    row_gate *= 1.f / sqrtf(mean + a.eps);
   }
 
   float y[P][8];
-  float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int j = t + i * threads;
@@ -127,7 +146,6 @@ __global__ void __launch_bounds__(L > 0 ? 256 : 1024) block_norm_kernel(const No
     for (int e = 0; e < 8; ++e) {
       y[i][e] += row_gate * f[e];
       if (j >= a.pieces) y[i][e] = 0.f;  // an infinite row_gate times the padding's zeros is no number
-      sum += y[i][e] * y[i][e];
     }
     if (live && j < a.pieces) {
       if constexpr (WIDE) {
@@ -142,7 +160,11 @@ __global__ void __launch_bounds__(L > 0 ? 256 : 1024) block_norm_kernel(const No
       }
     }
   }
-  const float inv = 1.f / sqrtf(row_sum<L>(sum * a.inv_n, exchange[1]) + a.eps);
+  const float mean = mean_square<L, P>(a.inv_n, exchange[1], [&](int i, float(&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = y[i][e];
+  });
+  const float inv = 1.f / sqrtf(mean + a.eps);
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int j = t + i * threads;
