@@ -163,10 +163,12 @@ __device__ __forceinline__ u32x4_t load_once(const uint8_t* p) {  // read once: 
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
 }
 
-// Lets `fn` have `bytes` of dynamic LDS on the current device; `raised` holds the devices where it has.
+constexpr int kDefaultLds = 64 * 1024;  // of a workgroup, static and dynamic
+
+// Lets `fn` have `bytes` of dynamic LDS on the current device; `raised` holds the devices where it has.  Called where static
+// and dynamic LDS together may pass kDefaultLds.
 inline bool raise_lds(const void* fn, int bytes, std::atomic<uint64_t>& raised) {
   int dev = 0;
-  if (bytes <= 64 * 1024) return true;
   if (hipGetDevice(&dev) != hipSuccess) return false;
   const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
   if (bit & raised.load(std::memory_order_relaxed)) return true;

@@ -29,6 +29,7 @@ constexpr int kBlock = QF_FP8_BLOCK;
 constexpr int kMaxT = QF_FP8_MAX_DECODE_M;
 constexpr int kMaxPairs = kMaxT * QF_MOE_MAX_TOP_K;          // (token, chosen expert) pairs, so chosen experts too
 constexpr int kMaxUpWaves = 16;
+constexpr int kUpWaveLds = 4096;  // a wavefront's partial tiles: gate and up, two buffers
 constexpr int kDownGrid = 256;  // workgroups of the second launch where it splits: one a CU
 constexpr int kDownWaves = 8;
 constexpr int kDownTiles = 2;  // tiles of 16 output channels a workgroup
@@ -478,6 +479,19 @@ int up_waves(int h_blocks) {
   return waves < 4 ? 4 : waves;
 }
 
+// The first launch's kernels by the routing's shape.  With 15 or 16 wavefronts the partial tiles and the routing pass the LDS
+// that a launch may have unasked.
+struct UpKernel {
+  void (*fn)(MoeArgs);
+  std::atomic<uint64_t> raised;
+};
+UpKernel& up_kernel(bool shared_waves, int E) {
+  static UpKernel kernels[] = {{&moe_up_kernel<16, 4>, {0}}, {&moe_up_kernel<16, 8>, {0}}, {&moe_up_kernel<64, 1>, {0}},
+                               {&moe_up_kernel<64, 2>, {0}}, {&moe_up_kernel<64, 4>, {0}}, {&moe_up_kernel<64, 8>, {0}}};
+  if (shared_waves && E <= 128) return kernels[E <= 64 ? 0 : 1];
+  return kernels[E <= 64 ? 2 : E <= 128 ? 3 : E <= 256 ? 4 : 5];
+}
+
 // Splits of the second launch: one workgroup a CU where the tile groups alone are fewer, and a unit a wavefront at least, as
 // joining them takes about 2 us (H 512: 4 units 4.2 us, 7.0 in 16 splits; 16 units 5.7 and 7.9; H 1024: 30 units 7.4 in
 // one, 6.4 in 2 or 8).
@@ -552,10 +566,11 @@ int qf_moe_few_tokens(const uint16_t* x, int64_t ldx, const void* logits, int64_
   const unsigned grid = (unsigned)(items < resident - 1 ? items + 1 : resident);
   // Routing: a wavefront a token where there are as many, else 16 lanes a token, so that 4 tokens share a round's latency (16
   // tokens, 8 of 16 experts, H 512, I 128: 9.8 -> 6.8 us; 16 lanes for one token: +0.5 us).
-  const auto up = T > waves && E <= 64 ? &moe_up_kernel<16, 4> : T > waves && E <= 128 ? &moe_up_kernel<16, 8>
-                  : E <= 64 ? &moe_up_kernel<64, 1> : E <= 128 ? &moe_up_kernel<64, 2> : E <= 256 ? &moe_up_kernel<64, 4>
-                                                                                             : &moe_up_kernel<64, 8>;
-  hipLaunchKernelGGL(up, dim3(grid), dim3(waves * kWave), waves * 4096, s, a);
+  UpKernel& up = up_kernel(T > waves, E);
+  const int lds = waves * kUpWaveLds;
+  if (lds + (int)sizeof(RoutingLds) > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(up.fn), kMaxUpWaves * kUpWaveLds, up.raised))
+    return QF_ERR_HIP;
+  hipLaunchKernelGGL(up.fn, dim3(grid), dim3(waves * kWave), lds, s, a);
   if (hipGetLastError() != hipSuccess) return QF_ERR_HIP;
   hipLaunchKernelGGL(moe_down_kernel, dim3((unsigned)down_groups(H), (unsigned)a.splits), dim3(kDownWaves * kWave), 0, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
