@@ -150,7 +150,9 @@ def fp8_w8a16_mm(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dt
 def fp8_w8a8_mm(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype: torch.dtype = _BF16,
                 bias: Optional[torch.Tensor] = None, out_features: Optional[int] = None) -> torch.Tensor:
     """y[M, N] = xq @ W^T (+ bias) for any M, xq the activations rounded to e4m3 per token and block of 128
-    (quantize_tokens_fp8): exact products, fp32 sums, one rounding to out_dtype.  Arguments as fp8_w8a16_mm."""
+    (quantize_tokens_fp8): fp32 sums, one rounding to out_dtype.  The products are not exact: of 8 neighbouring k the f8
+    matrix instruction drops what lies below 2^(e - 13), e the largest exponent sum among them, which was 1.5e-5 to 3.6e-5
+    of a result on normal values (about 15 bits, with fp32 output too).  Arguments as fp8_w8a16_mm."""
     return _product(x, w, w_scale, bias, out_dtype, out_features, False)
 
 
