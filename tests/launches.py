@@ -101,3 +101,24 @@ def record(calls):
             pending = []
     assert len(got) == len(calls)
     return got
+
+
+def w8a8_splits(call, recorded):
+    """(channels and tokens of the last launch's tile, its K splits, whether a launch of whole rounds goes before it)."""
+    _, _, M, N, _ = call
+    tiles = [l for l in recorded[2] if l.kernel == "fp8_tile_kernel"]
+    shape = lambda l: (16 * l.params[1][0] * l.params[1][2], 16 * l.params[1][1] * l.params[1][3])  # noqa: E731
+    if len(tiles) == 2:
+        channels, tokens = shape(tiles[0])
+        N -= tiles[0].grid[0] // -(-M // tokens) * channels
+    channels, tokens = shape(tiles[-1])
+    n = -(-N // channels) * -(-M // tokens)
+    assert tiles[-1].grid[0] % n == 0
+    return channels, tokens, tiles[-1].grid[0] // n, len(tiles) == 2
+
+
+def decode_splits(call, recorded):
+    """K splits of a ("decode", ...) call: its workspace is the counters and a KiB for each split and tile."""
+    _, bytes_, _ = recorded
+    counters = 64 * 1024
+    return 1 if bytes_ == 0 else (bytes_ - counters) // (1024 * -(-call[3] // 16))
