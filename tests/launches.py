@@ -103,6 +103,12 @@ def record(calls):
     return got
 
 
+def decode_form(call, recorded):
+    """(layout, blocks a wavefront, KiB of x in LDS a block or 0, K split) of a ("decode", ...) call."""
+    _, bytes_, made = recorded
+    return (*made[-1].params, bytes_ > 0)
+
+
 def w8a8_splits(call, recorded):
     """(channels and tokens of the last launch's tile, its K splits, whether a launch of whole rounds goes before it)."""
     _, _, M, N, _ = call
@@ -115,6 +121,12 @@ def w8a8_splits(call, recorded):
     n = -(-N // channels) * -(-M // tokens)
     assert tiles[-1].grid[0] % n == 0
     return channels, tokens, tiles[-1].grid[0] // n, len(tiles) == 2
+
+
+def w8a8_form(call, recorded):
+    """(layout, channels, tokens, K split, behind a first launch) of a ("w8a8", ...) call."""
+    channels, tokens, splits, behind = w8a8_splits(call, recorded)
+    return call[1], channels, tokens, splits > 1, behind
 
 
 def decode_splits(call, recorded):

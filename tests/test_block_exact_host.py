@@ -1,4 +1,7 @@
-"""That the integer products of exact_cases would show a lost block and a sum kept in 16 bits."""
+"""That the integer products of exact_cases would show a lost block and a sum kept in 16 bits, and that they take every
+form of the kernels (by what the entry points would launch, without a GPU)."""
+import random
+
 import pytest
 import torch
 
@@ -15,6 +18,19 @@ def _recorded(kind, cases):
 @pytest.fixture(scope="module")
 def plans():
     return _recorded("decode", X.DECODE), _recorded("w8a8", X.W8A8)
+
+
+def test_every_form_is_taken(plans):
+    rng = random.Random(3)
+    size = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))  # noqa: E731
+    decode = [(rng.randint(0, 1), rng.randint(1, 16), size(1, 40000), 64 * size(1, 1000)) for _ in range(40000)]
+    w8a8 = [(rng.randint(0, 1), size(1, 3000), size(1, 40000), 64 * size(1, 300)) for _ in range(20000)]
+    w8a8 += [(rng.randint(0, 1), size(250, 3000), size(1500, 40000), 64 * size(8, 300)) for _ in range(20000)]
+    for kind, sizes, form, own in (("decode", decode, launches.decode_form, plans[0]), ("w8a8", w8a8, launches.w8a8_form, plans[1])):
+        sizes = list(dict.fromkeys(c for c in sizes if c[2] * c[3] <= 3e8))
+        reached = {form(*r) for r in _recorded(kind, sizes).values()}
+        taken = {form(*r) for r in own.values()}
+        assert not reached - taken, f"{kind} forms without a case: {sorted(reached - taken)}"
 
 
 def _columns(N):
