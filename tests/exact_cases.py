@@ -75,3 +75,88 @@ def reference(xd, q, s, bias):
         y[:, at] = xd @ w.t() + bias[at].double()
     assert y.abs().max() < 2 ** 24
     return y.float()
+
+
+# ---- experts' layer: (T, E, k, H, I), k a power of two ----
+# the routing's kernels; H and I that end in half a block, an odd last tile; second products with and without splits of the
+# units; one and two passes over the blocks of H, 4 to 16 wavefronts; one unit a wavefront and many
+MOE = [
+    (1, 1, 1, 64, 64), (1, 8, 2, 128, 128), (16, 4, 1, 64, 320), (16, 16, 8, 256, 128), (7, 130, 16, 128, 64), (5, 512, 8, 64, 64),
+    (3, 300, 4, 128, 192), (16, 65, 2, 1088, 192), (16, 100, 8, 320, 192), (4, 8, 8, 2112, 1344), (9, 20, 16, 64, 1344),
+    (2, 3, 2, 4096, 64), (2, 3, 2, 4160, 64), (3, 4, 2, 8192, 192), (16, 40, 8, 2688, 448), (1, 12, 8, 2048, 768),
+    (7, 24, 4, 2112, 1344), (16, 24, 8, 2048, 768), (1, 70, 1, 192, 2112), (2, 9, 4, 7168, 320), (6, 10, 2, 512, 64)]
+
+
+def experts(T, E, k, Hd, I, seed=0):
+    """(x bf16, logits fp32, [(q13 e4m3 [2 I, H], s13)], [(q2 e4m3 [H, I], s2)], {token: its experts}) with
+
+    * gate sums about 1024 (1024 from k = 0, the others' sum stays beside it), where silu(g) = g / (1 + exp(-g)) is g in fp32;
+    * up sums of at most 12, six values a row, so that an activation is a whole number below 2^15: one bf16 does not hold
+      it, the sum of two does;
+    * a token's experts equally likely, 1, 2, 4, ... k of them, so that their weights are powers of two.
+
+    W2 is sparse: the sum of all |c w2 a| stays below 2^24 of its unit."""
+    g = H.gen(seed + T + 3 * E + 5 * Hd + 7 * I)
+    ib, hb = H.blocks(I), H.blocks(Hd)
+    x = ints(g, 1, T, Hd).to(torch.bfloat16)
+    x[:, 0] = 8.0
+    up, down = [], []
+    for _ in range(E):
+        gate, ups = ints(g, 1, I, Hd), torch.zeros(I, Hd, dtype=torch.int8)
+        gate[:, 0] = 0
+        gate = gate.float()
+        gate[:, 0] = 128.0
+        ups.scatter_(1, torch.randint(1, Hd, (I, 6), generator=g), (2 * torch.randint(0, 2, (I, 6), generator=g) - 1).to(torch.int8))
+        s = 2.0 ** torch.randint(0, 2, (2 * ib, hb), generator=g)
+        s[:ib, 0] = 1.0
+        up.append((torch.cat([gate, ups.float()]).to(H.FP8), s))
+        w2 = ints(g, 2, Hd, I) * (torch.rand(Hd, I, generator=g) < 0.06)
+        down.append((w2.float().to(H.FP8), 2.0 ** torch.randint(0, 2, (hb, ib), generator=g)))
+    logits, chosen = torch.full((T, E), -float("inf")), {}
+    for t in range(T):
+        n = 2 ** int(torch.randint(0, k.bit_length(), (1,), generator=g)) if t % 3 == 2 else k
+        chosen[t] = sorted(torch.randperm(E, generator=g)[:n].tolist())
+        logits[t, chosen[t]] = float(t % 5) - 2.0
+    return x, logits, up, down, chosen
+
+
+def activations(x, q13, s13, without=None):
+    """fp64 [I] activations of one token; without: (0 gate or 1 up, block of H) that is left out."""
+    I = q13.shape[0] // 2
+    ends = []
+    for half, rows, scales in ((0, slice(0, I), slice(0, H.blocks(I))), (1, slice(I, 2 * I), slice(H.blocks(I), None))):
+        w = H.widen(q13[rows], s13[scales])
+        if without is not None and without[0] == half:
+            w[:, H.BLOCK * without[1]:H.BLOCK * (without[1] + 1)] = 0
+        ends.append(w @ x.double())
+    return ends
+
+
+def layer_units(x, up, down, chosen):
+    """{token: (c, fp64 [experts, half blocks of I, 2 (bf16 parts), H])}: what each part adds to y[t] / c."""
+    out = {}
+    for t, ids in chosen.items():
+        c = 1.0 / len(ids)
+        units = []
+        for e in ids:
+            gate, ups = activations(x[t], *up[e])
+            assert gate.min() >= 32 and gate.max() < 2048 and ups.abs().max() <= 12
+            a = gate * ups
+            hi = a.to(torch.bfloat16).double()
+            lo = a - hi
+            assert torch.equal(lo.to(torch.bfloat16).double(), lo)
+            w2 = H.widen(*down[e])
+            assert (w2.abs() @ a.abs()).max() * 1.0 < 2 ** 24 / 16  # of up to 16 experts, in units of c
+            parts = [(w2 * v).view(w2.shape[0], -1, 64).sum(2).t() for v in (hi, lo)]
+            units.append(torch.stack(parts, 1))
+        out[t] = c, torch.stack(units)
+    return out
+
+
+def layer(units, T, Hd):
+    """y bf16 from layer_units: the exact sums, rounded once."""
+    y = torch.zeros(T, Hd, dtype=torch.float64)
+    for t, (c, u) in units.items():
+        y[t] = c * u.sum((0, 1, 2))
+    assert torch.equal(y.float().double(), y)
+    return y.float().to(torch.bfloat16)
