@@ -96,7 +96,8 @@ __device__ __forceinline__ int xcd_order(int i, int n) {
 // adds the splits in split order.
 //
 // Bound by the weights' bytes: 5 x 34816 x 5120 30.4 us (5.9 TB/s), 1 x 5120 x 5120 8.6, 16 x 5120 x 17408 19.2 (row-major
-// 21).  A request behind a run's last tile cost 0.5 us there and 1.6 at 34816 channels.  Row-major slots a wavefront, 5 x
+// 21), over three sets of weights, part of them in the last-level cache; over 1.5 GB of them, a call in a graph, 33.6 (5.3
+// TB/s), 8.3 and row-major 24.5.  A request behind a run's last tile cost 0.5 us there and 1.6 at 34816 channels.  Row-major slots a wavefront, 5 x
 // 34816 x 5120: 2 35.7 us, 3 36.8, 4 40.2.  The nontemporal hint: TILED 30.4 us, 32 without it where the weights do not stand
 // in the last-level cache; row-major copies with it 5% faster there and 20% slower where they do.
 // ---------------------------------------------------------------------------------------------

@@ -7,8 +7,9 @@
 // One pass: a row's values are read once into registers, 16 bytes a lane and piece, the two sums of squares meet by DPP
 // (and through LDS where a row spans wavefronts), and y (before its rounding) feeds the second norm from registers.  All
 // arithmetic is fp32 in a fixed order, each output rounded once.  Bound by memory: 8 bytes a value with a bf16 residual,
-// 12 with fp32, 2 more with a gate a value.  Measured: 2048 x 5120, fp32 residual, 24 us (5.2 TB/s, a large copy's rate);
-// 8191 x 2568 with a gate a value 35 us (6.0 TB/s); one row of 5120 3.0 us, a launch and three trips to memory and LDS.
+// 12 with fp32, 2 more with a gate a value.  Measured: 2048 x 5120, fp32 residual, 24 us (5.2 TB/s, a large copy's rate; 28
+// and 4.4 TB/s where the rows come from HBM); 8191 x 2568 with a gate a value 35 us (6.0 TB/s; 37 and 5.7); one row of 5120
+// 3.1 us, a launch and three trips to memory and LDS.
 #include "qf_block_common.h"
 
 namespace qfb {
