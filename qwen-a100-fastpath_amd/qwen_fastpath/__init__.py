@@ -23,6 +23,9 @@ from .fp8 import (  # noqa: F401
     quantize_tokens_fp8)
 from .moe import moe_few_tokens  # noqa: F401
 from .norm import block_norm_rows  # noqa: F401
+from .kv4 import kv4_attention, kv4_cache, kv4_load, kv4_store  # noqa: F401
+from .rope import qk_norm_rope  # noqa: F401
+from .step import StepTables, step_tables  # noqa: F401
 from .patches import (  # noqa: F401
     Int8Head,
     W8A16LinearMethod,
