@@ -12,12 +12,11 @@
 //   attn_tile_kernel     many rows (prompt chunks): each wavefront its own rows, all their positions
 #include "qf_kv4_common.h"
 
-#include <mutex>
+#include <float.h>
+#include <math.h>
 
 namespace qfk {
 
-constexpr int kAttnThreads = 256;
-constexpr int kAttnWaves = kAttnThreads / kWave;
 constexpr int kStep = 2 * kTile;  // positions of a step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMinChunk = 4 * kStep;
@@ -34,10 +33,12 @@ struct AttnArgs {
   int64_t sbt;
   const int32_t *seq_lens, *cu_q;
   int B, Q, T, H, HKV, G, page, max_blocks;
-  int rows;     // of a request: at most Q * G
+  int rows;     // split kernel: the most rows of a request that it takes
+  int few;      // tile kernel: requests of up to so many rows are the split kernel's
   int workers;  // split kernel: positions are split so that about this many workgroups a kv head share the batch
-  float qk_scale;
-  Divisor by_g, by_page;
+  float qk_scale;  // |scale| * log2(e): scores are kept in base 2
+  uint32_t flip;   // the queries' signs, changed for a negative scale
+  Divisor by_g, by_page, by_workers;
   float* o_part;   // [HKV][slots][rows][D]
   float2* ml_part; // [HKV][slots][rows]: exponent reference, sum
   int2* plan;      // [B]: first slot and slots of a request
@@ -57,12 +58,15 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
     r.tok0 = b * a.Q;
     r.n = a.Q;
   }
-  r.seq = max(a.seq_lens[b], 0);
-  if ((int64_t)a.max_blocks * a.page < r.seq) r.seq = a.max_blocks * a.page;
+  r.seq = min(max(a.seq_lens[b], 0), a.max_blocks * a.page);  // below 2^31 - 63
   return r;
 }
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The largest, NaN where one is.  (fmaxf, which leaves NaN out, would first quiet each operand that comes from a matrix
+// instruction.)
+__device__ __forceinline__ float largest(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 
 __device__ __forceinline__ float quarters_max(float v) {  // over the 4 lanes l, l^16, l^32, l^48
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -78,7 +82,9 @@ template <int D>
 struct StepData {
   static constexpr int kDwords = D < 128 ? 2 : 4;  // of a half's keys, and of its values
   static constexpr int kHalves = Record<D>::kHalves;
-  uint32_t k[2][kHalves][kDwords], v[2][kHalves][kDwords], ks[2][kHalves], vs[2][kHalves];
+  typedef uint32_t Run __attribute__((ext_vector_type(kDwords)));
+  Run k[2][kHalves], v[2][kHalves];
+  uint32_t ks[2][kHalves], vs[2][kHalves];
 };
 
 template <int D, int RT>
@@ -118,7 +124,8 @@ struct Walk {
       const uint16_t* p = a.q + (int64_t)(r.tok0 + qi) * a.sq_t + (int64_t)(hkv * a.G + (row - qi * a.G)) * a.sq_h;
 #pragma unroll
       for (int s = 0; s < kKSteps; ++s)
-        qf[rt][s] = *reinterpret_cast<const bf16x8_t*>(p + s / kDwords * 128 + qg * 8 * kDwords + s % kDwords * 8);
+        qf[rt][s] = __builtin_bit_cast(
+            bf16x8_t, *reinterpret_cast<const u32x4_t*>(p + s / kDwords * 128 + qg * 8 * kDwords + s % kDwords * 8) ^ a.flip);
       last[rt] = r.seq - r.n + qi;
       m[rt] = -__builtin_inff();
       l[rt] = 0.f;
@@ -130,50 +137,30 @@ struct Walk {
     bt_row = a.bt + (int64_t)b * a.sbt;
   }
 
-  // The record that holds position pos (a multiple of 16), the same in every lane.
-  __device__ __forceinline__ const uint8_t* record(int pos) const {
+  // Offset from `base` of the record that holds position pos (a multiple of 16).
+  __device__ __forceinline__ int64_t record(int pos) const {
     const int pg = divide(pos, a.by_page);
     int64_t block = bt_row[pg];
     block = block < 0 ? 0 : block >= a.num_blocks ? a.num_blocks - 1 : block;
-    return base + block * a.stride + (pos - pg * a.page) / kTile * R::kBytes;
+    return block * a.stride + (pos - pg * a.page) / kTile * R::kBytes;
   }
 
-  __device__ __forceinline__ void load(Data& s, const uint8_t* r0, const uint8_t* r1) const {
+  __device__ __forceinline__ void load_keys(Data& s, const uint8_t* r0, const uint8_t* r1) const {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const uint8_t* r = t == 0 ? r0 : r1;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
-        const uint8_t* kp = r + l16 * (D / 2) + h * 64 + qg * (4 * kDwords);
-        const uint8_t* vp = r + R::kValues + h * 1024 + lane * (4 * kDwords);
-        if constexpr (kDwords == 4) {
-          const u32x4_t kk = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp));
-          const u32x4_t vv = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vp));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s.k[t][h][i] = kk[i];
-            s.v[t][h][i] = vv[i];
-          }
-          s.ks[t][h] = r[R::kKeyScales + (4 * h + qg) * kTile + l16];
-          s.vs[t][h] = *reinterpret_cast<const uint32_t*>(r + R::kValueScales + (4 * h + l16 / 4) * kTile + 4 * qg);
-        } else {
-          const u32x2_t kk = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(kp));
-          const u32x2_t vv = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(vp));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            s.k[t][h][i] = kk[i];
-            s.v[t][h][i] = vv[i];
-          }
-          s.ks[t][h] = r[R::kKeyScales + qg / 2 * kTile + l16];
-          s.vs[t][h] = *reinterpret_cast<const uint32_t*>(r + R::kValueScales + l16 / 8 * kTile + 4 * qg);
-        }
+        const uint8_t* p = r + l16 * (D / 2) + h * 64 + qg * (4 * kDwords);
+        s.k[t][h] = *reinterpret_cast<const typename Data::Run*>(p);
+        s.ks[t][h] = *reinterpret_cast<const uint32_t*>(r + R::kKeyScales + (kDwords == 4 ? 4 * h + qg : qg / 2) * kTile + (l16 & 12));
       }
     }
   }
 
   // A value's block of NaN at a position that some rows see and others do not: the product would give it to all rows.  Where a
   // step holds one, its scales are cleared for the product and the rows that see it are made NaN here.
-  __device__ __forceinline__ void masked_nan(Data& s, int pos, const uint8_t* r0, const uint8_t* r1) {
+  __device__ __forceinline__ void masked_nan(Data& s, int pos, int end) {
     bool any = false;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -193,15 +180,20 @@ struct Walk {
             s.vs[t][h] |= 127u << (8 * i);
             clear(s, t, h, i);
           }
-    // the lane's outputs are values 128 h + 32 qg .. of its rows (D = 64: 16 qg ..): one block each
-    for (int p = 0; p < kStep; ++p) {
-      const uint8_t* r = (p < kTile ? r0 : r1) + p % kTile;
+    mark_nan(pos, min(pos + kStep, end));
+  }
+
+  // NaN into the outputs of the rows that see a value's block of NaN among positions from .. to - 1 (the lane's outputs are values
+  // 128 h + 32 qg .. of its rows, for D = 64 16 qg ..: one block each).
+  __device__ __forceinline__ void mark_nan(int from, int to) {
+    for (int p = from; p < to; ++p) {
+      const uint8_t* r = base + record(p / kTile * kTile) + p % kTile;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         const uint32_t byte = r[R::kValueScales + (kDwords == 4 ? 4 * h + qg : qg / 2) * kTile];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          if (byte == 255u && pos + p <= last[rt]) {
+          if (byte == 255u && p <= last[rt]) {
 #pragma unroll
             for (int u = 0; u < kPerHalf; ++u) o[rt][h * kPerHalf + u] = o[rt][h * kPerHalf + u] + __builtin_nanf("");
           }
@@ -218,61 +210,56 @@ struct Walk {
     }
   }
 
-  // Positions pos .. pos + 31, those from `end` on hold nothing.  r0, r1: the records (read again in a rare case only).
-  __device__ __forceinline__ void step(Data& s, int pos, int end, const uint8_t* r0, const uint8_t* r1) {
-    f32x4_t sc[RT][2];
+  typedef f32x4_t Scores[RT][2];
+
+  // The lane's byte of a dword of 4 positions' scales, turned to an fp32's exponent.  (`here`: where it is used; moved up to its
+  // load, the instruction would wait for it.)
+  __device__ __forceinline__ float key_scale(uint32_t w) const {
+    w = here(w);
+    return __uint_as_float(__builtin_amdgcn_alignbit(w, w, (uint32_t)(8 * (l16 & 3) + 9)));
+  }
+
+  // S^T of a step's 32 positions, 2 RT chains of matrix instructions side by side.
+  __device__ __forceinline__ void scores(const Data& s, Scores& sc) const {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const float k0 = key_scale(s.ks[0][h]), k1 = key_scale(s.ks[1][h]);
+#pragma unroll
+      for (int c = 0; c < kDwords; ++c) {
+        const bf16x8_t f0 = __builtin_bit_cast(bf16x8_t, widen8(s.k[0][h][c], k0));
+        const bf16x8_t f1 = __builtin_bit_cast(bf16x8_t, widen8(s.k[1][h][c], k1));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          sc[rt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f0, qf[rt][h * kDwords + c], sc[rt][0], 0, 0, 0);
+          sc[rt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f1, qf[rt][h * kDwords + c], sc[rt][1], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // -inf where a row does not see a position.
+  __device__ __forceinline__ void mask(Scores& sc, int pos) const {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      const int p0 = pos + t * kTile + 4 * qg;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sc[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const float ks = scale_f32(s.ks[t][h]);
-#pragma unroll
-        for (int c = 0; c < kDwords; ++c) {
-          const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, widen8(s.k[t][h][c], ks));
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            sc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][h * kDwords + c], sc[rt][t], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+        for (int i = 0; i < 4; ++i) sc[rt][t][i] = p0 + i <= last[rt] ? sc[rt][t][i] : -__builtin_inff();
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) sc[rt][t] *= a.qk_scale;
-    if (pos + kStep > diag || pos + kStep > end) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int p0 = pos + t * kTile + 4 * qg;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sc[rt][t][i] = p0 + i < end && p0 + i <= last[rt] ? sc[rt][t][i] : -__builtin_inff();
-        // what stands behind the end may be anything, a NaN among it: weight 0 times 0
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (p0 + i >= end) {
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-              s.vs[t][h] &= ~(255u << (8 * i));
-              s.vs[t][h] |= 127u << (8 * i);
-              clear(s, t, h, i);
-            }
-          }
-      }
-      masked_nan(s, pos, r0, r1);
-    }
-    // The row's exponent reference moves only when a score exceeds it by 2^8: the weights stay below that, and the
-    // accumulators are rarely rescaled.  The result is that of the running maximum up to rounding.
+  }
+
+  // The rows' exponent references brought up to the scores.  A reference moves only when a score exceeds it by 2^8: the weights
+  // stay below that, and the accumulators are rarely rescaled.  The result is that of the running maximum up to rounding.
+  __device__ __forceinline__ void refer(const Scores& sc) {
     bool above = false;
     float mx[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      mx[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
-                     fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
+      const f32x4_t x = sc[rt][0], y = sc[rt][1];
+      mx[rt] = a.qk_scale * largest(largest(largest(largest(x[0], x[1]), x[2]), largest(largest(x[3], y[0]), y[1])), largest(y[2], y[3]));
       above |= mx[rt] > m[rt] + kRescale;
     }
     if (__any(above)) {
@@ -286,23 +273,59 @@ struct Walk {
         for (int u = 0; u < kDTiles; ++u) o[rt][u] *= keep;
       }
     }
-    bf16x8_t pf[RT];
+  }
+
+  // The softmax weights of the scores, rounded to bf16, as the operand P^T.
+  __device__ __forceinline__ void weigh(const Scores& sc, bf16x8_t (&pf)[RT]) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float ref = m[rt] == -__builtin_inff() ? 0.f : m[rt];  // a row that has seen nothing yet
       float w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = fast_exp2(sc[rt][i / 4][i % 4] - ref);
+      for (int i = 0; i < 8; ++i) w[i] = fast_exp2(__builtin_fmaf(sc[rt][i / 4][i % 4], a.qk_scale, -ref));
       l[rt] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       pf[rt] = __builtin_bit_cast(bf16x8_t, pack8(w));
     }
+  }
+
+  // Positions pos .. pos + 31, those from `end` on hold nothing.
+  __device__ __forceinline__ void step(Data& s, int pos, int end) {
+    Scores sc;
+    scores(s, sc);
+    if (pos + kStep > diag || pos + kStep > end) {
+      mask(sc, pos);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int p0 = pos + t * kTile + 4 * qg;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (p0 + i < end) continue;
+          // what stands behind the end may be anything, a NaN among it: weight 0 times 0
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt][t][i] = -__builtin_inff();
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            s.vs[t][h] &= ~(255u << (8 * i));
+            s.vs[t][h] |= 127u << (8 * i);
+            clear(s, t, h, i);
+          }
+        }
+      }
+      masked_nan(s, pos, end);
+    }
+    refer(sc);
+    bf16x8_t pf[RT];
+    weigh(sc, pf);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       float vs[2][4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vs[t][i] = scale_f32(s.vs[t][h] >> (8 * i) & 255u);
+      for (int t = 0; t < 2; ++t) {
+        vs[t][0] = scale_of<0>(s.vs[t][h]);
+        vs[t][1] = scale_of<1>(s.vs[t][h]);
+        vs[t][2] = scale_of<2>(s.vs[t][h]);
+        vs[t][3] = scale_of<3>(s.vs[t][h]);
+      }
       auto values = [&](auto byte) {  // value n = 2 byte and 2 byte + 1 of the lane's run, as operands over the 8 positions
         constexpr int kB = decltype(byte)::value;
         u32x4_t even, odd;
@@ -341,26 +364,149 @@ struct Walk {
     }
   }
 
-  // Steps first, first + by, ... below n_steps, of positions from `begin` on.
-  __device__ __forceinline__ void run(int begin, int end, int first, int by) {
+  // ---- the split kernel's way: steps through LDS ----
+  // A lane's bytes go from global memory to LDS and from there to the same lane's registers, so LDS is a place to wait in, without
+  // registers, for the step after the one that is computed.
+  static constexpr int kCodes = 2 * 2 * kHalves * kDwords * 4 * kWave;         // a step's codes, keys then values
+  static constexpr int kScales = D < 128 ? 256 : 2 * D;                        // and scales (D = 64: half of it is not read)
+  static constexpr int kSlot = kCodes + kScales;
+  static constexpr int kCopies = kCodes / 1024 + kScales / 256;                // instructions of a step
+  typedef const void __attribute__((address_space(1)))* gptr_t;
+  typedef void __attribute__((address_space(3)))* lptr_t;
+
+  __device__ __forceinline__ void copy(const uint8_t* from, uint8_t* to) const {
+    __builtin_amdgcn_global_load_lds((gptr_t)from, (lptr_t)to, 16, 0, 2);  // 2: read once, not kept
+  }
+  __device__ __forceinline__ void copy_step(const uint8_t* r0, const uint8_t* r1, uint8_t* slot) const {
+    if constexpr (kDwords == 4) {
+      const uint32_t key = (uint32_t)(l16 * (D / 2) + qg * 16), value = (uint32_t)(R::kValues + lane * 16);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const uint8_t* r = t == 0 ? r0 : r1;
+          copy(r + h * 64 + key, slot + (t * kHalves + h) * 1024);
+          copy(r + h * 1024 + value, slot + (2 * kHalves + t * kHalves + h) * 1024);
+        }
+    } else {  // a record's codes are a KiB, the keys' half first
+      copy(r0 + lane * 16, slot);
+      copy(r1 + lane * 16, slot + 1024);
+    }
+    uint8_t* const to = slot + kCodes;
+    if constexpr (D == 256) {
+      __builtin_amdgcn_global_load_lds((gptr_t)(r0 + R::kKeyScales + lane * 4), (lptr_t)to, 4, 0, 2);
+      __builtin_amdgcn_global_load_lds((gptr_t)(r1 + R::kKeyScales + lane * 4), (lptr_t)(to + 256), 4, 0, 2);
+    } else {  // both records' scales in one instruction
+      constexpr int kLanes = D / 4;
+      const uint8_t* r = lane / kLanes % 2 == 0 ? r0 : r1;
+      __builtin_amdgcn_global_load_lds((gptr_t)(r + R::kKeyScales + lane % kLanes * 4), (lptr_t)to, 4, 0, 2);
+    }
+  }
+
+  // The step's data out of its slot.  One block with its own wait: the compiler would wait for every copy in flight before
+  // an LDS read that it sees.
+  __device__ __forceinline__ void read_step(Data& s, const uint8_t* slot) const {
+    const uint32_t at = lds_addr(slot);
+    const uint32_t ks = at + kCodes + (uint32_t)((kDwords == 4 ? qg : qg / 2) * kTile + (l16 & 12));
+    const uint32_t vs = at + kCodes + (uint32_t)(D / 2 + (kDwords == 4 ? l16 / 4 : l16 / 8) * kTile + 4 * qg);
+    if constexpr (D == 64) {
+      const uint32_t k = at + (uint32_t)(l16 * 32 + qg * 8), v = at + 512 + (uint32_t)(lane * 8);
+      u32x2_t k0, k1, v0, v1;
+      asm volatile(
+          "ds_read_b64 %0, %8\n\tds_read_b64 %1, %8 offset:1024\n\tds_read_b32 %4, %10\n\tds_read_b32 %5, %10 offset:64\n\t"
+          "ds_read_b64 %2, %9\n\tds_read_b64 %3, %9 offset:1024\n\tds_read_b32 %6, %11\n\tds_read_b32 %7, %11 offset:64\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(k0), "=&v"(k1), "=&v"(v0), "=&v"(v1), "=&v"(s.ks[0][0]), "=&v"(s.ks[1][0]), "=&v"(s.vs[0][0]), "=&v"(s.vs[1][0])
+          : "v"(k), "v"(v), "v"(ks), "v"(vs)
+          : "memory");
+      s.k[0][0] = k0;
+      s.k[1][0] = k1;
+      s.v[0][0] = v0;
+      s.v[1][0] = v1;
+    } else if constexpr (D == 128) {
+      u32x4_t k0, k1, v0, v1;
+      asm volatile(
+          "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b32 %4, %9\n\tds_read_b32 %5, %9 offset:128\n\t"
+          "ds_read_b128 %2, %8 offset:2048\n\tds_read_b128 %3, %8 offset:3072\n\tds_read_b32 %6, %10\n\t"
+          "ds_read_b32 %7, %10 offset:128\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(k0), "=&v"(k1), "=&v"(v0), "=&v"(v1), "=&v"(s.ks[0][0]), "=&v"(s.ks[1][0]), "=&v"(s.vs[0][0]), "=&v"(s.vs[1][0])
+          : "v"(at + (uint32_t)lane * 16), "v"(ks), "v"(vs)
+          : "memory");
+      s.k[0][0] = k0;
+      s.k[1][0] = k1;
+      s.v[0][0] = v0;
+      s.v[1][0] = v1;
+    } else {
+      u32x4_t k[4], v[4];
+      uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+      asm volatile(
+          "ds_read_b128 %0, %16\n\tds_read_b128 %1, %16 offset:1024\n\tds_read_b128 %2, %16 offset:2048\n\t"
+          "ds_read_b128 %3, %16 offset:3072\n\tds_read_b32 %8, %17\n\tds_read_b32 %9, %17 offset:64\n\t"
+          "ds_read_b32 %10, %17 offset:256\n\tds_read_b32 %11, %17 offset:320\n\tds_read_b128 %4, %16 offset:4096\n\t"
+          "ds_read_b128 %5, %16 offset:5120\n\tds_read_b128 %6, %16 offset:6144\n\tds_read_b128 %7, %16 offset:7168\n\t"
+          "ds_read_b32 %12, %18\n\tds_read_b32 %13, %18 offset:64\n\tds_read_b32 %14, %18 offset:256\n\t"
+          "ds_read_b32 %15, %18 offset:320\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(a0),
+            "=&v"(a1), "=&v"(a2), "=&v"(a3), "=&v"(b0), "=&v"(b1), "=&v"(b2), "=&v"(b3)
+          : "v"(at + (uint32_t)lane * 16), "v"(ks), "v"(vs)
+          : "memory");
+      s.ks[0][0] = a0;
+      s.ks[0][kHalves - 1] = a1;
+      s.ks[1][0] = a2;
+      s.ks[1][kHalves - 1] = a3;
+      s.vs[0][0] = b0;
+      s.vs[0][kHalves - 1] = b1;
+      s.vs[1][0] = b2;
+      s.vs[1][kHalves - 1] = b3;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          s.k[t][h] = k[(t * kHalves + h) % 4];
+          s.v[t][h] = v[(t * kHalves + h) % 4];
+        }
+    }
+  }
+
+  // Steps first, first + by, ... of the positions begin .. end - 1, through two slots of kSlot bytes.  The records of 32 steps are
+  // looked up at once, a record a lane.
+  __device__ __forceinline__ void run(int begin, int end, int first, int by, uint8_t* slots) {
     const int n_steps = (end - begin + kStep - 1) / kStep;
+    const int mine = first < n_steps ? (n_steps - 1 - first) / by + 1 : 0;
     const int last_tile = (end - 1) / kTile * kTile;
-    if (first >= n_steps) return;
-    Data s[2];
-    const uint8_t *r0[2], *r1[2];
-    auto fetch = [&](int i, int u) {
-      const int pos = begin + min(i, n_steps - 1) * kStep;
-      r0[u] = record(pos);
-      r1[u] = record(min(pos + kTile, last_tile));
-      load(s[u], r0[u], r1[u]);
+    uint32_t rec_lo = 0, rec_hi = 0;
+    auto look_up = [&](int i) {
+      const int pos = begin + (first + min(i + lane / 2, mine - 1) * by) * kStep + lane % 2 * kTile;
+      const int64_t at = record(min(pos, last_tile));
+      rec_lo = (uint32_t)at;
+      rec_hi = (uint32_t)(at >> 32);
     };
-    fetch(first, 0);
+    auto where = [&](int l) {
+      const uint32_t lo = __builtin_amdgcn_readlane(rec_lo, l), hi = __builtin_amdgcn_readlane(rec_hi, l);
+      return base + (int64_t)(((uint64_t)hi << 32) | lo);
+    };
+    auto issue = [&](int i) {
+      if (i % 32 == 0 && i > 0) {
+        look_up(i);
+        wait_vmcnt<0>();
+      }
+      copy_step(where(2 * (i % 32)), where(2 * (i % 32) + 1), slots + i % 2 * kSlot);
+    };
+    if (mine > 0) look_up(0);
+    wait_vmcnt<0>();  // the queries too: the copies alone are counted below
+    if (mine > 0) issue(0);
 #pragma unroll 1
-    for (int i = first; i < n_steps; i += 2 * by) {
-      fetch(i + by, 1);
-      step(s[0], begin + i * kStep, end, r0[0], r1[0]);
-      fetch(i + 2 * by, 0);
-      if (i + by < n_steps) step(s[1], begin + (i + by) * kStep, end, r0[1], r1[1]);
+    for (int i = 0; i < mine; ++i) {
+      if (i + 1 < mine) {
+        issue(i + 1);  // into the slot of step i - 1, whose reads have returned
+        wait_vmcnt<kCopies>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      asm volatile("" ::: "memory");
+      Data now;
+      read_step(now, slots + i % 2 * kSlot);
+      step(now, begin + (first + i * by) * kStep, end);
     }
   }
 
@@ -397,55 +543,73 @@ struct Place {
 };
 __device__ __forceinline__ bool place_of(const AttnArgs& a, int slot, Place& p) {
   const int lane = threadIdx.x % kWave;
-  uint64_t total = 0;
-  for (int base = 0; base < a.B; base += kWave) {
-    const int b = base + lane;
-    if (b < a.B) {
-      const Request r = request(a, b);
-      total += r.n > 0 ? (uint32_t)r.seq : 0u;
-    }
-  }
+  auto steps = [&](int b) {  // of request b: -1 where it has no tokens, or too many
+    if (b >= a.B) return -1;
+    const Request r = request(a, b);
+    return r.n > 0 && r.n * a.G <= a.rows ? (r.seq + kStep - 1) / kStep : -1;
+  };
+  int mine = steps(lane);
+  uint32_t most;  // steps of a chunk
+  {
+    uint32_t sum = max(mine, 0);
+    uint64_t total = 0;
+    if (a.B > kWave) {
+      uint64_t all = sum;
+      for (int b = lane + kWave; b < a.B; b += kWave) all += (uint32_t)max(steps(b), 0);
 #pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint32_t lo = __shfl_xor((int)(uint32_t)total, d), hi = __shfl_xor((int)(uint32_t)(total >> 32), d);
-    total += ((uint64_t)hi << 32) | lo;
-  }
-  const uint64_t even = (total + a.workers - 1) / (uint32_t)a.workers;
-  const uint64_t chunk = (max(even, (uint64_t)kMinChunk) + kStep - 1) / kStep * kStep;
-  p.chunk = chunk > 0x7fffffe0 ? 0x7fffffe0 : (int)chunk;
-  int before = 0;
-  bool found = false;
-  for (int base = 0; base < a.B; base += kWave) {
-    const int b = base + lane;
-    int n = 0;
-    if (b < a.B) {
-      const Request r = request(a, b);
-      n = r.n > 0 ? max((int)(((uint32_t)r.seq + (uint32_t)(p.chunk - 1)) / (uint32_t)p.chunk), 1) : 0;
+      for (int d = 1; d < kWave; d *= 2) {
+        const uint32_t lo = __shfl_xor((int)(uint32_t)all, d), hi = __shfl_xor((int)(uint32_t)(all >> 32), d);
+        all += ((uint64_t)hi << 32) | lo;
+      }
+      total = all;
+    } else {
+      total = (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)sum), kWave - 1);  // at most 64 * 2^26
     }
+    most = total < 0x80000000u ? (uint32_t)divide((int)total, a.by_workers) + 1 : (uint32_t)(total / (uint32_t)a.workers) + 1;
+    most = min(max(most, (uint32_t)(kMinChunk / kStep)), 1u << 26);
+  }
+  p.chunk = (int)min(most * kStep, 0x7fffffe0u);
+  int before = 0;
+  for (int base = 0;; base += kWave) {
+    if (base > 0) mine = steps(base + lane);
+    const int n = mine < 0 ? 0 : max((int)(((uint32_t)mine + most - 1) / most), 1);
     const int upto = before + wave_scan(n);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kWave && b < a.B) a.plan[b] = make_int2(upto - n, n);
-    const uint64_t mine = __ballot(slot >= upto - n && slot < upto);
-    if (mine != 0 && !found) {
-      const int i = __builtin_ctzll(mine);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kWave && base + lane < a.B) a.plan[base + lane] = make_int2(upto - n, n);
+    const uint64_t here = __ballot(slot >= upto - n && slot < upto);
+    if (here != 0) {
+      const int i = __builtin_ctzll(here);
       p.b = base + i;
       p.first = __builtin_amdgcn_readlane(upto - n, i);
       p.splits = __builtin_amdgcn_readlane(n, i);
       p.split = slot - p.first;
-      found = true;
-      if (blockIdx.x != 0) break;
+      if (blockIdx.x != 0) return true;
     }
     before = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (base + kWave >= a.B) break;
   }
-  return found;
+  return blockIdx.x == 0 ? before > 0 : false;
 }
 
-// RG groups of 16 RT rows; the wavefronts of a group share its positions.
+// 4 wavefronts a workgroup: several workgroups a CU then hide each other's start, merge and end (48 requests of up to 9000
+// positions, 64 heads over 8: 25 us, 33 with 8 wavefronts and four slots each; 38000 positions, D = 256: 27.7 and 29.5).
+constexpr int kSplitWaves = 4;
+template <int D, int RT>
+constexpr int split_lds() {  // the slots, then the wavefronts' tiles
+  constexpr int slots = kSplitWaves * 2 * Walk<D, RT>::kSlot, merge = kSplitWaves * RT * D * 64;
+  return slots > merge ? slots : merge;
+}
+
+// RG groups of 16 RT rows; the wavefronts of a group share its positions.  A partial result is a tile of 16 rows x 16 values a
+// KiB, as the accumulators hold it: lane (row l16, quarter qg), the value that Walk::value_at names.  attn_combine_kernel adds them.
+// (Adding them in this launch, by the last split to arrive, took longer: its reads wait for the others' writes, their count and each
+// other, 1000 positions 9.6 against 8.8 us, 8000 positions 18.6 against 12.)
 template <int D, int RT, int RG>
-__global__ __launch_bounds__(kAttnThreads) void attn_split_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kSplitWaves * kWave) void attn_split_kernel(AttnArgs a) {
   using W = Walk<D, RT>;
-  constexpr int kShare = kAttnWaves / RG;  // wavefronts of a row group
-  extern __shared__ __align__(16) float lds[];  // [2][RT][D / 16][64 lanes x 4]
-  __shared__ float row_m[kAttnWaves][RT][16], row_l[kAttnWaves][RT][16];
+  constexpr int kWaves = kSplitWaves, kShare = kWaves / RG;  // wavefronts of a row group
+  constexpr int kTiles = RG * RT * W::kDTiles;
+  extern __shared__ __align__(16) uint8_t lds[];  // the slots, then [wavefront][RT][D / 16] tiles
+  __shared__ float row_m[kWaves][RT][16], row_l[kWaves][RT][16], row_inv[RG * RT][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rg = wave % RG, share = wave / RG;
   const int hkv = blockIdx.y;
@@ -460,16 +624,17 @@ __global__ __launch_bounds__(kAttnThreads) void attn_split_kernel(AttnArgs a) {
   w.start(r, p.b, hkv, rg * RT * 16);
   const int begin = p.split * p.chunk;  // below 2^31: split s > 0 starts inside the sequence
   const int end = min(r.seq - begin, p.chunk) + begin;
-  if (begin < end) w.run(begin, end, share, kShare);
+  w.run(begin, end, share, kShare, lds + wave * 2 * W::kSlot);
 
-  // ---- the wavefronts' states against their common reference ----
+  // ---- the wavefronts' states against their common reference, through LDS ----
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) w.l[rt] = quarters_sum(w.l[rt]);
   if (w.qg == 0) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) row_m[wave][rt][w.l16] = w.m[rt];
   }
-  __syncthreads();
+  __syncthreads();  // and every slot is done with
+  f32x4_t* const tiles = reinterpret_cast<f32x4_t*>(lds);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     float top = row_m[rg][rt][w.l16];
@@ -477,136 +642,318 @@ __global__ __launch_bounds__(kAttnThreads) void attn_split_kernel(AttnArgs a) {
     for (int i = 1; i < kShare; ++i) top = fmaxf(top, row_m[i * RG + rg][rt][w.l16]);
     const float keep = fast_exp2(w.m[rt] - (top == -__builtin_inff() ? 0.f : top));
     w.m[rt] = top;
-    w.l[rt] *= keep;
 #pragma unroll
-    for (int u = 0; u < W::kDTiles; ++u) w.o[rt][u] *= keep;
-    if (w.qg == 0) row_l[wave][rt][w.l16] = w.l[rt];
+    for (int u = 0; u < W::kDTiles; ++u) tiles[((wave * RT + rt) * W::kDTiles + u) * kWave + w.lane] = w.o[rt][u] * keep;
+    if (w.qg == 0) row_l[wave][rt][w.l16] = w.l[rt] * keep;
   }
-  auto at = [&](int half, int rt, int u) {
-    return reinterpret_cast<f32x4_t*>(lds) + ((half * RT + rt) * W::kDTiles + u) * kWave + w.lane;
-  };
-#pragma unroll
-  for (int from = kAttnWaves / 2; from >= RG; from /= 2) {  // wavefronts from .. 2 from - 1 hand theirs to 0 .. from - 1
-    if (wave >= from && wave < 2 * from) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int u = 0; u < W::kDTiles; ++u) *at(wave - from, rt, u) = w.o[rt][u];
-    }
-    __syncthreads();
-    if (wave < from) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int u = 0; u < W::kDTiles; ++u) w.o[rt][u] += *at(wave, rt, u);
-    }
-    if (from > RG) __syncthreads();
-  }
-  if (share != 0) return;
+  __syncthreads();
   const int rows = r.n * a.G;
-  const int64_t part = ((int64_t)hkv * a.slots + blockIdx.x) * a.rows;
+  const int64_t slot = (int64_t)hkv * a.slots + blockIdx.x;
+  auto none_seen = [&](int row) { return r.seq - r.n + divide(row, a.by_g) < 0; };
+  if (share == 0 && w.qg == 0) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = (rg * RT + rt) * 16 + w.l16;
-    w.l[rt] = row_l[rg][rt][w.l16];
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = (rg * RT + rt) * 16 + w.l16;
+      float l = row_l[rg][rt][w.l16];
 #pragma unroll
-    for (int i = 1; i < kShare; ++i) w.l[rt] += row_l[i * RG + rg][rt][w.l16];
-    if (row >= rows) continue;
-    if (p.splits == 1) {
-      w.write(r, hkv, row, rt);
-      continue;
+      for (int i = 1; i < kShare; ++i) l += row_l[i * RG + rg][rt][w.l16];
+      row_inv[rg * RT + rt][w.l16] = none_seen(row) ? 0.f : 1.f / l;
+      if (p.splits > 1 && row < rows) a.ml_part[slot * a.rows + row] = make_float2(w.m[rt], l);
     }
-    float* to = a.o_part + (part + row) * D;
+  }
+#pragma unroll 1
+  for (int k = wave; k < kTiles; k += kWaves) {  // tile u of row tile rt of row group g
+    const int g = k / (RT * W::kDTiles), at = (k - g * RT * W::kDTiles) * kWave + w.lane;
+    f32x4_t sum = tiles[g * RT * W::kDTiles * kWave + at];
 #pragma unroll
-    for (int h = 0; h < W::kHalves; ++h)
+    for (int i = 1; i < kShare; ++i) sum += tiles[(i * RG + g) * RT * W::kDTiles * kWave + at];
+    if (p.splits == 1) {
+      tiles[k * kWave + w.lane] = sum;  // (tile k of wavefront 0's, or of wavefront 1's where that is the second row group)
+    } else if (k / W::kDTiles * 16 + w.l16 < rows) {
+      reinterpret_cast<f32x4_t*>(a.o_part)[(slot * kTiles + k) * kWave + w.lane] = sum;
+    }
+  }
+  if (p.splits > 1) return;
+  __syncthreads();
+  const float* const sums = reinterpret_cast<const float*>(lds);
+#pragma unroll 1
+  for (int k = wave; k < RG * RT * W::kHalves * 4; k += kWaves) {  // component i of half h of row tile rt
+    const int i = k % 4, h = k / 4 % W::kHalves, rt = k / (4 * W::kHalves), row = rt * 16 + w.l16;
+    if (row >= rows) continue;
+    const int qi = divide(row, a.by_g);
+    const float inv = row_inv[rt][w.l16];
+    uint32_t v[W::kPerHalf / 2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < W::kPerHalf; n += 4) {
-          const int u = h * W::kPerHalf + n;
-          *reinterpret_cast<f32x4_t*>(to + w.value_at(h, i) + n) =
-              f32x4_t{w.o[rt][u][i], w.o[rt][u + 1][i], w.o[rt][u + 2][i], w.o[rt][u + 3][i]};
-        }
-    if (w.qg == 0) a.ml_part[part + row] = make_float2(w.m[rt], w.l[rt]);
+    for (int n = 0; n < W::kPerHalf / 2; ++n) {
+      const float* t = sums + ((rt * W::kDTiles + h * W::kPerHalf + 2 * n) * kWave + w.lane) * 4 + i;
+      v[n] = pack_bf16(t[0] * inv, t[4 * kWave] * inv);
+    }
+    uint16_t* to = a.out + (int64_t)(r.tok0 + qi) * a.so_t + (int64_t)(hkv * a.G + (row - qi * a.G)) * a.so_h + w.value_at(h, i);
+    if constexpr (W::kPerHalf == 8) {
+      *reinterpret_cast<u32x4_t*>(to) = u32x4_t{v[0], v[1], v[2], v[3]};
+    } else {
+      *reinterpret_cast<u32x2_t*>(to) = u32x2_t{v[0], v[1]};
+    }
   }
 }
 
-// A workgroup a packed row: D / 4 threads a split, the splits over 256 / (D / 4) groups of threads, then the groups in LDS.
+// A workgroup a pair of tiles (values n and n + 1 of each lane's run): 4 wavefronts a tile share the splits, up to 16 of which each
+// requests at once (they come from other XCDs' writes, a microsecond away); then the wavefronts through LDS.
+constexpr int kCombineWaves = 8;
 template <int D>
-__global__ __launch_bounds__(kAttnThreads) void attn_combine_kernel(AttnArgs a) {
-  constexpr int kLanes = D / 4, kGroups = kAttnThreads / kLanes;
-  __shared__ float sm_m[kGroups], sm_l[kGroups];
-  __shared__ __align__(16) f32x4_t sm_o[kGroups][kLanes];
-  const int b = blockIdx.x, row = blockIdx.y, hkv = blockIdx.z;
+__global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(AttnArgs a) {
+  using W = Walk<D, 1>;
+  constexpr int kGroups = kCombineWaves / 2;
+  __shared__ float sm_m[kGroups][kWave], sm_l[kGroups][kWave];
+  __shared__ __align__(16) f32x4_t sm_o[kCombineWaves][kWave];
+  const int pair = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tile = 2 * pair + wave % 2, g = wave / 2;
+  const int l16 = lane % 16, qg = lane / 16, row = tile / W::kDTiles * 16 + l16;
   const Request r = request(a, b);
   const int2 place = a.plan[b];
-  if (row >= r.n * a.G || place.y < 2) return;
-  const int g = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
-  const int64_t part = ((int64_t)hkv * a.slots + place.x) * a.rows + row;
+  const int rows = r.n * a.G;
+  if (place.y < 2 || tile / W::kDTiles * 16 >= rows) return;
+  const int kTiles = gridDim.x * 2;
+  const int64_t slot = (int64_t)hkv * a.slots + place.x;
   float m = -__builtin_inff(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = g; s < place.y; s += kGroups) {
-    const float2 ml = a.ml_part[part + (int64_t)s * a.rows];
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.o_part + (part + (int64_t)s * a.rows) * D + 4 * j);
-    const float top = fmaxf(m, ml.x);
-    const float ref = top == -__builtin_inff() ? 0.f : top;
-    const float keep = fast_exp2(m - ref), w = fast_exp2(ml.x - ref);
-    o = o * keep + v * w;
-    l = l * keep + ml.y * w;
-    m = top;
-  }
-  if (j == 0) {
-    sm_m[g] = m;
-    sm_l[g] = l;
-  }
-  sm_o[g][j] = o;
-  __syncthreads();
-  if (g != 0) return;
-  float top = sm_m[0];
+  if (row < rows) {
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.o_part) + tile * kWave + lane;
+    auto add = [&](int s, auto batch) {  // the splits s, s + kGroups, ... that there are, `batch` of them
+      constexpr int kBatch = decltype(batch)::value;
+      float2 ml[kBatch];
+      f32x4_t v[kBatch];
 #pragma unroll
-  for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sm_m[i]);
+      for (int i = 0; i < kBatch; ++i) {
+        const int at = min(s + i * kGroups, place.y - 1);
+        ml[i] = a.ml_part[(slot + at) * a.rows + row];
+        v[i] = from[(slot + at) * kTiles * kWave];
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (s + i * kGroups >= place.y) break;
+        const float top = fmaxf(m, ml[i].x);
+        const float ref = top == -__builtin_inff() ? 0.f : top;
+        const float keep = fast_exp2(m - ref), weight = fast_exp2(ml[i].x - ref);
+        o = o * keep + v[i] * weight;
+        l = l * keep + ml[i].y * weight;
+        m = top;
+      }
+    };
+    int s = g;
+    for (; s + 4 * kGroups < place.y; s += 16 * kGroups) add(s, std::integral_constant<int, 16>{});
+    if (s < place.y) add(s, std::integral_constant<int, 4>{});
+  }
+  if (wave % 2 == 0) {
+    sm_m[g][lane] = m;
+    sm_l[g][lane] = l;
+  }
+  sm_o[wave][lane] = o;
+  __syncthreads();
+  if (wave != 0 || row >= rows) return;
+  float top = sm_m[0][lane];
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sm_m[i][lane]);
   const float ref = top == -__builtin_inff() ? 0.f : top;
-  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f32x4_t even = {0.f, 0.f, 0.f, 0.f}, odd = even;
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    const float w = fast_exp2(sm_m[i] - ref);
-    o += sm_o[i][j] * w;
-    l += sm_l[i] * w;
+    const float weight = fast_exp2(sm_m[i][lane] - ref);
+    even += sm_o[2 * i][lane] * weight;
+    odd += sm_o[2 * i + 1][lane] * weight;
+    l += sm_l[i][lane] * weight;
   }
   const int qi = divide(row, a.by_g);
   const float inv = r.seq - r.n + qi < 0 ? 0.f : 1.f / l;
-  uint16_t* to = a.out + (int64_t)(r.tok0 + qi) * a.so_t + (int64_t)(hkv * a.G + (row - qi * a.G)) * a.so_h + 4 * j;
-  *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+  using Rec = Record<D>;
+  const int u = tile % W::kDTiles, h = u / W::kPerHalf, n = u % W::kPerHalf;
+  uint16_t* to = a.out + (int64_t)(r.tok0 + qi) * a.so_t + (int64_t)(hkv * a.G + (row - qi * a.G)) * a.so_h +
+                 16 * Rec::kWidth * h + Rec::kWidth * 4 * qg + n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(to + Rec::kWidth * i) = pack_bf16(even[i] * inv, odd[i] * inv);
 }
 
-// Rows 32 (4 x + wavefront) .. + 31 of request z, kv head y.
-constexpr int kTileRT = 2;
+// Many rows: 8 wavefronts with 16 kRT rows each walk over the same positions, 64 a stage.  Each wavefront reads the keys' codes
+// itself (the other seven find them in the cache next to the CU) and widens them; the values are widened once for all of them,
+// an eighth a wavefront, into LDS, in the order of the operand: two buffers, one barrier a stage.
 template <int D>
-__global__ __launch_bounds__(kAttnThreads) void attn_tile_kernel(AttnArgs a) {
+struct TileShape {
+  static constexpr int kRT = D == 256 ? 1 : 2;
+  static constexpr int kWaves = 8;
+  static constexpr int kRows = 16 * kRT * kWaves;
+};
+constexpr int kStage = 64;
+
+template <int D>
+__global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel(AttnArgs a) {
+  using S = TileShape<D>;
+  using W = Walk<D, S::kRT>;
+  using R = Record<D>;
+  __shared__ __align__(16) u32x2_t frags[2][2][W::kDTiles][kWave][2];  // [buffer][step][value tile][lane][record]
+  __shared__ uint32_t odd[2][S::kWaves];                              // a wavefront met a block of NaN that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int hkv = blockIdx.y, b = blockIdx.z;
   const Request r = request(a, b);
-  const int r0 = (blockIdx.x * kAttnWaves + wave) * 16 * kTileRT;
-  if (r0 >= r.n * a.G) return;
-  Walk<D, kTileRT> w(a);
+  const int rows = r.n * a.G;
+  const int row0 = (gridDim.x - 1 - blockIdx.x) * S::kRows;  // the rows that see most come first
+  if (row0 >= rows || rows <= a.few) return;
+  const int r0 = row0 + wave * 16 * S::kRT;
+  W w(a);
   w.start(r, b, hkv, r0);
-  const int last_row = min(r0 + 16 * kTileRT, r.n * a.G) - 1;
-  const int end = max(r.seq - r.n + divide(last_row, a.by_g) + 1, 0);
-  if (end > 0) w.run(0, end, 0, 1);
+  auto seen = [&](int row) { return max(r.seq - r.n + divide(min(row, rows - 1), a.by_g) + 1, 0); };
+  const int end = seen(row0 + S::kRows - 1), all_see = seen(row0);
+  const int n_stages = (end + kStage - 1) / kStage;
+  const int last_tile = (end - 1) / kTile * kTile;
+
+  // The records of 16 stages are looked up at once, a record a lane.
+  uint32_t rec_lo = 0, rec_hi = 0;
+  auto look_up = [&](int stage) {
+    const int64_t at = w.record(min(stage * kStage + w.lane * kTile, last_tile));
+    rec_lo = (uint32_t)at;
+    rec_hi = (uint32_t)(at >> 32);
+  };
+  auto where = [&](int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane(rec_lo, l), hi = __builtin_amdgcn_readlane(rec_hi, l);
+    return w.base + (int64_t)(((uint64_t)hi << 32) | lo);
+  };
+
+  // This wavefront's share of a stage's values: of record `mine` its half (D = 256) or half of its bytes.
+  constexpr int kBytes = D == 256 ? 4 : D / 64;  // of each lane's run: 2 kBytes tiles
+  const int mine = wave / 2, half = D == 256 ? wave % 2 : 0, byte0 = D == 256 ? 0 : wave % 2 * kBytes;
+  typename W::Data::Run v;
+  uint32_t vs;
+  auto load_values = [&](int stage) {
+    const uint8_t* rec = where(stage % 16 * 4 + mine);
+    v = *reinterpret_cast<const typename W::Data::Run*>(rec + R::kValues + half * 1024 + w.lane * 4 * W::kDwords);
+    vs = *reinterpret_cast<const uint32_t*>(rec + R::kValueScales + (W::kDwords == 4 ? 4 * half + w.l16 / 4 : w.l16 / 8) * kTile + 4 * w.qg);
+  };
+  auto widen_values = [&](int stage) {
+    const int pos = stage * kStage + mine * kTile;
+    if (pos + kTile > all_see) {  // behind the end anything may stand; a block of NaN would reach rows that do not see it
+      bool any = false;
 #pragma unroll
-  for (int rt = 0; rt < kTileRT; ++rt) {
+      for (int i = 0; i < 4; ++i) {
+        const bool gone = pos + 4 * w.qg + i >= end, nan = (vs >> (8 * i) & 255u) == 255u;
+        any |= nan && !gone;
+        if (gone || nan) {
+          vs = (vs & ~(255u << (8 * i))) | 127u << (8 * i);
+          if constexpr (W::kDwords == 4) {
+            v[i] = 0;
+          } else {
+            v[i / 2] &= i % 2 ? 0xffffu : 0xffff0000u;
+          }
+        }
+      }
+      const bool met = __any(any);
+      if (w.lane == 0) odd[stage & 1][wave] = met;
+    }
+    const uint32_t bytes = here(vs);
+    const float s[4] = {scale_of<0>(bytes), scale_of<1>(bytes), scale_of<2>(bytes), scale_of<3>(bytes)};
+    auto pair = [&](auto byte) {
+      constexpr int kB = decltype(byte)::value;
+      uint32_t x[4];
+      if constexpr (D == 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = widen2<kB>(v[i], s[i]);
+      } else if constexpr (D == 128) {  // bytes byte0 + kB, moved down
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = widen2<kB>(v[i] >> (8 * byte0), s[i]);
+      } else {
+        const uint32_t lo = v[0] >> (8 * byte0), hi = v[1] >> (8 * byte0);
+        x[0] = widen2<0>(lo, s[0]);
+        x[1] = widen2<2>(lo, s[1]);
+        x[2] = widen2<0>(hi, s[2]);
+        x[3] = widen2<2>(hi, s[3]);
+      }
+      const int u = half * W::kPerHalf + 2 * (byte0 + kB);
+      frags[stage & 1][mine / 2][u][w.lane][mine % 2] =
+          u32x2_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100), __builtin_amdgcn_perm(x[3], x[2], 0x05040100)};
+      frags[stage & 1][mine / 2][u + 1][w.lane][mine % 2] =
+          u32x2_t{__builtin_amdgcn_perm(x[1], x[0], 0x07060302), __builtin_amdgcn_perm(x[3], x[2], 0x07060302)};
+    };
+    pair(std::integral_constant<int, 0>{});
+    if constexpr (kBytes > 1) pair(std::integral_constant<int, 1>{});
+    if constexpr (kBytes > 2) {
+      pair(std::integral_constant<int, 2>{});
+      pair(std::integral_constant<int, 3>{});
+    }
+  };
+
+  // The scores of step i + 1 are computed beside the weights of step i, so that the matrix cores have work while the exponentials
+  // are computed.
+  const bool live = r0 < rows;
+  typename W::Data keys[2];
+  typename W::Scores sc[2];
+  auto key_records = [&](int i, auto&& take) { take(where(i % 32 * 2), where(i % 32 * 2 + 1)); };  // of step i, of those looked up
+  auto step = [&](int i, int buffer, auto parity) {
+    constexpr int kP = decltype(parity)::value;
+    key_records(i + 2, [&](auto* x, auto* y) { w.load_keys(keys[kP], x, y); });  // the keys of step i are used up
+    if (!live) return;
+    constexpr int kAhead = W::kDTiles < 8 ? W::kDTiles : 8;  // operands read before the scores; the others where registers are free
+    bf16x8_t vf[W::kDTiles];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) vf[u] = *reinterpret_cast<const bf16x8_t*>(&frags[buffer][kP][u][w.lane][0]);
+    if ((i + 1) * kStep > w.diag) w.mask(sc[kP], i * kStep);
+    w.refer(sc[kP]);
+    w.scores(keys[1 - kP], sc[1 - kP]);
+    bf16x8_t pf[S::kRT];
+    w.weigh(sc[kP], pf);
+    if constexpr (kAhead < W::kDTiles) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = kAhead; u < W::kDTiles; ++u) vf[u] = *reinterpret_cast<const bf16x8_t*>(&frags[buffer][kP][u][w.lane][0]);
+#pragma unroll
+    for (int u = 0; u < W::kDTiles; ++u)
+#pragma unroll
+      for (int rt = 0; rt < S::kRT; ++rt) w.o[rt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[u], pf[rt], w.o[rt][u], 0, 0, 0);
+  };
+  if (n_stages > 0) {
+    look_up(0);
+    load_values(0);
+    key_records(0, [&](auto* x, auto* y) { w.load_keys(keys[0], x, y); });
+    key_records(1, [&](auto* x, auto* y) { w.load_keys(keys[1], x, y); });
+    widen_values(0);
+    w.scores(keys[0], sc[0]);
+  }
+#pragma unroll 1
+  for (int stage = 0; stage < n_stages; ++stage) {
+    ring_barrier();  // this stage's values stand, the stage before is done with
+    if ((stage + 1) % 16 == 0) look_up(stage + 1);  // past the last stage: its last record again
+    load_values(stage + 1);
+    step(2 * stage, stage & 1, std::integral_constant<int, 0>{});
+    step(2 * stage + 1, stage & 1, std::integral_constant<int, 1>{});
+    if ((stage + 1) * kStage > all_see) {
+      uint32_t met = 0;
+#pragma unroll
+      for (int i = 0; i < S::kWaves; ++i) met |= (stage * kStage + i / 2 * kTile + kTile > all_see) ? odd[stage & 1][i] : 0u;
+      if (met != 0) w.mark_nan(max(stage * kStage, all_see / kTile * kTile), min((stage + 1) * kStage, end));
+    }
+    if (stage + 1 < n_stages) widen_values(stage + 1);
+  }
+#pragma unroll
+  for (int rt = 0; rt < S::kRT; ++rt) {
     w.l[rt] = quarters_sum(w.l[rt]);
     const int row = r0 + rt * 16 + w.l16;
-    if (row < r.n * a.G) w.write(r, hkv, row, rt);
+    if (row < rows) w.write(r, hkv, row, rt);
   }
 }
 
 typedef void (*AttnFn)(AttnArgs);
 
+struct Split {
+  AttnFn fn;
+  int row_tiles, threads, lds;
+};
 template <int D>
-AttnFn split_kernel(int rt) {
-  return rt == 1 ? &attn_split_kernel<D, 1, 1> : rt == 2 ? &attn_split_kernel<D, 2, 1> : &attn_split_kernel<D, 2, 2>;
+Split split_kernel(int rt) {
+  constexpr int threads = kSplitWaves * kWave;
+  if (rt == 1) return {&attn_split_kernel<D, 1, 1>, 1, threads, split_lds<D, 1>()};
+  if (rt == 2) return {&attn_split_kernel<D, 2, 1>, 2, threads, split_lds<D, 2>()};
+  return {&attn_split_kernel<D, 2, 2>, 4, threads, split_lds<D, 2>()};
+}
+Split split_of(int D, int rows) {
+  const int rt = (rows + 15) / 16;
+  return D == 64 ? split_kernel<64>(rt) : D == 128 ? split_kernel<128>(rt) : split_kernel<256>(rt);
 }
 
 int compute_units() {
@@ -623,27 +970,32 @@ int compute_units() {
 
 // How a call runs: its launches and the parts of its workspace.
 struct Plan {
-  bool split;
+  bool tiles, split;  // the tile kernel; the split kernel with the combination
   int workers, slots, rows;
   size_t o, ml, plan, bytes;  // offsets and size of the workspace
 };
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Requests of up to QF_KV4_MAX_ROWS packed rows are split over positions, larger ones tiled over rows; a batch with lengths of its
+// own may hold both kinds (a chunk of 700 tokens beside single ones of 4000 positions).
 Plan plan_of(const qf_kv4_attention_args& u) {
   Plan p = {};
   const int64_t rows = (int64_t)u.q_len * (u.num_heads / u.num_kv_heads);
-  p.split = rows <= QF_KV4_MAX_ROWS;
+  p.tiles = rows > QF_KV4_MAX_ROWS;
+  p.split = !p.tiles || u.cu_q != nullptr;
   if (!p.split) return p;
-  p.rows = (int)rows;
-  const int cus = compute_units();
+  p.rows = rows < QF_KV4_MAX_ROWS ? (int)rows : QF_KV4_MAX_ROWS;
+  // A workgroup a CU; two where the requests by themselves fill the machine, so that the longest of them is cut finer (48 requests
+  // of up to 9000 positions over 8 kv heads: 28.2 -> 25.0 us; 16 requests of up to 3000, which do not: 18.8 -> 22.7).
+  const int cus = compute_units() * ((int64_t)u.num_reqs * u.num_kv_heads >= compute_units() ? 2 : 1);
   p.workers = (cus + u.num_kv_heads - 1) / u.num_kv_heads;
   p.slots = p.workers + u.num_reqs;
-  size_t n = QF_W8A16_COUNTER_BYTES;
-  const size_t parts = (size_t)u.num_kv_heads * p.slots * p.rows;
+  size_t n = 0;
+  const size_t parts = (size_t)u.num_kv_heads * p.slots;
   p.o = n;
-  n += round256(parts * u.head_size * sizeof(float));
+  n += parts * split_of(u.head_size, p.rows).row_tiles * 16 * u.head_size * sizeof(float);
   p.ml = n;
-  n += round256(parts * sizeof(float2));
+  n += round256(parts * p.rows * sizeof(float2));
   p.plan = n;
   p.bytes = n + round256((size_t)u.num_reqs * sizeof(int2));
   return p;
@@ -657,9 +1009,9 @@ bool sizes_fit(const qf_kv4_attention_args& u) {
 
 std::atomic<uint64_t> g_raised[3][5];
 
-int launch(AttnFn fn, dim3 grid, size_t lds, std::atomic<uint64_t>& raised, hipStream_t s, const AttnArgs& a) {
+int launch(AttnFn fn, dim3 grid, int threads, size_t lds, std::atomic<uint64_t>& raised, hipStream_t s, const AttnArgs& a) {
   if (lds + 4096 > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(fn), (int)lds, raised)) return QF_ERR_HIP;
-  hipLaunchKernelGGL(fn, grid, dim3(kAttnThreads), lds, s, a);
+  hipLaunchKernelGGL(fn, grid, dim3(threads), lds, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
 
@@ -678,7 +1030,7 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
       u.bt_stride < 0 || u.num_tokens < 1 || u.num_reqs < 1 || u.q_len < 1 || u.num_heads < 1 || u.num_kv_heads < 1 ||
       u.page_size < 1 || !(u.scale == u.scale) || (!u.cu_q && (int64_t)u.num_reqs * u.q_len > u.num_tokens))
     return QF_ERR_INVALID_ARG;
-  if (!sizes_fit(u) || u.page_size % kTile || u.cache_stride % 16 || !aligned16(u.cache) ||
+  if (!sizes_fit(u) || (int64_t)u.max_blocks * u.page_size > 0x7fffffc0 || u.page_size % kTile || u.cache_stride % 16 || !aligned16(u.cache) ||
       u.cache_stride < (int64_t)u.num_kv_heads * (u.page_size / kTile) * 17 * u.head_size)
     return QF_ERR_UNSUPPORTED;
   for (const qf_heads* h : {&u.query, &u.out})
@@ -710,27 +1062,30 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   a.page = u.page_size;
   a.max_blocks = u.max_blocks;
   a.rows = p.rows;
+  a.few = p.split ? p.rows : 0;
   a.workers = p.workers;
   a.slots = p.slots;
-  a.qk_scale = u.scale * kLog2e;
+  a.qk_scale = fmaxf(fabsf(u.scale) * kLog2e, FLT_MIN);  // not 0: a masked score is -inf
+  a.flip = u.scale < 0 ? 0x80008000u : 0;
   a.by_g = divisor(a.G);
   a.by_page = divisor(u.page_size);
+  a.by_workers = divisor(p.split ? p.workers : 1);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int D = u.head_size, di = D == 64 ? 0 : D == 128 ? 1 : 2;
-  if (!p.split) {
+  if (p.tiles) {
     const int64_t rows = (int64_t)u.q_len * a.G;
-    const int per = kAttnWaves * 16 * kTileRT;
+    const int per = D == 256 ? TileShape<256>::kRows : TileShape<128>::kRows;
+    static_assert(TileShape<64>::kRows == TileShape<128>::kRows && TileShape<256>::kWaves == TileShape<128>::kWaves, "one shape");
     const AttnFn fn = D == 64 ? &attn_tile_kernel<64> : D == 128 ? &attn_tile_kernel<128> : &attn_tile_kernel<256>;
-    return launch(fn, dim3((unsigned)((rows + per - 1) / per), a.HKV, a.B), 0, g_raised[di][0], s, a);
+    const int st = launch(fn, dim3((unsigned)((rows + per - 1) / per), a.HKV, a.B), TileShape<128>::kWaves * kWave, 0, g_raised[di][0], s, a);
+    if (st != QF_OK || !p.split) return st;
   }
   a.o_part = reinterpret_cast<float*>(ws + p.o);
   a.ml_part = reinterpret_cast<float2*>(ws + p.ml);
   a.plan = reinterpret_cast<int2*>(ws + p.plan);
-  const int rt = (p.rows + 15) / 16;
-  const AttnFn fn = D == 64 ? split_kernel<64>(rt) : D == 128 ? split_kernel<128>(rt) : split_kernel<256>(rt);
+  const Split k = split_of(D, p.rows);
   const AttnFn comb = D == 64 ? &attn_combine_kernel<64> : D == 128 ? &attn_combine_kernel<128> : &attn_combine_kernel<256>;
-  const size_t lds = (size_t)2 * (rt == 1 ? 1 : 2) * 16 * D * sizeof(float);  // the first round of the wavefronts' merge
-  const int st = launch(fn, dim3(p.slots, a.HKV), lds, g_raised[di][rt], s, a);
+  const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, k.lds, g_raised[di][k.row_tiles], s, a);
   if (st != QF_OK) return st;
-  return launch(comb, dim3(a.B, p.rows, a.HKV), 0, g_raised[di][0], s, a);
+  return launch(comb, dim3(k.row_tiles * D / 32, a.HKV, a.B), kCombineWaves * kWave, 0, g_raised[di][0], s, a);
 }

@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -115,8 +116,10 @@ PyObject* tables(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                                 (int)bt->size(1), ptr<int32_t>(*stack), ptr<int32_t>(*count), (int)stack->size(0), (int)B,
                                 (int)page, (int)T, s, s + at_seq, t, t + T, s + at_held, s + at_count, s + at_fits, stream);
   if (rc != QF_OK) return PyLong_FromLong(rc);
-  at::Tensor out[] = {small.narrow(0, 0, B + 1), small.narrow(0, at_seq, B), tokens.select(0, 0), tokens.select(0, 1),
-                      small.narrow(0, at_held, B), small.narrow(0, at_count, 1), small.narrow(0, at_fits, 1)};
+  at::AutoDispatchBelowADInplaceOrView guard;  // views of fresh integer tensors: nothing for autograd
+  const auto part = [](const at::Tensor& of, int64_t from, int64_t n) { return of.as_strided({n}, {1}, from); };
+  at::Tensor out[] = {part(small, 0, B + 1), part(small, at_seq, B), part(tokens, 0, T), part(tokens, T, T),
+                      part(small, at_held, B), part(small, at_count, 1), part(small, at_fits, 1)};
   PyObject* all = PyTuple_New(7);
   for (int i = 0; all != nullptr && i < 7; ++i) {
     PyObject* o = THPVariable_Wrap(std::move(out[i]));
@@ -261,25 +264,24 @@ PyObject* load(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// attention(query, cache, seq_lens, block_table, scale, q_len, cu_q, out, workspace, device, stream) -> out.
-// workspace(cache, bytes): a buffer whose first QF_W8A16_COUNTER_BYTES bytes are zero.
+// attention(query, cache, seq_lens, block_table, scale, q_len, cu_q, out, device, stream) -> out.
 PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  if (!ready(n_args, 11, "attention")) return nullptr;
+  if (!ready(n_args, 10, "attention")) return nullptr;
   qf_kv4_attention_args u = {};
   u.scale = (float)PyFloat_AsDouble(args[4]);
-  const int64_t q_len = PyLong_AsLongLong(args[5]), device = PyLong_AsLongLong(args[9]);
-  void* const stream = (void*)PyLong_AsUnsignedLongLong(args[10]);
+  const int64_t q_len = PyLong_AsLongLong(args[5]), device = PyLong_AsLongLong(args[8]);
+  void* const stream = (void*)PyLong_AsUnsignedLongLong(args[9]);
   if (PyErr_Occurred()) return nullptr;
   const at::Tensor *query, *c, *seq, *bt, *cu, *out;
   int64_t HK, D, page;
   if (!unpack(args[0], device, &query) || !unpack(args[1], device, &c) || !unpack(args[2], device, &seq) ||
       !unpack(args[3], device, &bt) || !unpack_or_none(args[6], device, &cu) || !unpack_or_none(args[7], device, &out) ||
-      !cache4(*c, &HK, &D, &page) || query->dim() != 3 || seq->dim() != 1)
+      !cache4(*c, &HK, &D, &page) || query->dim() != 3 || seq->dim() != 1 || bt->dim() != 2)
     Py_RETURN_NONE;
   const int64_t T = query->size(0), H = query->size(1), B = seq->size(0);
   if (T < 1 || T > kIntMax || B < 1 || B > kIntMax || H < 1 || H > kIntMax || HK > kIntMax || H % HK || q_len < 1 ||
-      q_len > kIntMax || !heads(*query, T, H, D, &u.query) || !vec(*seq, at::kInt, B) || !table(*bt, B, &u.bt_stride) ||
+      q_len > kIntMax || bt->size(1) * page > 0x7fffffc0 || !heads(*query, T, H, D, &u.query) || !vec(*seq, at::kInt, B) || !table(*bt, B, &u.bt_stride) ||
       !(u.scale == u.scale) || (cu != nullptr ? !vec(*cu, at::kInt, B + 1) : B * q_len > T))
     Py_RETURN_NONE;
   u.cache = c->data_ptr();
@@ -303,15 +305,9 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   }
   if (!heads(*out, T, H, D, &u.out) || !separate(u.out, T, H, D)) Py_RETURN_NONE;
   const size_t bytes = qf_kv4_attention_workspace_bytes(&u);
-  at::Tensor ws;
-  if (bytes > 0) {
-    PyObject* o = PyObject_CallFunction(args[8], "OK", args[1], (unsigned long long)bytes);
-    if (o == nullptr) return nullptr;
-    if (THPVariable_Check(o)) ws = THPVariable_Unpack(o);  // kept by its owner
-    Py_DECREF(o);
-    if (!ws.defined()) Py_RETURN_NONE;
-  }
-  const int rc = qf_kv4_attention(&u, bytes ? ws.data_ptr() : nullptr, bytes ? (size_t)ws.numel() : 0, stream);
+  at::Tensor ws;  // the caching allocator's: one a call, capture-safe
+  if (bytes > 0) ws = at::empty({(int64_t)bytes}, c->options());
+  const int rc = qf_kv4_attention(&u, bytes ? ws.data_ptr() : nullptr, bytes, stream);
   if (rc != QF_OK) return PyLong_FromLong(rc);
   if (made.defined()) return THPVariable_Wrap(std::move(made));
   Py_INCREF(args[7]);

@@ -262,8 +262,8 @@ __global__ __launch_bounds__(kRopeThreads) void kv4_load_kernel(LoadArgs a) {
       w = *reinterpret_cast<const uint16_t*>(rec + R::value(q, 8 * j)) |
           (uint32_t)*reinterpret_cast<const uint16_t*>(rec + R::value(q, 8 * j + 4)) << 16;
     }
-    k = widen8(*reinterpret_cast<const uint32_t*>(rec + R::key(q, 8 * j)), scale_f32(rec[R::key_scale(q, 8 * j)]));
-    v = widen8(w, scale_f32(rec[R::value_scale(q, 8 * j)]));
+    k = widen8(*reinterpret_cast<const uint32_t*>(rec + R::key(q, 8 * j)), scale_of<0>(rec[R::key_scale(q, 8 * j)]));
+    v = widen8(w, scale_of<0>(rec[R::value_scale(q, 8 * j)]));
   }
   *reinterpret_cast<u32x4_t*>(a.key + at * D + 8 * j) = k;
   *reinterpret_cast<u32x4_t*>(a.value + at * D + 8 * j) = v;

@@ -14,7 +14,6 @@ import torch
 
 from . import _kv4_lib as K
 from .rope import _run
-from .w8a16 import _workspace
 
 
 def kv4_cache(num_blocks: int, page_size: int, num_kv_heads: int, head_size: int, device="cuda") -> torch.Tensor:
@@ -52,10 +51,6 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor) -> Tuple[torch.Tensor, to
     return K.call("load", dev, K.plain(cache), slots)
 
 
-def _zeroed(cache: torch.Tensor, nbytes: int) -> torch.Tensor:
-    return _workspace(cache.device, nbytes)
-
-
 def kv4_attention(query: torch.Tensor, cache: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, scale: float, *,
                   q_len: Optional[int] = None, cu_q: Optional[torch.Tensor] = None, max_q: Optional[int] = None,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -73,12 +68,12 @@ def kv4_attention(query: torch.Tensor, cache: torch.Tensor, seq_lens: torch.Tens
         raise ValueError("q_len is given, or cu_q with max_q")
     most = int(q_len if cu_q is None else max_q)
     if query.is_cuda:
-        r = K.try_call("attention", query, cache, seq_lens, block_table, scale, most, cu_q, out, _zeroed)
+        r = K.try_call("attention", query, cache, seq_lens, block_table, scale, most, cu_q, out)
         if r is not None:
             return r
     D = K.head_size(query, "query")
     T, H = query.shape[:2]
-    h, d, _ = K.cache_sizes(cache)
+    h, d, page = K.cache_sizes(cache)
     dev = K.gpu(query, cache, seq_lens, block_table, cu_q, out)
     if d != D or H % h:
         raise ValueError(f"the cache holds {h} heads of {d} values, query has {H} of {D}")
@@ -91,6 +86,8 @@ def kv4_attention(query: torch.Tensor, cache: torch.Tensor, seq_lens: torch.Tens
     if (block_table.shape[1] > 1 and block_table.stride(1) != 1) or (
             block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
         block_table = block_table.contiguous()
+    if block_table.shape[1] * page > 0x7FFFFFC0:
+        raise ValueError(f"a row of the table holds up to {0x7FFFFFC0} positions, got {block_table.shape[1]} pages of {page}")
     if scale != scale:
         raise ValueError("scale is NaN")
     if most < 1:
@@ -104,4 +101,4 @@ def kv4_attention(query: torch.Tensor, cache: torch.Tensor, seq_lens: torch.Tens
     query = K.heads(query, (T, H, D), "query")
     if T == 0 or B == 0:
         return query.new_empty((T, H, D)) if out is None else out
-    return K.call("attention", dev, query, K.plain(cache), seq_lens, K.plain(block_table), scale, most, cu_q, out, _zeroed)
+    return K.call("attention", dev, query, K.plain(cache), seq_lens, K.plain(block_table), scale, most, cu_q, out)

@@ -123,14 +123,14 @@ def _attention(ws=P, nbytes=1 << 40, **kw):
     (dict(cache_stride=2 * 17 * 128 + 4), UNSUPPORTED), (dict(cache_stride=17 * 128), UNSUPPORTED), (dict(cache=P + 8), UNSUPPORTED),
     (dict(query=K.Heads(P + 8, 1024, 128)), UNSUPPORTED), (dict(out=K.Heads(P, 1028, 128)), UNSUPPORTED),
     (dict(query=K.Heads(P, 1024, -128)), UNSUPPORTED), (dict(num_reqs=65536, num_tokens=1 << 20), UNSUPPORTED),
-    (dict(q_len=1 << 30, num_tokens=1 << 30, cu_q=P), UNSUPPORTED)])
+    (dict(q_len=1 << 30, num_tokens=1 << 30, cu_q=P), UNSUPPORTED), (dict(max_blocks=1 << 27), UNSUPPORTED)])
 def test_attention_refusals(kw, want):
     assert _attention(**kw)[0] == want
 
 
 def test_attention_workspace():
     need = _attention(ws=None)[1]
-    assert need > 65536 and _attention(ws=None)[0] == WORKSPACE
+    assert need > 0 and _attention(ws=None)[0] == WORKSPACE
     assert _attention(nbytes=need - 1)[0] == WORKSPACE and _attention(ws=P + 8)[0] == WORKSPACE
     assert _attention(num_heads=9)[1] == 0 and _attention(head_size=96)[1] == 0 and _attention(q_len=0)[1] == 0
 
@@ -194,6 +194,7 @@ WRONG = [
     ("attention", dict(query=z(6, 4, 64, dtype=BF16))), ("attention", dict(seq_lens=z(3, dtype=I64))),
     ("attention", dict(seq_lens=z(3, 1, dtype=I32))), ("attention", dict(block_table=z(2, 2, dtype=I32))),
     ("attention", dict(block_table=z(3, 2, dtype=I64))), ("attention", dict(block_table=z(3, 0, dtype=I32))),
+    ("attention", dict(block_table=z(1, dtype=I32).expand(3, 1 << 27))),
     ("attention", dict(scale=float("nan"))), ("attention", dict(out=z(5, 4, 128, dtype=BF16))), ("attention", dict(out=z(6, 4, 128))),
 ]
 
