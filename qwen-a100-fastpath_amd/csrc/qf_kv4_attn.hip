@@ -42,6 +42,7 @@ struct AttnArgs {
   float* o_part;   // [HKV][slots][rows][D]
   float2* ml_part; // [HKV][slots][rows]: exponent reference, sum
   int2* plan;      // [B]: first slot and slots of a request
+  int row_tiles, tile_splits;  // tile kernel: of a request at most, and of a row tile at most; partials [B][HKV][row tile][split]
   int slots;
 };
 
@@ -145,19 +146,6 @@ struct Walk {
     return block * a.stride + (pos - pg * a.page) / kTile * R::kBytes;
   }
 
-  __device__ __forceinline__ void load_keys(Data& s, const uint8_t* r0, const uint8_t* r1) const {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint8_t* r = t == 0 ? r0 : r1;
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const uint8_t* p = r + l16 * (D / 2) + h * 64 + qg * (4 * kDwords);
-        s.k[t][h] = *reinterpret_cast<const typename Data::Run*>(p);
-        s.ks[t][h] = *reinterpret_cast<const uint32_t*>(r + R::kKeyScales + (kDwords == 4 ? 4 * h + qg : qg / 2) * kTile + (l16 & 12));
-      }
-    }
-  }
-
   // A value's block of NaN at a position that some rows see and others do not: the product would give it to all rows.  Where a
   // step holds one, its scales are cleared for the product and the rows that see it are made NaN here.
   __device__ __forceinline__ void masked_nan(Data& s, int pos, int end) {
@@ -253,13 +241,22 @@ struct Walk {
 
   // The rows' exponent references brought up to the scores.  A reference moves only when a score exceeds it by 2^8: the weights
   // stay below that, and the accumulators are rarely rescaled.  The result is that of the running maximum up to rounding.
-  __device__ __forceinline__ void refer(const Scores& sc) {
+  template <int N>
+  __device__ __forceinline__ void refer(const Scores (&sc)[N]) {
     bool above = false;
     float mx[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const f32x4_t x = sc[rt][0], y = sc[rt][1];
-      mx[rt] = a.qk_scale * largest(largest(largest(largest(x[0], x[1]), x[2]), largest(largest(x[3], y[0]), y[1])), largest(y[2], y[3]));
+      float top = sc[0][rt][0][0];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const f32x4_t x = sc[n][rt][0], y = sc[n][rt][1];
+        top = largest(largest(top, x[1]), n == 0 ? x[2] : x[0]);
+        top = largest(largest(top, n == 0 ? x[3] : x[2]), y[0]);
+        top = largest(largest(top, y[1]), y[2]);
+        top = n == 0 ? largest(top, y[3]) : largest(largest(top, x[3]), y[3]);
+      }
+      mx[rt] = a.qk_scale * top;
       above |= mx[rt] > m[rt] + kRescale;
     }
     if (__any(above)) {
@@ -290,7 +287,8 @@ struct Walk {
 
   // Positions pos .. pos + 31, those from `end` on hold nothing.
   __device__ __forceinline__ void step(Data& s, int pos, int end) {
-    Scores sc;
+    Scores all[1];
+    Scores& sc = all[0];
     scores(s, sc);
     if (pos + kStep > diag || pos + kStep > end) {
       mask(sc, pos);
@@ -313,7 +311,7 @@ struct Walk {
       }
       masked_nan(s, pos, end);
     }
-    refer(sc);
+    refer(all);
     bf16x8_t pf[RT];
     weigh(sc, pf);
 #pragma unroll
@@ -697,24 +695,262 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void attn_split_kernel(AttnArg
   }
 }
 
+// Many rows: 8 wavefronts with 16 kRT rows each walk over the same positions, 64 a stage.  A stage's keys and values are widened
+// once for all of them, an eighth a wavefront, into LDS, in the order of the operands (8 KiB of fragments a wavefront and step of
+// either, at D = 128): two buffers, one barrier a stage.
+template <int D>
+struct TileShape {
+  static constexpr int kRT = D == 256 ? 1 : 2;
+  static constexpr int kWaves = 8;
+  static constexpr int kRows = 16 * kRT * kWaves;
+  static constexpr int kFragments = 4 * (D / 32) + 2 * (D / 16);  // KiB of a stage: 4 records' keys, 2 steps' values
+  static constexpr int kLds = 2 * kFragments * 1024;
+};
+constexpr int kStage = 64;
+
+// The stages of a row tile that sees the positions below `end`, over at most a.tile_splits workgroups of 4 stages or more.
+__device__ __forceinline__ void stage_splits(const AttnArgs& a, int end, int& splits, int& per) {
+  const int n = max((end + kStage - 1) / kStage, 1);
+  splits = min(a.tile_splits, max(n / 4, 1));
+  per = (n + splits - 1) / splits;
+  splits = (n + per - 1) / per;
+}
+__device__ __forceinline__ int64_t tile_slot(const AttnArgs& a, int b, int hkv, int row_tile) {
+  return (((int64_t)b * a.HKV + hkv) * a.row_tiles + row_tile) * a.tile_splits;
+}
+
+template <int D>
+__global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel(AttnArgs a) {
+  using S = TileShape<D>;
+  using W = Walk<D, S::kRT>;
+  using R = Record<D>;
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ uint32_t odd[2][S::kWaves];  // a wavefront met a block of NaN that not all rows see
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int hkv = blockIdx.y, b = blockIdx.z;
+  const Request r = request(a, b);
+  const int rows = r.n * a.G;
+  const int row_tile = a.row_tiles - 1 - blockIdx.x / a.tile_splits;  // the rows that see most come first
+  const int row0 = row_tile * S::kRows;
+  if (row0 >= rows || rows <= a.few) return;
+  const int r0 = row0 + wave * 16 * S::kRT;
+  W w(a);
+  w.start(r, b, hkv, r0);
+  auto seen = [&](int row) { return max(r.seq - r.n + divide(min(row, rows - 1), a.by_g) + 1, 0); };
+  const int own_end = r0 < rows ? seen(r0 + 16 * S::kRT - 1) : 0;  // positions that a row of this wavefront sees
+  const int end = seen(row0 + S::kRows - 1), all_see = seen(row0);
+  int splits, per;
+  stage_splits(a, end, splits, per);
+  const int split = blockIdx.x % a.tile_splits;
+  if (split >= splits) return;
+  const int first_stage = split * per, n_stages = min((end + kStage - 1) / kStage, first_stage + per);
+  const int last_tile = (end - 1) / kTile * kTile;
+
+  // fragment f of a stage's keys (record f / (D / 32)), and of its values (step f / (D / 16))
+  auto key_at = [&](int buffer, int f) { return lds + ((buffer * S::kFragments + f) * kWave + w.lane) * 16; };
+  auto value_at = [&](int buffer, int f) { return key_at(buffer, 4 * W::kKSteps + f); };
+
+  // The records of 16 stages are looked up at once, a record a lane.
+  uint32_t rec_lo = 0, rec_hi = 0;
+  auto look_up = [&](int stage) {
+    const int64_t at = w.record(min(stage * kStage + w.lane * kTile, last_tile));
+    rec_lo = (uint32_t)at;
+    rec_hi = (uint32_t)(at >> 32);
+  };
+  auto where = [&](int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane(rec_lo, l), hi = __builtin_amdgcn_readlane(rec_hi, l);
+    return w.base + (int64_t)(((uint64_t)hi << 32) | lo);
+  };
+
+  // This wavefront's share of a stage: of record `mine` a half of each lane's run (D = 256: one of its halves).
+  const int mine = wave / 2, part = wave % 2, half = D == 256 ? part : 0;
+  constexpr int kKeyDwords = D == 256 ? 4 : W::kDwords / 2;  // of each lane's keys
+  constexpr int kBytes = D == 256 ? 4 : D / 64;              // of each lane's run of values: 2 kBytes tiles
+  const int byte0 = D == 256 ? 0 : part * kBytes;
+  typedef uint32_t Keys __attribute__((ext_vector_type(kKeyDwords)));
+  Keys k;
+  typename W::Data::Run v;
+  uint32_t ks, vs;
+  auto load_share = [&](int stage) {
+    const uint8_t* rec = where(stage % 16 * 4 + mine);
+    k = *reinterpret_cast<const Keys*>(rec + w.l16 * (D / 2) + half * 64 + w.qg * (4 * W::kDwords) + (D == 256 ? 0 : part * 4 * kKeyDwords));
+    v = *reinterpret_cast<const typename W::Data::Run*>(rec + R::kValues + half * 1024 + w.lane * 4 * W::kDwords);
+    ks = *reinterpret_cast<const uint32_t*>(rec + R::kKeyScales + (W::kDwords == 4 ? 4 * half + w.qg : w.qg / 2) * kTile + (w.l16 & 12));
+    vs = *reinterpret_cast<const uint32_t*>(rec + R::kValueScales + (W::kDwords == 4 ? 4 * half + w.l16 / 4 : w.l16 / 8) * kTile + 4 * w.qg);
+  };
+  auto widen_share = [&](int stage) {
+    const int pos = stage * kStage + mine * kTile, buffer = stage & 1;
+    const float scale = w.key_scale(ks);
+    const int f = mine * W::kKSteps + (D == 256 ? half * W::kDwords : part * kKeyDwords);
+#pragma unroll
+    for (int c = 0; c < kKeyDwords; ++c) *reinterpret_cast<u32x4_t*>(key_at(buffer, f + c)) = widen8(k[c], scale);
+    if (pos + kTile > all_see) {  // behind the end anything may stand; a block of NaN would reach rows that do not see it
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool gone = pos + 4 * w.qg + i >= end, nan = (vs >> (8 * i) & 255u) == 255u;
+        any |= nan && !gone;
+        if (gone || nan) {
+          vs = (vs & ~(255u << (8 * i))) | 127u << (8 * i);
+          if constexpr (W::kDwords == 4) {
+            v[i] = 0;
+          } else {
+            v[i / 2] &= i % 2 ? 0xffffu : 0xffff0000u;
+          }
+        }
+      }
+      const bool met = __any(any);
+      if (w.lane == 0) odd[buffer][wave] = met;
+    }
+    const uint32_t bytes = here(vs);
+    const float s[4] = {scale_of<0>(bytes), scale_of<1>(bytes), scale_of<2>(bytes), scale_of<3>(bytes)};
+    auto pair = [&](auto byte) {
+      constexpr int kB = decltype(byte)::value;
+      uint32_t x[4];
+      if constexpr (D == 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = widen2<kB>(v[i], s[i]);
+      } else if constexpr (D == 128) {  // bytes byte0 + kB, moved down
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = widen2<kB>(v[i] >> (8 * byte0), s[i]);
+      } else {
+        const uint32_t lo = v[0] >> (8 * byte0), hi = v[1] >> (8 * byte0);
+        x[0] = widen2<0>(lo, s[0]);
+        x[1] = widen2<2>(lo, s[1]);
+        x[2] = widen2<0>(hi, s[2]);
+        x[3] = widen2<2>(hi, s[3]);
+      }
+      const int u = mine / 2 * W::kDTiles + half * W::kPerHalf + 2 * (byte0 + kB);
+      *reinterpret_cast<u32x2_t*>(value_at(buffer, u) + mine % 2 * 8) =
+          u32x2_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100), __builtin_amdgcn_perm(x[3], x[2], 0x05040100)};
+      *reinterpret_cast<u32x2_t*>(value_at(buffer, u + 1) + mine % 2 * 8) =
+          u32x2_t{__builtin_amdgcn_perm(x[1], x[0], 0x07060302), __builtin_amdgcn_perm(x[3], x[2], 0x07060302)};
+    };
+    pair(std::integral_constant<int, 0>{});
+    if constexpr (kBytes > 1) pair(std::integral_constant<int, 1>{});
+    if constexpr (kBytes > 2) {
+      pair(std::integral_constant<int, 2>{});
+      pair(std::integral_constant<int, 3>{});
+    }
+  };
+
+  auto compute = [&](int pos, int buffer) {
+    if (pos >= own_end) return;
+    typename W::Scores sc[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int rt = 0; rt < S::kRT; ++rt) sc[n][rt][0] = sc[n][rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < W::kKSteps; ++c) {
+        const bf16x8_t f0 = *reinterpret_cast<const bf16x8_t*>(key_at(buffer, 2 * n * W::kKSteps + c));
+        const bf16x8_t f1 = *reinterpret_cast<const bf16x8_t*>(key_at(buffer, (2 * n + 1) * W::kKSteps + c));
+#pragma unroll
+        for (int rt = 0; rt < S::kRT; ++rt) {
+          sc[n][rt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f0, w.qf[rt][c], sc[n][rt][0], 0, 0, 0);
+          sc[n][rt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f1, w.qf[rt][c], sc[n][rt][1], 0, 0, 0);
+        }
+      }
+    }
+    constexpr int kAhead = W::kDTiles < 8 ? W::kDTiles : 8;  // operands requested before they are needed
+    bf16x8_t vf[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) vf[u] = *reinterpret_cast<const bf16x8_t*>(value_at(buffer, u));
+    if (pos + kStage > w.diag) {
+      w.mask(sc[0], pos);
+      w.mask(sc[1], pos + kStep);
+    }
+    w.refer(sc);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      bf16x8_t pf[S::kRT];
+      w.weigh(sc[n], pf);
+#pragma unroll
+      for (int u = 0; u < W::kDTiles; ++u) {
+        const int f = n * W::kDTiles + u;
+#pragma unroll
+        for (int rt = 0; rt < S::kRT; ++rt)
+          w.o[rt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[f % kAhead], pf[rt], w.o[rt][u], 0, 0, 0);
+        if (f + kAhead < 2 * W::kDTiles) vf[f % kAhead] = *reinterpret_cast<const bf16x8_t*>(value_at(buffer, f + kAhead));
+      }
+    }
+  };
+  if (first_stage < n_stages) {
+    look_up(first_stage / 16 * 16);
+    load_share(first_stage);
+    widen_share(first_stage);
+    if ((first_stage + 1) % 16 == 0) look_up(first_stage + 1);
+    load_share(first_stage + 1);  // past the last stage: the last record again
+  }
+#pragma unroll 1
+  for (int stage = first_stage; stage < n_stages; ++stage) {
+    ring_barrier();  // this stage's fragments stand, the stage before is done with
+    if (stage + 1 < n_stages) widen_share(stage + 1);
+    if ((stage + 2) % 16 == 0) look_up(stage + 2);
+    load_share(stage + 2);
+    compute(stage * kStage, stage & 1);
+    if ((stage + 1) * kStage > all_see) {
+      uint32_t met = 0;
+#pragma unroll
+      for (int i = 0; i < S::kWaves; ++i) met |= (stage * kStage + i / 2 * kTile + kTile > all_see) ? odd[stage & 1][i] : 0u;
+      if (met != 0) w.mark_nan(max(stage * kStage, all_see / kTile * kTile), min((stage + 1) * kStage, end));
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < S::kRT; ++rt) {
+    w.l[rt] = quarters_sum(w.l[rt]);
+    const int row = r0 + rt * 16 + w.l16;
+    if (row >= rows) continue;
+    if (splits == 1) {
+      w.write(r, hkv, row, rt);
+      continue;
+    }
+    const int64_t slot = tile_slot(a, b, hkv, row_tile) + split;
+    const int at = wave * S::kRT + rt;
+#pragma unroll
+    for (int u = 0; u < W::kDTiles; ++u)
+      reinterpret_cast<f32x4_t*>(a.o_part)[((slot * (S::kRows / 16) + at) * W::kDTiles + u) * kWave + w.lane] = w.o[rt][u];
+    if (w.qg == 0) a.ml_part[slot * S::kRows + at * 16 + w.l16] = make_float2(w.m[rt], w.l[rt]);
+  }
+}
+
 // A workgroup a pair of tiles (values n and n + 1 of each lane's run): 4 wavefronts a tile share the splits, up to 16 of which each
 // requests at once (they come from other XCDs' writes, a microsecond away); then the wavefronts through LDS.
 constexpr int kCombineWaves = 8;
-template <int D>
+// TILED: of the tile kernel's splits, else of the split kernel's.
+template <int D, bool TILED>
 __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(AttnArgs a) {
   using W = Walk<D, 1>;
+  constexpr int kPairs = TileShape<D>::kRows / 16 * W::kDTiles / 2;  // of a row tile (TILED)
   constexpr int kGroups = kCombineWaves / 2;
   __shared__ float sm_m[kGroups][kWave], sm_l[kGroups][kWave];
   __shared__ __align__(16) f32x4_t sm_o[kCombineWaves][kWave];
-  const int pair = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z;
+  const int hkv = blockIdx.y, b = blockIdx.z;
+  const int pair = TILED ? blockIdx.x % kPairs : blockIdx.x, row_tile = TILED ? blockIdx.x / kPairs : 0;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tile = 2 * pair + wave % 2, g = wave / 2;
-  const int l16 = lane % 16, qg = lane / 16, row = tile / W::kDTiles * 16 + l16;
+  const int l16 = lane % 16, qg = lane / 16, part_row = tile / W::kDTiles * 16 + l16;
+  const int row = row_tile * TileShape<D>::kRows + part_row;
   const Request r = request(a, b);
-  const int2 place = a.plan[b];
   const int rows = r.n * a.G;
-  if (place.y < 2 || tile / W::kDTiles * 16 >= rows) return;
-  const int kTiles = gridDim.x * 2;
-  const int64_t slot = (int64_t)hkv * a.slots + place.x;
+  if (row - l16 >= rows) return;
+  int splits, kTiles, slot_rows;
+  int64_t slot;
+  if constexpr (TILED) {
+    if (rows <= a.few) return;
+    int per;
+    const int last_row = min((row_tile + 1) * TileShape<D>::kRows, rows) - 1;
+    stage_splits(a, max(r.seq - r.n + divide(last_row, a.by_g) + 1, 0), splits, per);
+    slot = tile_slot(a, b, hkv, row_tile);
+    kTiles = 2 * kPairs;
+    slot_rows = TileShape<D>::kRows;
+  } else {
+    const int2 place = a.plan[b];
+    splits = place.y;
+    slot = (int64_t)hkv * a.slots + place.x;
+    kTiles = gridDim.x * 2;
+    slot_rows = a.rows;
+  }
+  if (splits < 2) return;
   float m = -__builtin_inff(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   if (row < rows) {
@@ -725,13 +961,13 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(Att
       f32x4_t v[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int at = min(s + i * kGroups, place.y - 1);
-        ml[i] = a.ml_part[(slot + at) * a.rows + row];
+        const int at = min(s + i * kGroups, splits - 1);
+        ml[i] = a.ml_part[(slot + at) * slot_rows + part_row];
         v[i] = from[(slot + at) * kTiles * kWave];
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (s + i * kGroups >= place.y) break;
+        if (s + i * kGroups >= splits) break;
         const float top = fmaxf(m, ml[i].x);
         const float ref = top == -__builtin_inff() ? 0.f : top;
         const float keep = fast_exp2(m - ref), weight = fast_exp2(ml[i].x - ref);
@@ -741,8 +977,8 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(Att
       }
     };
     int s = g;
-    for (; s + 4 * kGroups < place.y; s += 16 * kGroups) add(s, std::integral_constant<int, 16>{});
-    if (s < place.y) add(s, std::integral_constant<int, 4>{});
+    for (; s + 4 * kGroups < splits; s += 16 * kGroups) add(s, std::integral_constant<int, 16>{});
+    if (s < splits) add(s, std::integral_constant<int, 4>{});
   }
   if (wave % 2 == 0) {
     sm_m[g][lane] = m;
@@ -772,170 +1008,6 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(Att
                  16 * Rec::kWidth * h + Rec::kWidth * 4 * qg + n;
 #pragma unroll
   for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(to + Rec::kWidth * i) = pack_bf16(even[i] * inv, odd[i] * inv);
-}
-
-// Many rows: 8 wavefronts with 16 kRT rows each walk over the same positions, 64 a stage.  Each wavefront reads the keys' codes
-// itself (the other seven find them in the cache next to the CU) and widens them; the values are widened once for all of them,
-// an eighth a wavefront, into LDS, in the order of the operand: two buffers, one barrier a stage.
-template <int D>
-struct TileShape {
-  static constexpr int kRT = D == 256 ? 1 : 2;
-  static constexpr int kWaves = 8;
-  static constexpr int kRows = 16 * kRT * kWaves;
-};
-constexpr int kStage = 64;
-
-template <int D>
-__global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel(AttnArgs a) {
-  using S = TileShape<D>;
-  using W = Walk<D, S::kRT>;
-  using R = Record<D>;
-  __shared__ __align__(16) u32x2_t frags[2][2][W::kDTiles][kWave][2];  // [buffer][step][value tile][lane][record]
-  __shared__ uint32_t odd[2][S::kWaves];                              // a wavefront met a block of NaN that not all rows see
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int hkv = blockIdx.y, b = blockIdx.z;
-  const Request r = request(a, b);
-  const int rows = r.n * a.G;
-  const int row0 = (gridDim.x - 1 - blockIdx.x) * S::kRows;  // the rows that see most come first
-  if (row0 >= rows || rows <= a.few) return;
-  const int r0 = row0 + wave * 16 * S::kRT;
-  W w(a);
-  w.start(r, b, hkv, r0);
-  auto seen = [&](int row) { return max(r.seq - r.n + divide(min(row, rows - 1), a.by_g) + 1, 0); };
-  const int end = seen(row0 + S::kRows - 1), all_see = seen(row0);
-  const int n_stages = (end + kStage - 1) / kStage;
-  const int last_tile = (end - 1) / kTile * kTile;
-
-  // The records of 16 stages are looked up at once, a record a lane.
-  uint32_t rec_lo = 0, rec_hi = 0;
-  auto look_up = [&](int stage) {
-    const int64_t at = w.record(min(stage * kStage + w.lane * kTile, last_tile));
-    rec_lo = (uint32_t)at;
-    rec_hi = (uint32_t)(at >> 32);
-  };
-  auto where = [&](int l) {
-    const uint32_t lo = __builtin_amdgcn_readlane(rec_lo, l), hi = __builtin_amdgcn_readlane(rec_hi, l);
-    return w.base + (int64_t)(((uint64_t)hi << 32) | lo);
-  };
-
-  // This wavefront's share of a stage's values: of record `mine` its half (D = 256) or half of its bytes.
-  constexpr int kBytes = D == 256 ? 4 : D / 64;  // of each lane's run: 2 kBytes tiles
-  const int mine = wave / 2, half = D == 256 ? wave % 2 : 0, byte0 = D == 256 ? 0 : wave % 2 * kBytes;
-  typename W::Data::Run v;
-  uint32_t vs;
-  auto load_values = [&](int stage) {
-    const uint8_t* rec = where(stage % 16 * 4 + mine);
-    v = *reinterpret_cast<const typename W::Data::Run*>(rec + R::kValues + half * 1024 + w.lane * 4 * W::kDwords);
-    vs = *reinterpret_cast<const uint32_t*>(rec + R::kValueScales + (W::kDwords == 4 ? 4 * half + w.l16 / 4 : w.l16 / 8) * kTile + 4 * w.qg);
-  };
-  auto widen_values = [&](int stage) {
-    const int pos = stage * kStage + mine * kTile;
-    if (pos + kTile > all_see) {  // behind the end anything may stand; a block of NaN would reach rows that do not see it
-      bool any = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool gone = pos + 4 * w.qg + i >= end, nan = (vs >> (8 * i) & 255u) == 255u;
-        any |= nan && !gone;
-        if (gone || nan) {
-          vs = (vs & ~(255u << (8 * i))) | 127u << (8 * i);
-          if constexpr (W::kDwords == 4) {
-            v[i] = 0;
-          } else {
-            v[i / 2] &= i % 2 ? 0xffffu : 0xffff0000u;
-          }
-        }
-      }
-      const bool met = __any(any);
-      if (w.lane == 0) odd[stage & 1][wave] = met;
-    }
-    const uint32_t bytes = here(vs);
-    const float s[4] = {scale_of<0>(bytes), scale_of<1>(bytes), scale_of<2>(bytes), scale_of<3>(bytes)};
-    auto pair = [&](auto byte) {
-      constexpr int kB = decltype(byte)::value;
-      uint32_t x[4];
-      if constexpr (D == 256) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = widen2<kB>(v[i], s[i]);
-      } else if constexpr (D == 128) {  // bytes byte0 + kB, moved down
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = widen2<kB>(v[i] >> (8 * byte0), s[i]);
-      } else {
-        const uint32_t lo = v[0] >> (8 * byte0), hi = v[1] >> (8 * byte0);
-        x[0] = widen2<0>(lo, s[0]);
-        x[1] = widen2<2>(lo, s[1]);
-        x[2] = widen2<0>(hi, s[2]);
-        x[3] = widen2<2>(hi, s[3]);
-      }
-      const int u = half * W::kPerHalf + 2 * (byte0 + kB);
-      frags[stage & 1][mine / 2][u][w.lane][mine % 2] =
-          u32x2_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100), __builtin_amdgcn_perm(x[3], x[2], 0x05040100)};
-      frags[stage & 1][mine / 2][u + 1][w.lane][mine % 2] =
-          u32x2_t{__builtin_amdgcn_perm(x[1], x[0], 0x07060302), __builtin_amdgcn_perm(x[3], x[2], 0x07060302)};
-    };
-    pair(std::integral_constant<int, 0>{});
-    if constexpr (kBytes > 1) pair(std::integral_constant<int, 1>{});
-    if constexpr (kBytes > 2) {
-      pair(std::integral_constant<int, 2>{});
-      pair(std::integral_constant<int, 3>{});
-    }
-  };
-
-  // The scores of step i + 1 are computed beside the weights of step i, so that the matrix cores have work while the exponentials
-  // are computed.
-  const bool live = r0 < rows;
-  typename W::Data keys[2];
-  typename W::Scores sc[2];
-  auto key_records = [&](int i, auto&& take) { take(where(i % 32 * 2), where(i % 32 * 2 + 1)); };  // of step i, of those looked up
-  auto step = [&](int i, int buffer, auto parity) {
-    constexpr int kP = decltype(parity)::value;
-    key_records(i + 2, [&](auto* x, auto* y) { w.load_keys(keys[kP], x, y); });  // the keys of step i are used up
-    if (!live) return;
-    constexpr int kAhead = W::kDTiles < 8 ? W::kDTiles : 8;  // operands read before the scores; the others where registers are free
-    bf16x8_t vf[W::kDTiles];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) vf[u] = *reinterpret_cast<const bf16x8_t*>(&frags[buffer][kP][u][w.lane][0]);
-    if ((i + 1) * kStep > w.diag) w.mask(sc[kP], i * kStep);
-    w.refer(sc[kP]);
-    w.scores(keys[1 - kP], sc[1 - kP]);
-    bf16x8_t pf[S::kRT];
-    w.weigh(sc[kP], pf);
-    if constexpr (kAhead < W::kDTiles) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int u = kAhead; u < W::kDTiles; ++u) vf[u] = *reinterpret_cast<const bf16x8_t*>(&frags[buffer][kP][u][w.lane][0]);
-#pragma unroll
-    for (int u = 0; u < W::kDTiles; ++u)
-#pragma unroll
-      for (int rt = 0; rt < S::kRT; ++rt) w.o[rt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[u], pf[rt], w.o[rt][u], 0, 0, 0);
-  };
-  if (n_stages > 0) {
-    look_up(0);
-    load_values(0);
-    key_records(0, [&](auto* x, auto* y) { w.load_keys(keys[0], x, y); });
-    key_records(1, [&](auto* x, auto* y) { w.load_keys(keys[1], x, y); });
-    widen_values(0);
-    w.scores(keys[0], sc[0]);
-  }
-#pragma unroll 1
-  for (int stage = 0; stage < n_stages; ++stage) {
-    ring_barrier();  // this stage's values stand, the stage before is done with
-    if ((stage + 1) % 16 == 0) look_up(stage + 1);  // past the last stage: its last record again
-    load_values(stage + 1);
-    step(2 * stage, stage & 1, std::integral_constant<int, 0>{});
-    step(2 * stage + 1, stage & 1, std::integral_constant<int, 1>{});
-    if ((stage + 1) * kStage > all_see) {
-      uint32_t met = 0;
-#pragma unroll
-      for (int i = 0; i < S::kWaves; ++i) met |= (stage * kStage + i / 2 * kTile + kTile > all_see) ? odd[stage & 1][i] : 0u;
-      if (met != 0) w.mark_nan(max(stage * kStage, all_see / kTile * kTile), min((stage + 1) * kStage, end));
-    }
-    if (stage + 1 < n_stages) widen_values(stage + 1);
-  }
-#pragma unroll
-  for (int rt = 0; rt < S::kRT; ++rt) {
-    w.l[rt] = quarters_sum(w.l[rt]);
-    const int row = r0 + rt * 16 + w.l16;
-    if (row < rows) w.write(r, hkv, row, rt);
-  }
 }
 
 typedef void (*AttnFn)(AttnArgs);
@@ -971,10 +1043,14 @@ int compute_units() {
 // How a call runs: its launches and the parts of its workspace.
 struct Plan {
   bool tiles, split;  // the tile kernel; the split kernel with the combination
-  int workers, slots, rows;
-  size_t o, ml, plan, bytes;  // offsets and size of the workspace
+  int workers, slots, rows;         // split kernel
+  int row_tiles, tile_splits;       // tile kernel
+  size_t o, ml, plan, tile_o, tile_ml, bytes;  // offsets and size of the workspace
 };
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+constexpr size_t kTilePartials = (size_t)128 << 20;  // most bytes of the tile kernel's partial results
+int tile_rows(int D) { return D == 256 ? TileShape<256>::kRows : D == 128 ? TileShape<128>::kRows : TileShape<64>::kRows; }
 
 // Requests of up to QF_KV4_MAX_ROWS packed rows are split over positions, larger ones tiled over rows; a batch with lengths of its
 // own may hold both kinds (a chunk of 700 tokens beside single ones of 4000 positions).
@@ -983,14 +1059,37 @@ Plan plan_of(const qf_kv4_attention_args& u) {
   const int64_t rows = (int64_t)u.q_len * (u.num_heads / u.num_kv_heads);
   p.tiles = rows > QF_KV4_MAX_ROWS;
   p.split = !p.tiles || u.cu_q != nullptr;
-  if (!p.split) return p;
+  size_t n = 0;
+  if (p.tiles) {
+    const int per = tile_rows(u.head_size);
+    p.row_tiles = (int)((rows + per - 1) / per);
+    // Positions are split where the row tiles leave compute units idle (100 tokens behind 4000 positions, 64 heads over 8: 115 -> 34
+    // us; twice as many splits 47).
+    const int64_t all = (int64_t)p.row_tiles * u.num_reqs, by_tokens = ((int64_t)u.num_tokens * (u.num_heads / u.num_kv_heads) + per - 1) / per + u.num_reqs;
+    const int64_t groups = (all < by_tokens ? all : by_tokens) * u.num_kv_heads;
+    int64_t splits = compute_units() / groups;
+    splits = splits < 1 ? 1 : splits > 16 ? 16 : splits;
+    const size_t slot = (size_t)per * u.head_size * sizeof(float);
+    while (splits > 1 && (size_t)all * u.num_kv_heads * splits * slot > kTilePartials) --splits;
+    p.tile_splits = (int)splits;
+    if (splits > 1) {
+      const size_t slots = (size_t)all * u.num_kv_heads * splits;
+      p.tile_o = n;
+      n += slots * slot;
+      p.tile_ml = n;
+      n += round256(slots * per * sizeof(float2));
+    }
+  }
+  if (!p.split) {
+    p.bytes = n;
+    return p;
+  }
   p.rows = rows < QF_KV4_MAX_ROWS ? (int)rows : QF_KV4_MAX_ROWS;
   // A workgroup a CU; two where the requests by themselves fill the machine, so that the longest of them is cut finer (48 requests
   // of up to 9000 positions over 8 kv heads: 28.2 -> 25.0 us; 16 requests of up to 3000, which do not: 18.8 -> 22.7).
   const int cus = compute_units() * ((int64_t)u.num_reqs * u.num_kv_heads >= compute_units() ? 2 : 1);
   p.workers = (cus + u.num_kv_heads - 1) / u.num_kv_heads;
   p.slots = p.workers + u.num_reqs;
-  size_t n = 0;
   const size_t parts = (size_t)u.num_kv_heads * p.slots;
   p.o = n;
   n += parts * split_of(u.head_size, p.rows).row_tiles * 16 * u.head_size * sizeof(float);
@@ -1072,19 +1171,28 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   a.by_workers = divisor(p.split ? p.workers : 1);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int D = u.head_size, di = D == 64 ? 0 : D == 128 ? 1 : 2;
+  a.row_tiles = p.row_tiles;
+  a.tile_splits = p.tile_splits;
   if (p.tiles) {
-    const int64_t rows = (int64_t)u.q_len * a.G;
-    const int per = D == 256 ? TileShape<256>::kRows : TileShape<128>::kRows;
-    static_assert(TileShape<64>::kRows == TileShape<128>::kRows && TileShape<256>::kWaves == TileShape<128>::kWaves, "one shape");
+    a.o_part = reinterpret_cast<float*>(ws + p.tile_o);
+    a.ml_part = reinterpret_cast<float2*>(ws + p.tile_ml);
+    static_assert(TileShape<64>::kWaves == TileShape<128>::kWaves && TileShape<256>::kWaves == TileShape<128>::kWaves, "one shape");
     const AttnFn fn = D == 64 ? &attn_tile_kernel<64> : D == 128 ? &attn_tile_kernel<128> : &attn_tile_kernel<256>;
-    const int st = launch(fn, dim3((unsigned)((rows + per - 1) / per), a.HKV, a.B), TileShape<128>::kWaves * kWave, 0, g_raised[di][0], s, a);
-    if (st != QF_OK || !p.split) return st;
+    const int lds = D == 64 ? TileShape<64>::kLds : D == 128 ? TileShape<128>::kLds : TileShape<256>::kLds;
+    int st = launch(fn, dim3((unsigned)(p.row_tiles * p.tile_splits), a.HKV, a.B), TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
+    if (st != QF_OK) return st;
+    if (p.tile_splits > 1) {
+      const AttnFn comb = D == 64 ? &attn_combine_kernel<64, true> : D == 128 ? &attn_combine_kernel<128, true> : &attn_combine_kernel<256, true>;
+      st = launch(comb, dim3((unsigned)(p.row_tiles * (tile_rows(D) / 16 * (D / 32))), a.HKV, a.B), kCombineWaves * kWave, 0, g_raised[di][0], s, a);
+      if (st != QF_OK) return st;
+    }
+    if (!p.split) return QF_OK;
   }
   a.o_part = reinterpret_cast<float*>(ws + p.o);
   a.ml_part = reinterpret_cast<float2*>(ws + p.ml);
   a.plan = reinterpret_cast<int2*>(ws + p.plan);
   const Split k = split_of(D, p.rows);
-  const AttnFn comb = D == 64 ? &attn_combine_kernel<64> : D == 128 ? &attn_combine_kernel<128> : &attn_combine_kernel<256>;
+  const AttnFn comb = D == 64 ? &attn_combine_kernel<64, false> : D == 128 ? &attn_combine_kernel<128, false> : &attn_combine_kernel<256, false>;
   const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, k.lds, g_raised[di][k.row_tiles], s, a);
   if (st != QF_OK) return st;
   return launch(comb, dim3(k.row_tiles * D / 32, a.HKV, a.B), kCombineWaves * kWave, 0, g_raised[di][0], s, a);
