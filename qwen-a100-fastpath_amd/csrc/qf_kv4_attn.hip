@@ -1028,18 +1028,6 @@ Split split_of(int D, int rows) {
   return D == 64 ? split_kernel<64>(rt) : D == 128 ? split_kernel<128>(rt) : split_kernel<256>(rt);
 }
 
-int compute_units() {
-  static std::atomic<int> cus[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  int n = cus[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
-    cus[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 // How a call runs: its launches and the parts of its workspace.
 struct Plan {
   bool tiles, split;  // the tile kernel; the split kernel with the combination

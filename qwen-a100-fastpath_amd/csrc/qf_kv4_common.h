@@ -5,6 +5,9 @@
 #include "qf_block_common.h"
 #include "qf_kv4.h"
 
+#include <algorithm>
+#include <atomic>
+
 namespace qfk {
 
 using namespace qfb;
@@ -24,6 +27,18 @@ inline Divisor divisor(int d) {
   return Divisor{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), l};
 }
 __device__ __forceinline__ int divide(int n, Divisor d) { return (int)(((uint64_t)(uint32_t)n * d.m) >> (31 + d.shift)); }
+
+inline int compute_units() {  // of the current device
+  static std::atomic<int> cus[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = cus[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+    cus[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 // Offsets in a record of 16 positions of a head of D values.
 template <int D>

@@ -1,9 +1,14 @@
 // qf_kv4_rope.hip — norms of query and key heads with the position rotation and the write into the cache (gfx950).
 //
-// A row is a head of a token: D / 8 lanes of 16 bytes each, 64 / (D / 8) rows a wavefront side by side; the rows of a token
-// are its query heads, its key heads and its value heads in this order.  Per row: the mean of squares over its lanes (DPP
-// adds), the norm's factor, the rotation (the other value of a pair stands in the same lane, or rot / 16 lanes away and comes
-// by a lane permutation), one rounding to bf16, and for keys and values their page, or blocks of 32 values (4 lanes) to 4 bits.
+// A row is a head of a token: D / 8 lanes of 16 bytes each, 64 / (D / 8) rows of one kind (query, key, value) a chunk, side by side
+// in a wavefront.  Per row: the mean of squares over its lanes (DPP adds), the norm's factor, the rotation (the other value of a
+// pair stands in the same lane, or rot / 16 lanes away and comes by a lane permutation), one rounding to bf16, and for keys and
+// values their page, or blocks of 32 values (4 lanes) to 4 bits.
+//
+// A wavefront takes several chunks of one kind, the next one's rows requested before the last one's work, and the angles and
+// weights, which a lane needs for one token only, once for all of them.  Queries: the chunks are heads of one token.  Keys and values: a chunk is one head
+// of 64 / L neighbouring tokens, whose bytes of a 4-bit record stand together, and the 4 wavefronts of a workgroup take further
+// neighbours.
 #include "qf_kv4_common.h"
 
 namespace qfk {
@@ -11,11 +16,19 @@ namespace qfk {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeWaves = kRopeThreads / kWave;
 
+// Chunks of a wavefront: one until each compute unit has 8 wavefronts, then up to 4.  Measured with 1, 2, 4 and 8 chunks: 5 tokens of
+// 64 + 8 heads of 128 (112 chunks) 5.7, 6.3, 7.8, 10.7 us; 333 of 24 + 4 of 256 (5300) 8.8, 8.4, 9.7, 11.8; 2048 of 64 + 8 of 128
+// (41 000) 30.9, 27.3, 25.0, 24.8; 8191 of 16 + 2 of 128 (41 000, into pages) 27.7, 22.4, 22.1, 26.5.
+constexpr int kWavesBeforeMore = 8;
+constexpr int kMostChunks = 4;
+
 struct RopeArgs {
   qf_qk_norm_rope_args u;
-  Divisor by_page, by_parts;
-  int rows;   // of a token
-  int parts;  // wavefronts of a token
+  Divisor by_page, by_q, by_kv;
+  int chunks;            // of a wavefront
+  int kv_waves;          // wavefronts of keys and values, whole workgroups; those of queries follow
+  int q_items;           // wavefronts of a token's queries
+  int k_items, v_items;  // workgroups of 4 * 64 / L tokens' keys and values
 };
 
 template <typename T>
@@ -50,61 +63,106 @@ __device__ __forceinline__ void load4<uint16_t>(float (&f)[4], const uint16_t* p
   f[3] = bf16_hi(v.y);
 }
 
-// The angles of a lane's 8 values: of each value (halves: value i and i + rot / 2 turn by one angle), or of its 4 pairs.
-struct Angles {
-  float c[8], s[8];
+// What a row's 8 values of a lane become is n_i = factor (x_i a_i + o_i b_i): o the values that pair with x, a and b the norm's
+// weights times the angle's cosine and (with its sign) sine.
+struct Turn {
+  u32x4_t w, wo;     // the weights of x and of o, bf16
+  float c[8], s[8];  // -s where a value is the first of its pair; c = 1 and s = -0 outside the rotation
+  double offset, eps;
+  bool norm;
 };
 
-// The lane's 8 values of a row turned and normalised, in R (fp32 or fp64).  `other`: the bf16 values that pair with these.
-// sign: -1 where these are the first of their pairs, 1 where they are the second, 0 outside the rotation.
-template <int L, bool INTERLEAVED, typename R>
-__device__ __forceinline__ u32x4_t turned(u32x4_t mine, u32x4_t other, bool norm, const float (&w)[8], const float (&wo)[8],
-                                          const Angles& at, int sign, R offset, R eps) {
-  float x[8], o[8], y[8];
-  unpack8(mine, x);
-  unpack8(other, o);
-  R factor = 1;
-  if (norm) {
-    R sum = 0;
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int L>
+__device__ __forceinline__ double group_sum(double v) {  // as the sum of floats
+  v += dpp_f64<0xB1>(v);
+  v += dpp_f64<0x4E>(v);
+  v += dpp_f64<0x141>(v);
+  if constexpr (L >= 16) v += dpp_f64<0x140>(v);
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  return v;
+}
+
+template <int L, bool INTERLEAVED>
+__device__ __forceinline__ void paired(u32x4_t x, int other, bool turn, float (&o)[8]) {
+  if constexpr (INTERLEAVED) {
+    unpack8(x, o);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += (R)x[i] * (R)x[i];
-    if constexpr (sizeof(R) == 8) {
+    for (int i = 0; i < 8; i += 2) {
+      const float first = o[i];
+      o[i] = turn ? o[i + 1] : 0.0f;
+      o[i + 1] = turn ? first : 0.0f;
+    }
+  } else {
+    u32x4_t y;
 #pragma unroll
-      for (int m = 1; m < L; m *= 2) sum += __shfl_xor(sum, m);
-    } else {
-      sum = group_sum<L>(sum);
-      // squares outside fp32's range (their sum is not a number that holds them): this row in fp64
-      if (!(sum >= 0x1p-90f && sum <= 0x1p+126f))
-        return turned<L, INTERLEAVED, double>(mine, other, norm, w, wo, at, sign, (double)offset, (double)eps);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t from = (uint32_t)__shfl((int)x[i], other);
+      y[i] = turn ? from : 0;  // (an infinity times no sine is not a number)
     }
-    const R mean = sum * (R)(1.0 / (8 * L)) + eps;
-    if constexpr (sizeof(R) == 8) {
-      factor = 1.0 / sqrt(mean);
-    } else {
-      factor = 1.0f / sqrtf(mean);
-    }
+    unpack8(y, o);
   }
-  R n[8];
+}
+
+// In fp32, a and b as computed once for all rows of a wavefront.
+template <int L>
+__device__ __forceinline__ u32x4_t turned(u32x4_t mine, float (&o)[8], const Turn& at, const float (&a)[8], const float (&b)[8]) {
+  float x[8];
+  unpack8(mine, x);
+  float factor = 1.0f;
+  if (at.norm) {
+    float sum = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = norm ? (R)x[i] * factor * (offset + (R)w[i]) : (R)x[i];
-  if (sign != 0) {
-    if constexpr (INTERLEAVED) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const R a = n[2 * i], b = n[2 * i + 1], c = at.c[i], s = at.s[i];
-        n[2 * i] = a * c - b * s;
-        n[2 * i + 1] = b * c + a * s;
-      }
-    } else {
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    sum = group_sum<L>(sum);
+    float eps = (float)at.eps;
+    // Squares outside fp32's range (their sum does not hold them, nor is it nothing beside eps): the row times a power of two.
+    if (!(sum <= 0x1p+126f && (sum >= 0x1p-90f || at.eps >= 0x1p-110))) {
+      const float up = sum < 1.0f ? 0x1p+100f : 0x1p-80f;
+      sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const R m = norm ? (R)o[i] * factor * (offset + (R)wo[i]) : (R)o[i];
-        n[i] = n[i] * (R)at.c[i] + (sign < 0 ? -m : m) * (R)at.s[i];
+        x[i] *= up;
+        o[i] *= up;
+        sum = fmaf(x[i], x[i], sum);
       }
+      sum = group_sum<L>(sum);
+      eps = (float)(at.eps * ((double)up * up));
     }
+    factor = 1.0f / sqrtf(fmaf(sum, 1.0f / (8 * L), eps));
+  }
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = fmaf(o[i] * factor, b[i], x[i] * factor * a[i]);
+  return pack8(y);
+}
+
+// In fp64: the result, rounded to bf16, does not depend on the order of the sums.
+template <int L>
+__device__ __forceinline__ u32x4_t turned(u32x4_t mine, const float (&o)[8], const Turn& at) {
+  float x[8], w[8], wo[8], y[8];
+  unpack8(mine, x);
+  unpack8(at.w, w);
+  unpack8(at.wo, wo);
+  double factor = 1;
+  if (at.norm) {
+    double sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fma((double)x[i], (double)x[i], sum);
+    factor = 1.0 / sqrt(fma(group_sum<L>(sum), 1.0 / (8 * L), at.eps));
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = (float)n[i];
+  for (int i = 0; i < 8; ++i) {
+    const double n = (double)x[i] * factor * (at.offset + (double)w[i]), m = (double)o[i] * factor * (at.offset + (double)wo[i]);
+    y[i] = (float)fma(m, (double)at.s[i], n * (double)at.c[i]);
+    if (i % 2) __builtin_amdgcn_sched_barrier(0);  // (8 values in work at once take 60 registers more)
+  }
   return pack8(y);
 }
 
@@ -131,104 +189,159 @@ __device__ __forceinline__ uint32_t four_bits(u32x4_t v, uint32_t* byte) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, v3), scale, 3);
 }
 
-template <int D, bool INTERLEAVED, typename TABLE>
-__global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs args) {
+enum { kQuery, kKey, kKey4, kValue };  // kKey4: a key for the 4-bit cache
+
+// Chunks of a token's heads from `head` on, `step` heads apart.
+template <int D, bool INTERLEAVED, typename TABLE, int KIND>
+__device__ __forceinline__ void run_chunks(const RopeArgs& args, int t, int head, int step) {
   const qf_qk_norm_rope_args& a = args.u;
-  constexpr int L = D / 8;          // lanes of a row
-  constexpr int kRows = kWave / L;  // rows of a wavefront
-  const int lane = threadIdx.x % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kRopeWaves + threadIdx.x / kWave);
-  const int t = divide(wave, args.by_parts);
-  if (t >= a.num_tokens) return;
-  const int part = wave - t * args.parts;
-  const int j = lane % L;  // this lane's place in its row: values 8 j .. 8 j + 7
-  const int row = part * kRows + lane / L;
-  const bool live = row < args.rows;
-  const int H = a.query.data != nullptr ? a.num_heads : 0;
-  const int HK = a.num_kv_heads;
-  const bool is_q = row < H, is_k = !is_q && row < H + HK;
-  const int head = is_q ? row : is_k ? row - H : row - H - HK;
-  const qf_heads& from = is_q ? a.query : is_k ? a.key : a.value;
+  constexpr int L = D / 8;  // lanes of a row
+  const qf_heads& from = KIND == kQuery ? a.query : KIND == kValue ? a.value : a.key;
+  const qf_heads& to = KIND == kQuery ? a.query_out : a.key_out;
+  const int heads = t < a.num_tokens ? (KIND == kQuery ? a.num_heads : a.num_kv_heads) : 0;
+  const int lane = threadIdx.x % kWave, j = lane % L;  // this lane's place in its row: values 8 j .. 8 j + 7
+  const bool turn = KIND != kValue && 8 * j < a.rot && heads > 0;
+  int64_t pos = 0, slot = -1;
+  if (turn) pos = a.positions[t];
+  if (KIND != kQuery && a.cache_kind != QF_CACHE_NONE && heads > 0) slot = a.slots[t];
+  const uint16_t* p = from.data + t * from.stride_tok + head * from.stride_head + 8 * j;
+  u32x4_t next = {0, 0, 0, 0};
+  if (head < heads) next = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
 
-  u32x4_t x = {0, 0, 0, 0};
-  if (live) x = *reinterpret_cast<const u32x4_t*>(from.data + t * from.stride_tok + head * from.stride_head + 8 * j);
-
-  float w[8], wo[8];
-  Angles at;
-  const uint16_t* weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
-  const bool norm = live && weight != nullptr;
   const int half = a.rot / 16;  // lanes from a pair's first value to its second
-  const int other = INTERLEAVED || 8 * j >= a.rot ? j : j < half ? j + half : j - half;
-  if (norm) {
-    load8(w, weight + 8 * j);
-    load8(wo, weight + 8 * other);
-  }
-  int sign = 0;
-  if (8 * j < a.rot && (is_q || is_k)) {
-    int64_t pos = a.positions[t];
-    pos = pos < 0 ? 0 : pos >= a.num_positions ? a.num_positions - 1 : pos;
-    const TABLE* cs = static_cast<const TABLE*>(a.cos_sin) + pos * a.rot;
-    if constexpr (INTERLEAVED) {
-      sign = 1;
-      float c[4], s[4];
-      load4(c, cs + 4 * j);
-      load4(s, cs + a.rot / 2 + 4 * j);
+  const int other = INTERLEAVED || !turn ? j : j < half ? j + half : j - half;
+  const int partner = lane - j + other;
+  Turn at;
+  float fa[8], fb[8];
+  if constexpr (KIND != kValue) {
+    const uint16_t* weight = KIND == kQuery ? a.q_weight : a.k_weight;
+    at.norm = weight != nullptr;
+    at.offset = at.norm ? a.weight_offset : 1.0;
+    at.eps = a.eps;
+    at.w = at.wo = u32x4_t{0, 0, 0, 0};
+    if (at.norm) {
+      at.w = *reinterpret_cast<const u32x4_t*>(weight + 8 * j);
+      at.wo = *reinterpret_cast<const u32x4_t*>(weight + 8 * other);
+      if constexpr (INTERLEAVED) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        at.c[i] = c[i];
-        at.s[i] = s[i];
+        for (int i = 0; i < 4; ++i) at.wo[i] = __builtin_amdgcn_alignbit(at.w[i], at.w[i], 16);
       }
-    } else {
-      sign = j < half ? -1 : 1;
-      const int first = 8 * (j < half ? j : other);
-      load8(at.c, cs + first);
-      load8(at.s, cs + a.rot / 2 + first);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      at.c[i] = 1.0f;
+      at.s[i] = -0.0f;
+    }
+    if (turn) {
+      pos = pos < 0 ? 0 : pos >= a.num_positions ? a.num_positions - 1 : pos;
+      const TABLE* cs = static_cast<const TABLE*>(a.cos_sin) + pos * a.rot;
+      if constexpr (INTERLEAVED) {
+        float c[4], s[4];
+        load4(c, cs + 4 * j);
+        load4(s, cs + a.rot / 2 + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          at.c[2 * i] = at.c[2 * i + 1] = c[i];
+          at.s[2 * i] = -s[i];
+          at.s[2 * i + 1] = s[i];
+        }
+      } else {
+        const int first = 8 * (j < half ? j : other);
+        load8(at.c, cs + first);
+        load8(at.s, cs + a.rot / 2 + first);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) at.s[i] = j < half ? -at.s[i] : at.s[i];
+      }
+    }
+    if constexpr (KIND != kKey4) {
+      unpack8(at.w, fa);
+      unpack8(at.wo, fb);
+      const float offset = (float)at.offset;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        fa[i] = (offset + fa[i]) * at.c[i];
+        fb[i] = (offset + fb[i]) * at.s[i];
+      }
     }
   }
-  u32x4_t xo = x;
-  if constexpr (!INTERLEAVED) {
+  const bool kept = KIND != kQuery && slot >= 0 && slot < a.num_blocks * a.page_size;
+  int64_t block = 0;
+  if (kept) block = slot <= 0x7fffffff ? divide((int)slot, args.by_page) : slot / a.page_size;
+  const int place = kept ? (int)(slot - block * a.page_size) : 0;
+  uint16_t* out = KIND == kValue || to.data == nullptr ? nullptr : to.data + t * to.stride_tok + head * to.stride_head + 8 * j;
+#pragma unroll 1
+  for (int c = 0; c < args.chunks; ++c) {
+    u32x4_t x = next;
+    const bool in = head < heads;
+    head += step;
+    p += step * from.stride_head;
+    if (c + 1 < args.chunks && head < heads) next = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    if constexpr (KIND != kValue) {
+      float o[8];
+      if constexpr (KIND == kKey4) {
+        // Widened anew for each chunk: kept, the weights and angles would take 64 registers in fp64.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xo[i] = (uint32_t)__shfl((int)x[i], lane - j + other);
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(at.c[i]), "+v"(at.s[i]));
+        asm volatile("" : "+v"(at.w), "+v"(at.wo));
+        paired<L, INTERLEAVED>(x, partner, turn, o);
+        x = turned<L>(x, o, at);
+      } else {
+        paired<L, INTERLEAVED>(x, partner, turn, o);
+        x = turned<L>(x, o, at, fa, fb);
+      }
+      if (out != nullptr) {
+        if (in) *reinterpret_cast<u32x4_t*>(out) = x;
+        out += step * to.stride_head;
+      }
+    }
+    if constexpr (KIND != kQuery) {
+      if (!(kept && in)) continue;
+      if (KIND == kKey4 || (KIND == kValue && a.cache_kind == QF_CACHE_KV4)) {
+        using R = Record<D>;
+        uint8_t* rec = static_cast<uint8_t*>(a.cache) + block * a.cache_stride +
+                       ((int64_t)(head - step) * (a.page_size / kTile) + place / kTile) * R::kBytes;
+        const int q = place % kTile;
+        uint32_t byte;
+        const uint32_t codes = four_bits(x, &byte);
+        if constexpr (KIND == kKey4) {
+          *reinterpret_cast<uint32_t*>(rec + R::key(q, 8 * j)) = codes;
+        } else if constexpr (R::kWidth == 8) {
+          *reinterpret_cast<uint32_t*>(rec + R::value(q, 8 * j)) = codes;
+        } else {
+          *reinterpret_cast<uint16_t*>(rec + R::value(q, 8 * j)) = (uint16_t)codes;
+          *reinterpret_cast<uint16_t*>(rec + R::value(q, 8 * j + 4)) = (uint16_t)(codes >> 16);
+        }
+        if (j % 4 == 0) rec[KIND == kKey4 ? R::key_scale(q, 8 * j) : R::value_scale(q, 8 * j)] = (uint8_t)byte;
+      } else {
+        const qf_pages& pages = KIND == kValue ? a.value_pages : a.key_pages;
+        *reinterpret_cast<u32x4_t*>(pages.data + block * pages.stride_block + place * pages.stride_tok +
+                                    (head - step) * pages.stride_head + 8 * j) = x;
+      }
+    }
   }
+}
 
-  // Keys for the 4-bit cache in fp64: their codes do not depend on how a sum was ordered.
-  u32x4_t y = x;
-  const bool wide = a.cache_kind == QF_CACHE_KV4;
-  if (is_q || (is_k && !wide)) {
-    y = turned<L, INTERLEAVED, float>(x, xo, norm, w, wo, at, sign, (float)a.weight_offset, (float)a.eps);
-  } else if (is_k) {
-    y = turned<L, INTERLEAVED, double>(x, xo, norm, w, wo, at, sign, a.weight_offset, a.eps);
-  }
-  if (!live) return;
-  if (is_q || (is_k && a.key_out.data != nullptr)) {
-    const qf_heads& to = is_q ? a.query_out : a.key_out;
-    *reinterpret_cast<u32x4_t*>(to.data + t * to.stride_tok + head * to.stride_head + 8 * j) = y;
-  }
-  if (is_q || a.cache_kind == QF_CACHE_NONE) return;
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.num_blocks * a.page_size) return;
-  const int64_t block = slot <= 0x7fffffff ? divide((int)slot, args.by_page) : slot / a.page_size;
-  const int p = (int)(slot - block * a.page_size);
-  if (a.cache_kind == QF_CACHE_PAGES) {
-    const qf_pages& to = is_k ? a.key_pages : a.value_pages;
-    *reinterpret_cast<u32x4_t*>(to.data + block * to.stride_block + p * to.stride_tok + head * to.stride_head + 8 * j) = y;
+template <int D, bool INTERLEAVED, typename TABLE>
+__global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs args) {
+  constexpr int kRows = kWave / (D / 8);  // rows of a chunk
+  const int row = threadIdx.x % kWave / (D / 8);
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kRopeWaves + threadIdx.x / kWave);
+  if (wave >= args.kv_waves) {
+    const int t = divide(wave - args.kv_waves, args.by_q);
+    const int item = wave - args.kv_waves - t * args.q_items;
+    run_chunks<D, INTERLEAVED, TABLE, kQuery>(args, t, item * args.chunks * kRows + row, kRows);
     return;
   }
-  using R = Record<D>;
-  uint8_t* rec = static_cast<uint8_t*>(a.cache) + block * a.cache_stride +
-                 ((int64_t)head * (a.page_size / kTile) + p / kTile) * R::kBytes;
-  const int q = p % kTile;
-  uint32_t byte;
-  const uint32_t codes = four_bits(y, &byte);
-  if (is_k) {
-    *reinterpret_cast<uint32_t*>(rec + R::key(q, 8 * j)) = codes;
-  } else if constexpr (R::kWidth == 8) {
-    *reinterpret_cast<uint32_t*>(rec + R::value(q, 8 * j)) = codes;
+  const int n = wave / kRopeWaves, tokens = divide(n, args.by_kv);
+  const int item = n - tokens * (args.k_items + args.v_items);
+  const int t = (tokens * kRopeWaves + wave % kRopeWaves) * kRows + row;
+  if (item >= args.k_items) {
+    run_chunks<D, INTERLEAVED, TABLE, kValue>(args, t, (item - args.k_items) * args.chunks, 1);
+  } else if (args.u.cache_kind == QF_CACHE_KV4) {
+    run_chunks<D, INTERLEAVED, TABLE, kKey4>(args, t, item * args.chunks, 1);
   } else {
-    *reinterpret_cast<uint16_t*>(rec + R::value(q, 8 * j)) = (uint16_t)codes;
-    *reinterpret_cast<uint16_t*>(rec + R::value(q, 8 * j + 4)) = (uint16_t)(codes >> 16);
+    run_chunks<D, INTERLEAVED, TABLE, kKey>(args, t, item * args.chunks, 1);
   }
-  if (j % 4 == 0) rec[is_k ? R::key_scale(q, 8 * j) : R::value_scale(q, 8 * j)] = (uint8_t)byte;
 }
 
 struct LoadArgs {
@@ -237,6 +350,7 @@ struct LoadArgs {
   int page, HK, T;
   const int64_t* slots;
   uint16_t *key, *value;
+  Divisor by_heads, by_page;
 };
 
 // D / 8 lanes a head of a token: 8 values each of the key and of the value.
@@ -244,15 +358,15 @@ template <int D>
 __global__ __launch_bounds__(kRopeThreads) void kv4_load_kernel(LoadArgs a) {
   using R = Record<D>;
   constexpr int L = D / 8;
-  const int64_t i = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
-  const int j = (int)(i % L);
+  const uint32_t i = blockIdx.x * kRopeThreads + threadIdx.x;  // (a launch has less than 2^32 threads)
+  const int j = i % L;
   const int64_t at = i / L;  // token * HK + head
   if (at >= (int64_t)a.T * a.HK) return;
-  const int t = (int)(at / a.HK), head = (int)(at - (int64_t)t * a.HK);
+  const int t = divide((int)at, a.by_heads), head = (int)at - t * a.HK;
   const int64_t slot = a.slots[t];
   u32x4_t k = {0, 0, 0, 0}, v = k;
   if (slot >= 0 && slot < a.num_blocks * a.page) {
-    const int64_t block = slot / a.page;
+    const int64_t block = slot <= 0x7fffffff ? divide((int)slot, a.by_page) : slot / a.page;
     const int p = (int)(slot - block * a.page), q = p % kTile;
     const uint8_t* rec = a.cache + block * a.stride + ((int64_t)head * (a.page / kTile) + p / kTile) * R::kBytes;
     uint32_t w;
@@ -277,6 +391,7 @@ RopeFn rope_kernel(bool interleaved, bool f32) {
   return f32 ? &qk_norm_rope_kernel<D, false, float> : &qk_norm_rope_kernel<D, false, uint16_t>;
 }
 
+bool blocks_fit(int64_t blocks, int page) { return blocks <= (int64_t)1 << 40 && blocks <= ((int64_t)1 << 62) / page; }
 bool strides_fit(int64_t a, int64_t b, const void* p) { return a >= 0 && b >= 0 && a % 8 == 0 && b % 8 == 0 && aligned16(p); }
 
 }  // namespace qfk
@@ -307,15 +422,21 @@ extern "C" int qf_qk_norm_rope(const qf_qk_norm_rope_args* args, void* stream) {
     for (const qf_pages* p : {&u.key_pages, &u.value_pages})
       if (!strides_fit(p->stride_tok, p->stride_head, p->data) || p->stride_block < 0 || p->stride_block % 8)
         return QF_ERR_UNSUPPORTED;
-  const int64_t rows = (query ? u.num_heads : 0) + (int64_t)u.num_kv_heads * (cache ? 2 : 1);
-  const int per_wave = kWave / (D / 8);
-  const int64_t parts = (rows + per_wave - 1) / per_wave;
-  // wavefronts are counted in 31 bits
-  if (rows > 0x7fffffff || u.num_tokens * parts > 0x7fffffff - kRopeWaves || u.num_blocks > ((int64_t)1 << 40))
-    return QF_ERR_UNSUPPORTED;
-  const int64_t groups = (u.num_tokens * parts + kRopeWaves - 1) / kRopeWaves;
+  const int64_t rows = kWave / (D / 8), T = u.num_tokens;
+  auto over = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t q_chunks = query ? over(u.num_heads, rows) : 0;
+  const int64_t all = T * q_chunks + over(T, rows) * u.num_kv_heads * (cache ? 2 : 1);
+  const int ch = (int)std::min<int64_t>(std::max<int64_t>(all / (kWavesBeforeMore * (int64_t)compute_units()), 1), kMostChunks);
+  const int64_t q_items = over(q_chunks, ch), k_items = over(u.num_kv_heads, ch), v_items = cache ? k_items : 0;
+  if (q_items > 0xffffff || k_items > 0xffffff) return QF_ERR_UNSUPPORTED;
+  const int64_t kv_waves = over(T, kRopeWaves * rows) * kRopeWaves * (k_items + v_items);
+  const int64_t waves = kv_waves + over(T * q_items, kRopeWaves) * kRopeWaves;
+  // wavefronts are counted in 31 bits, slots in 62
+  if (waves > 0x7fffffff - kRopeWaves || (cache && !blocks_fit(u.num_blocks, u.page_size))) return QF_ERR_UNSUPPORTED;
+  const int64_t groups = waves / kRopeWaves;
   if (!grid_fits(groups, kRopeThreads)) return QF_ERR_UNSUPPORTED;
-  RopeArgs a = {u, divisor(cache ? u.page_size : 1), divisor((int)parts), (int)rows, (int)parts};
+  RopeArgs a = {u, divisor(cache ? u.page_size : 1), divisor(query ? (int)q_items : 1), divisor((int)(k_items + v_items)), ch,
+                (int)kv_waves, (int)q_items, (int)k_items, (int)v_items};
   const RopeFn fn = D == 64    ? rope_kernel<64>(u.interleaved, u.cos_sin_f32)
                     : D == 128 ? rope_kernel<128>(u.interleaved, u.cos_sin_f32)
                                : rope_kernel<256>(u.interleaved, u.cos_sin_f32);
@@ -329,13 +450,13 @@ extern "C" int qf_kv4_load(const void* cache, int64_t cache_stride, int64_t num_
     return QF_ERR_INVALID_ARG;
   const int D = head_size;
   if ((D != 64 && D != 128 && D != 256) || page_size % kTile || cache_stride % 16 || !aligned16(cache) || !aligned16(key) ||
-      !aligned16(value) || num_blocks > ((int64_t)1 << 40) ||
+      !aligned16(value) || !blocks_fit(num_blocks, page_size) ||
       cache_stride < (int64_t)num_kv_heads * (page_size / kTile) * 17 * D)
     return QF_ERR_UNSUPPORTED;
   const int64_t groups = ((int64_t)num_tokens * num_kv_heads * (D / 8) + kRopeThreads - 1) / kRopeThreads;
   if (!grid_fits(groups, kRopeThreads)) return QF_ERR_UNSUPPORTED;
   const LoadArgs a = {static_cast<const uint8_t*>(cache), cache_stride, num_blocks, page_size, num_kv_heads, num_tokens, slots,
-                      key, value};
+                      key, value, divisor(num_kv_heads), divisor(page_size)};
   const auto fn = D == 64 ? &kv4_load_kernel<64> : D == 128 ? &kv4_load_kernel<128> : &kv4_load_kernel<256>;
   hipLaunchKernelGGL(fn, dim3((unsigned)groups), dim3(kRopeThreads), 0, static_cast<hipStream_t>(stream), a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
