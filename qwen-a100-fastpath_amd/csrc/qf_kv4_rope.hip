@@ -206,7 +206,7 @@ __device__ __forceinline__ void run_chunks(const RopeArgs& args, int t, int head
   if (KIND != kQuery && a.cache_kind != QF_CACHE_NONE && heads > 0) slot = a.slots[t];
   const uint16_t* p = from.data + t * from.stride_tok + head * from.stride_head + 8 * j;
   u32x4_t next = {0, 0, 0, 0};
-  if (head < heads) next = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+  if (head < heads) next = *reinterpret_cast<const u32x4_t*>(p);
 
   const int half = a.rot / 16;  // lanes from a pair's first value to its second
   const int other = INTERLEAVED || !turn ? j : j < half ? j + half : j - half;
@@ -275,7 +275,7 @@ __device__ __forceinline__ void run_chunks(const RopeArgs& args, int t, int head
     const bool in = head < heads;
     head += step;
     p += step * from.stride_head;
-    if (c + 1 < args.chunks && head < heads) next = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    if (c + 1 < args.chunks && head < heads) next = *reinterpret_cast<const u32x4_t*>(p);
     if constexpr (KIND != kValue) {
       float o[8];
       if constexpr (KIND == kKey4) {
