@@ -373,7 +373,8 @@ struct Walk {
   typedef void __attribute__((address_space(3)))* lptr_t;
 
   __device__ __forceinline__ void copy(const uint8_t* from, uint8_t* to) const {
-    __builtin_amdgcn_global_load_lds((gptr_t)from, (lptr_t)to, 16, 0, 2);  // 2: read once, not kept
+    // 2: read once, not kept (one request of 100 000 positions 36 us, 39 kept; 48 requests out of 12 layers' caches 26.3, 27.6)
+    __builtin_amdgcn_global_load_lds((gptr_t)from, (lptr_t)to, 16, 0, 2);
   }
   __device__ __forceinline__ void copy_step(const uint8_t* r0, const uint8_t* r1, uint8_t* slot) const {
     if constexpr (kDwords == 4) {
@@ -466,7 +467,8 @@ struct Walk {
     }
   }
 
-  // Steps first, first + by, ... of the positions begin .. end - 1, through two slots of kSlot bytes.  The records of 32 steps are
+  // Steps first, first + by, ... of the positions begin .. end - 1, through two slots of kSlot bytes (100 000 positions 36 us, with
+  // three slots 39, with four 40: what is in flight is enough, and more of it in other places of the cache is read slower).  The records of 32 steps are
   // looked up at once, a record a lane.
   __device__ __forceinline__ void run(int begin, int end, int first, int by, uint8_t* slots) {
     const int n_steps = (end - begin + kStep - 1) / kStep;
@@ -914,26 +916,30 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   }
 }
 
-// A workgroup a pair of tiles (values n and n + 1 of each lane's run): 4 wavefronts a tile share the splits, up to 16 of which each
-// requests at once (they come from other XCDs' writes, a microsecond away); then the wavefronts through LDS.
-constexpr int kCombineWaves = 8;
+// A workgroup a slice (SLICES of them, 2 or 4) of a pair of tiles (values n and n + 1 of each lane's run): the splits are shared by
+// its wavefronts, and by halves of a wavefront where SLICES is 4, 4 requested by each at once (they come from other XCDs'
+// writes, a microsecond away); then the shares through LDS.
 // TILED: of the tile kernel's splits, else of the split kernel's.
-template <int D, bool TILED>
-__global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(AttnArgs a) {
+template <int D, bool TILED, int SLICES, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void attn_combine_kernel(AttnArgs a) {
   using W = Walk<D, 1>;
   constexpr int kPairs = TileShape<D>::kRows / 16 * W::kDTiles / 2;  // of a row tile (TILED)
-  constexpr int kGroups = kCombineWaves / 2;
-  __shared__ float sm_m[kGroups][kWave], sm_l[kGroups][kWave];
-  __shared__ __align__(16) f32x4_t sm_o[kCombineWaves][kWave];
+  constexpr int kSlice = kWave / SLICES;                             // lanes of a tile
+  constexpr int kGroups = WAVES * SLICES / 2;
+  __shared__ float2 sm_ml[kGroups][kSlice];
+  __shared__ __align__(16) f32x4_t sm_o[kGroups][2][kSlice];
   const int hkv = blockIdx.y, b = blockIdx.z;
-  const int pair = TILED ? blockIdx.x % kPairs : blockIdx.x, row_tile = TILED ? blockIdx.x / kPairs : 0;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tile = 2 * pair + wave % 2, g = wave / 2;
-  const int l16 = lane % 16, qg = lane / 16, part_row = tile / W::kDTiles * 16 + l16;
+  const int slice = blockIdx.x % SLICES, x = blockIdx.x / SLICES;
+  const int pair = TILED ? x % kPairs : x, row_tile = TILED ? x / kPairs : 0;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int at = lane % kSlice, odd = lane / kSlice % 2, g = wave * (SLICES / 2) + lane / (2 * kSlice);
+  const int tile_lane = slice * kSlice + at, tile = 2 * pair + odd;
+  const int l16 = tile_lane % 16, qg = tile_lane / 16, part_row = tile / W::kDTiles * 16 + l16;
   const int row = row_tile * TileShape<D>::kRows + part_row;
   const Request r = request(a, b);
   const int rows = r.n * a.G;
   if (row - l16 >= rows) return;
-  int splits, kTiles, slot_rows;
+  int splits, tiles, slot_rows;
   int64_t slot;
   if constexpr (TILED) {
     if (rows <= a.few) return;
@@ -941,29 +947,30 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(Att
     const int last_row = min((row_tile + 1) * TileShape<D>::kRows, rows) - 1;
     stage_splits(a, max(r.seq - r.n + divide(last_row, a.by_g) + 1, 0), splits, per);
     slot = tile_slot(a, b, hkv, row_tile);
-    kTiles = 2 * kPairs;
+    tiles = 2 * kPairs;
     slot_rows = TileShape<D>::kRows;
   } else {
     const int2 place = a.plan[b];
     splits = place.y;
     slot = (int64_t)hkv * a.slots + place.x;
-    kTiles = gridDim.x * 2;
+    tiles = gridDim.x / SLICES * 2;
     slot_rows = a.rows;
   }
   if (splits < 2) return;
   float m = -__builtin_inff(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   if (row < rows) {
-    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.o_part) + tile * kWave + lane;
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.o_part) + (slot * tiles + tile) * kWave + tile_lane;
+    const float2* stats = a.ml_part + slot * slot_rows + part_row;
     auto add = [&](int s, auto batch) {  // the splits s, s + kGroups, ... that there are, `batch` of them
       constexpr int kBatch = decltype(batch)::value;
       float2 ml[kBatch];
       f32x4_t v[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int at = min(s + i * kGroups, splits - 1);
-        ml[i] = a.ml_part[(slot + at) * slot_rows + part_row];
-        v[i] = from[(slot + at) * kTiles * kWave];
+        const int n = min(s + i * kGroups, splits - 1);
+        ml[i] = stats[(int64_t)n * slot_rows];
+        v[i] = from[(int64_t)n * (tiles * kWave)];
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -977,28 +984,26 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(Att
       }
     };
     int s = g;
-    for (; s + 4 * kGroups < splits; s += 16 * kGroups) add(s, std::integral_constant<int, 16>{});
-    if (s < splits) add(s, std::integral_constant<int, 4>{});
+    for (; s + 2 * kGroups < splits; s += 4 * kGroups) add(s, std::integral_constant<int, 4>{});
+    if (s < splits) add(s, std::integral_constant<int, 2>{});
   }
-  if (wave % 2 == 0) {
-    sm_m[g][lane] = m;
-    sm_l[g][lane] = l;
-  }
-  sm_o[wave][lane] = o;
+  if (odd == 0) sm_ml[g][at] = make_float2(m, l);
+  sm_o[g][odd][at] = o;
   __syncthreads();
-  if (wave != 0 || row >= rows) return;
-  float top = sm_m[0][lane];
+  if (threadIdx.x >= kSlice || row >= rows) return;
+  float top = sm_ml[0][at].x;
 #pragma unroll
-  for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sm_m[i][lane]);
+  for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sm_ml[i][at].x);
   const float ref = top == -__builtin_inff() ? 0.f : top;
-  f32x4_t even = {0.f, 0.f, 0.f, 0.f}, odd = even;
+  f32x4_t evens = {0.f, 0.f, 0.f, 0.f}, odds = evens;
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    const float weight = fast_exp2(sm_m[i][lane] - ref);
-    even += sm_o[2 * i][lane] * weight;
-    odd += sm_o[2 * i + 1][lane] * weight;
-    l += sm_l[i][lane] * weight;
+    const float2 ml = sm_ml[i][at];
+    const float weight = fast_exp2(ml.x - ref);
+    evens += sm_o[i][0][at] * weight;
+    odds += sm_o[i][1][at] * weight;
+    l += ml.y * weight;
   }
   const int qi = divide(row, a.by_g);
   const float inv = r.seq - r.n + qi < 0 ? 0.f : 1.f / l;
@@ -1007,7 +1012,7 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attn_combine_kernel(Att
   uint16_t* to = a.out + (int64_t)(r.tok0 + qi) * a.so_t + (int64_t)(hkv * a.G + (row - qi * a.G)) * a.so_h +
                  16 * Rec::kWidth * h + Rec::kWidth * 4 * qg + n;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(to + Rec::kWidth * i) = pack_bf16(even[i] * inv, odd[i] * inv);
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(to + Rec::kWidth * i) = pack_bf16(evens[i] * inv, odds[i] * inv);
 }
 
 typedef void (*AttnFn)(AttnArgs);
@@ -1026,6 +1031,18 @@ Split split_kernel(int rt) {
 Split split_of(int D, int rows) {
   const int rt = (rows + 15) / 16;
   return D == 64 ? split_kernel<64>(rt) : D == 128 ? split_kernel<128>(rt) : split_kernel<256>(rt);
+}
+
+struct Combine {
+  AttnFn fn;
+  int slices, threads;
+};
+template <bool TILED, int SLICES, int WAVES>
+Combine combine_of(int D) {
+  return {D == 64    ? &attn_combine_kernel<64, TILED, SLICES, WAVES>
+          : D == 128 ? &attn_combine_kernel<128, TILED, SLICES, WAVES>
+                     : &attn_combine_kernel<256, TILED, SLICES, WAVES>,
+          SLICES, WAVES * kWave};
 }
 
 // How a call runs: its launches and the parts of its workspace.
@@ -1097,6 +1114,7 @@ bool sizes_fit(const qf_kv4_attention_args& u) {
 std::atomic<uint64_t> g_raised[3][5];
 
 int launch(AttnFn fn, dim3 grid, int threads, size_t lds, std::atomic<uint64_t>& raised, hipStream_t s, const AttnArgs& a) {
+  if (!grid_fits(grid.x, threads)) return QF_ERR_UNSUPPORTED;
   if (lds + 4096 > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(fn), (int)lds, raised)) return QF_ERR_HIP;
   hipLaunchKernelGGL(fn, grid, dim3(threads), lds, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
@@ -1170,8 +1188,8 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
     int st = launch(fn, dim3((unsigned)(p.row_tiles * p.tile_splits), a.HKV, a.B), TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
     if (st != QF_OK) return st;
     if (p.tile_splits > 1) {
-      const AttnFn comb = D == 64 ? &attn_combine_kernel<64, true> : D == 128 ? &attn_combine_kernel<128, true> : &attn_combine_kernel<256, true>;
-      st = launch(comb, dim3((unsigned)(p.row_tiles * (tile_rows(D) / 16 * (D / 32))), a.HKV, a.B), kCombineWaves * kWave, 0, g_raised[di][0], s, a);
+      const Combine c = combine_of<true, 2, 4>(D);
+      st = launch(c.fn, dim3((unsigned)(p.row_tiles * (tile_rows(D) / 16 * (D / 32)) * c.slices), a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
       if (st != QF_OK) return st;
     }
     if (!p.split) return QF_OK;
@@ -1180,8 +1198,11 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   a.ml_part = reinterpret_cast<float2*>(ws + p.ml);
   a.plan = reinterpret_cast<int2*>(ws + p.plan);
   const Split k = split_of(D, p.rows);
-  const AttnFn comb = D == 64 ? &attn_combine_kernel<64, false> : D == 128 ? &attn_combine_kernel<128, false> : &attn_combine_kernel<256, false>;
+  const int64_t pairs = (int64_t)k.row_tiles * (D / 32) * a.HKV * a.B;
+  // Small slices where that gives a compute unit a few workgroups at most (3 queries behind 38 000 positions, 64 splits of 18 rows of
+  // 256: 26.4 -> 23.1 us with the splits themselves, 7 requests of 4 queries 12.6 -> 10.8; 16 requests of up to 3000 18.5, 18.7).
+  const Combine c = 4 * pairs <= 4 * compute_units() ? combine_of<false, 4, 8>(D) : combine_of<false, 2, 4>(D);
   const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, k.lds, g_raised[di][k.row_tiles], s, a);
   if (st != QF_OK) return st;
-  return launch(comb, dim3(k.row_tiles * D / 32, a.HKV, a.B), kCombineWaves * kWave, 0, g_raised[di][0], s, a);
+  return launch(c.fn, dim3(k.row_tiles * D / 32 * c.slices, a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
 }
