@@ -453,6 +453,7 @@ extern "C" int qf_kv4_load(const void* cache, int64_t cache_stride, int64_t num_
       !aligned16(value) || !blocks_fit(num_blocks, page_size) ||
       cache_stride < (int64_t)num_kv_heads * (page_size / kTile) * 17 * D)
     return QF_ERR_UNSUPPORTED;
+  if ((int64_t)num_tokens * num_kv_heads > 0x7fffffff) return QF_ERR_UNSUPPORTED;  // heads are counted in 31 bits
   const int64_t groups = ((int64_t)num_tokens * num_kv_heads * (D / 8) + kRopeThreads - 1) / kRopeThreads;
   if (!grid_fits(groups, kRopeThreads)) return QF_ERR_UNSUPPORTED;
   const LoadArgs a = {static_cast<const uint8_t*>(cache), cache_stride, num_blocks, page_size, num_kv_heads, num_tokens, slots,

@@ -105,6 +105,13 @@ def test_load_refusals(kw, want):
     assert K.load().qf_kv4_load(*(v[n] for n in "cache stride blocks page heads D slots T key value".split()), None) == want
 
 
+def test_a_load_whose_threads_pass_64_bits_is_refused():
+    """(2^31 - 1)^2 heads of 8 lanes are more than 2^64 threads: their number must not wrap to a small one."""
+    n = 2 ** 31 - 1
+    assert K.load().qf_kv4_load(P, 2 * 17 * 64 * n, 4, 32, n, 64, P, n, P, P, None) == UNSUPPORTED
+
+
+
 def _attention(ws=P, nbytes=1 << 40, **kw):
     v = dict(query=K.Heads(P, 1024, 128), out=K.Heads(P, 1024, 128), cache=P, cache_stride=2 * 17 * 128, num_blocks=9, block_table=P,
              bt_stride=8, seq_lens=P, cu_q=None, scale=0.1, max_blocks=8, num_tokens=8, num_reqs=4, q_len=2, num_heads=8,
