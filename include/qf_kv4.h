@@ -105,8 +105,8 @@ typedef struct qf_qk_norm_rope_args {
  * first `rot` values of a head are turned by the angles of the token's row of cos_sin: pairs (i, i + rot / 2), or (2 i, 2 i
  * + 1) with interleaved, (a, b) -> (a c - b s, b c + a s).  Rounded once to bf16.  With a cache, the rounded key and the
  * value go to the token's slot: as they are (pages), or in the 4-bit form of the bf16 values.  A slot outside
- * [0, num_blocks * page_size) is not written; of tokens with one slot any may be kept.  A position is kept inside
- * [0, num_positions).
+ * [0, num_blocks * page_size) is not written.  Two tokens must not have one slot: of what it then holds some bytes may be the
+ * one's and some the other's.  A position is kept inside [0, num_positions).
  * All arithmetic is fp32; that of keys for the 4-bit cache is fp64, so that no code depends on the order of a sum.
  * D = 64, 128 or 256; rot a multiple of 16 up to D, or 0 (no rotation: positions and cos_sin are not read). */
 int qf_qk_norm_rope(const qf_qk_norm_rope_args* args, void* stream);

@@ -468,8 +468,8 @@ struct Walk {
   }
 
   // Steps first, first + by, ... of the positions begin .. end - 1, through two slots of kSlot bytes (100 000 positions 36 us, with
-  // three slots 39, with four 40: what is in flight is enough, and more of it in other places of the cache is read slower).  The records of 32 steps are
-  // looked up at once, a record a lane.
+  // three slots 39, with four 40: what is in flight is enough, and more of it in other places of the cache is read slower).  The
+  // records of 32 steps are looked up at once, a record a lane.
   __device__ __forceinline__ void run(int begin, int end, int first, int by, uint8_t* slots) {
     const int n_steps = (end - begin + kStep - 1) / kStep;
     const int mine = first < n_steps ? (n_steps - 1 - first) / by + 1 : 0;

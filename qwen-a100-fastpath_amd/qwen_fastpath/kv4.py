@@ -25,8 +25,8 @@ def kv4_cache(num_blocks: int, page_size: int, num_kv_heads: int, head_size: int
 
 
 def kv4_store(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> None:
-    """key and value bf16 [T, H_kv, D] into the cache's slots (int64 [T]; those outside the cache, as -1, are not written; of
-    tokens with one slot any may be kept)."""
+    """key and value bf16 [T, H_kv, D] into the cache's slots (int64 [T]; those outside the cache, as -1, are not written; no
+    two tokens may have one slot: their bytes could mix in it)."""
     if key.is_cuda:
         if K.try_call("rope", None, key, value, None, None, None, None, cache, slots, 0.0, 0.0, False, None, None) is not None:
             return

@@ -33,9 +33,10 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
     rot]: each position's cosines, then its sines, rot a multiple of 16 up to D; positions int64 [T], kept inside the table; both
     None: no rotation.  A pair is (i, i + rot / 2), or (2 i, 2 i + 1) with `interleaved`.  D is 64, 128 or 256.
 
-    With a cache, the key and the value go to the slots (int64 [T]; those outside the cache, as -1, are not written): `cache`
-    is (key_cache, value_cache), bf16 [blocks, page, H_kv, D], or a 4-bit cache (kv4_cache).  The key is returned only where
-    key_out is given, or without a cache.  query_out and key_out may be query and key (in place); no other overlap.
+    With a cache, the key and the value go to the slots (int64 [T]; those outside the cache, as -1, are not written; no two
+    tokens may have one slot: their bytes could mix in it).  `cache` is (key_cache, value_cache), bf16 [blocks, page, H_kv, D],
+    or a 4-bit cache (kv4_cache).  The key is returned only where key_out is given, or without a cache.  query_out and key_out
+    may be query and key (in place); no other overlap.
     Arithmetic is fp32 with one rounding to bf16; keys for the 4-bit cache are computed in fp64, rounded to bf16 and these
     values quantised, so that a token's codes do not depend on the order of a sum."""
     if key.is_cuda:
