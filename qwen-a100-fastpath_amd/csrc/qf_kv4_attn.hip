@@ -1090,14 +1090,19 @@ Plan plan_of(const qf_kv4_attention_args& u) {
     return p;
   }
   p.rows = rows < QF_KV4_MAX_ROWS ? (int)rows : QF_KV4_MAX_ROWS;
-  // A workgroup a CU; two where the requests by themselves fill the machine, so that the longest of them is cut finer (48 requests
-  // of up to 9000 positions over 8 kv heads: 28.2 -> 25.0 us; 16 requests of up to 3000, which do not: 18.8 -> 22.7).
-  const int cus = compute_units() * ((int64_t)u.num_reqs * u.num_kv_heads >= compute_units() ? 2 : 1);
+  // A workgroup a compute unit.  Three where the requests by themselves fill the machine, so that the longest of them is cut finer and
+  // one's waits are another's work: 48 requests of up to 9000 positions over 8 kv heads 28.0 us with one, 24.9 with two, 23.0 with
+  // three; 16 requests, which do not fill it, 18.6 with one, 22.9 with two.  Not where the registers of a workgroup (over 180 a
+  // lane) leave no room for three (40 requests of 32 rows 29.8, 32.9, 33.0; D = 256, 70 requests of 30 rows 39.9, 46.4, 55.1), nor
+  // where each workgroup's look at all requests counts (260 over one kv head 16.3, 17.6, 18.9; 400 over 8 heads 56, 58, 60).
+  const int row_tiles = split_of(u.head_size, p.rows).row_tiles;
+  const bool full = (int64_t)u.num_reqs * u.num_kv_heads >= compute_units();
+  const int cus = compute_units() * (full && std::min(row_tiles, 2) * u.head_size <= 128 && u.num_reqs <= 128 ? 3 : 1);
   p.workers = (cus + u.num_kv_heads - 1) / u.num_kv_heads;
   p.slots = p.workers + u.num_reqs;
   const size_t parts = (size_t)u.num_kv_heads * p.slots;
   p.o = n;
-  n += parts * split_of(u.head_size, p.rows).row_tiles * 16 * u.head_size * sizeof(float);
+  n += parts * row_tiles * 16 * u.head_size * sizeof(float);
   p.ml = n;
   n += round256(parts * p.rows * sizeof(float2));
   p.plan = n;
@@ -1111,11 +1116,13 @@ bool sizes_fit(const qf_kv4_attention_args& u) {
          (int64_t)u.q_len * (u.num_heads / u.num_kv_heads) <= 0x3fffffff && u.num_kv_heads <= 65535 && u.num_reqs <= 65535;
 }
 
+constexpr int kAloneLds = 82 * 1024;  // of 160 KiB
+constexpr int kManyPositions = 4096;
 std::atomic<uint64_t> g_raised[3][5];
 
 int launch(AttnFn fn, dim3 grid, int threads, size_t lds, std::atomic<uint64_t>& raised, hipStream_t s, const AttnArgs& a) {
   if (!grid_fits(grid.x, threads)) return QF_ERR_UNSUPPORTED;
-  if (lds + 4096 > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(fn), (int)lds, raised)) return QF_ERR_HIP;
+  if (lds + 4096 > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(fn), std::max((int)lds, kAloneLds), raised)) return QF_ERR_HIP;
   hipLaunchKernelGGL(fn, grid, dim3(threads), lds, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
@@ -1202,7 +1209,10 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   // Small slices where that gives a compute unit a few workgroups at most (3 queries behind 38 000 positions, 64 splits of 18 rows of
   // 256: 26.4 -> 23.1 us with the splits themselves, 7 requests of 4 queries 12.6 -> 10.8; 16 requests of up to 3000 18.5, 18.7).
   const Combine c = 4 * pairs <= 4 * compute_units() ? combine_of<false, 4, 8>(D) : combine_of<false, 2, 4>(D);
-  const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, k.lds, g_raised[di][k.row_tiles], s, a);
+  // Where a workgroup a compute unit is all there is, none takes two of them: each asks for more than half of the LDS (100 000
+  // positions 35.7 -> 30.8 us, 30 000 17.0 -> 15.5, D = 256 19.6 -> 16.5; at 1000 8.6 -> 8.9, so not for tables that end there).
+  const bool alone = (int64_t)p.slots * a.HKV <= compute_units() * 5 / 4 && (int64_t)a.max_blocks * a.page >= kManyPositions;
+  const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, alone ? std::max(k.lds, kAloneLds) : k.lds, g_raised[di][k.row_tiles], s, a);
   if (st != QF_OK) return st;
   return launch(c.fn, dim3(k.row_tiles * D / 32 * c.slices, a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
 }
