@@ -780,10 +780,13 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   uint32_t ks, vs;
   auto load_share = [&](int stage) {
     const uint8_t* rec = where(stage % 16 * 4 + mine);
-    k = *reinterpret_cast<const Keys*>(rec + w.l16 * (D / 2) + half * 64 + w.qg * (4 * W::kDwords) + (D == 256 ? 0 : part * 4 * kKeyDwords));
+    k = *reinterpret_cast<const Keys*>(rec + w.l16 * (D / 2) + half * 64 + w.qg * (4 * W::kDwords) +
+                                       (D == 256 ? 0 : part * 4 * kKeyDwords));
     v = *reinterpret_cast<const typename W::Data::Run*>(rec + R::kValues + half * 1024 + w.lane * 4 * W::kDwords);
-    ks = *reinterpret_cast<const uint32_t*>(rec + R::kKeyScales + (W::kDwords == 4 ? 4 * half + w.qg : w.qg / 2) * kTile + (w.l16 & 12));
-    vs = *reinterpret_cast<const uint32_t*>(rec + R::kValueScales + (W::kDwords == 4 ? 4 * half + w.l16 / 4 : w.l16 / 8) * kTile + 4 * w.qg);
+    ks = *reinterpret_cast<const uint32_t*>(rec + R::kKeyScales + (W::kDwords == 4 ? 4 * half + w.qg : w.qg / 2) * kTile +
+                                            (w.l16 & 12));
+    vs = *reinterpret_cast<const uint32_t*>(rec + R::kValueScales + (W::kDwords == 4 ? 4 * half + w.l16 / 4 : w.l16 / 8) * kTile +
+                                            4 * w.qg);
   };
   auto widen_share = [&](int stage) {
     const int pos = stage * kStage + mine * kTile, buffer = stage & 1;
@@ -1075,7 +1078,8 @@ Plan plan_of(const qf_kv4_attention_args& u) {
     p.row_tiles = (int)((rows + per - 1) / per);
     // Positions are split where the row tiles leave compute units idle (100 tokens behind 4000 positions, 64 heads over 8: 115 -> 34
     // us; twice as many splits 47).
-    const int64_t all = (int64_t)p.row_tiles * u.num_reqs, by_tokens = ((int64_t)u.num_tokens * (u.num_heads / u.num_kv_heads) + per - 1) / per + u.num_reqs;
+    const int64_t all = (int64_t)p.row_tiles * u.num_reqs;
+    const int64_t by_tokens = ((int64_t)u.num_tokens * (u.num_heads / u.num_kv_heads) + per - 1) / per + u.num_reqs;
     const int64_t groups = (all < by_tokens ? all : by_tokens) * u.num_kv_heads;
     int64_t splits = compute_units() / groups;
     splits = splits < 1 ? 1 : splits > 16 ? 16 : splits;
@@ -1127,7 +1131,8 @@ std::atomic<uint64_t> g_raised[3][5];
 
 int launch(AttnFn fn, dim3 grid, int threads, size_t lds, std::atomic<uint64_t>& raised, hipStream_t s, const AttnArgs& a) {
   if (!grid_fits(grid.x, threads)) return QF_ERR_UNSUPPORTED;
-  if (lds + 4096 > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(fn), std::max((int)lds, kAloneLds), raised)) return QF_ERR_HIP;
+  if (lds + 4096 > kDefaultLds && !raise_lds(reinterpret_cast<const void*>(fn), std::max((int)lds, kAloneLds), raised))
+    return QF_ERR_HIP;
   hipLaunchKernelGGL(fn, grid, dim3(threads), lds, s, a);
   return hipGetLastError() == hipSuccess ? QF_OK : QF_ERR_HIP;
 }
@@ -1147,7 +1152,8 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
       u.bt_stride < 0 || u.num_tokens < 1 || u.num_reqs < 1 || u.q_len < 1 || u.num_heads < 1 || u.num_kv_heads < 1 ||
       u.page_size < 1 || !(u.scale == u.scale) || (!u.cu_q && (int64_t)u.num_reqs * u.q_len > u.num_tokens))
     return QF_ERR_INVALID_ARG;
-  if (!sizes_fit(u) || (int64_t)u.max_blocks * u.page_size > 0x7fffffc0 || u.page_size % kTile || u.cache_stride % 16 || !aligned16(u.cache) ||
+  if (!sizes_fit(u) || (int64_t)u.max_blocks * u.page_size > 0x7fffffc0 || u.page_size % kTile || u.cache_stride % 16 ||
+      !aligned16(u.cache) ||
       u.cache_stride < (int64_t)u.num_kv_heads * (u.page_size / kTile) * 17 * u.head_size)
     return QF_ERR_UNSUPPORTED;
   for (const qf_heads* h : {&u.query, &u.out})
@@ -1197,11 +1203,13 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
     static_assert(TileShape<64>::kWaves == TileShape<128>::kWaves && TileShape<256>::kWaves == TileShape<128>::kWaves, "one shape");
     const AttnFn fn = D == 64 ? &attn_tile_kernel<64> : D == 128 ? &attn_tile_kernel<128> : &attn_tile_kernel<256>;
     const int lds = D == 64 ? TileShape<64>::kLds : D == 128 ? TileShape<128>::kLds : TileShape<256>::kLds;
-    int st = launch(fn, dim3((unsigned)(p.row_tiles * p.tile_splits), a.HKV, a.B), TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
+    const dim3 grid((unsigned)(p.row_tiles * p.tile_splits), a.HKV, a.B);
+    int st = launch(fn, grid, TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
     if (st != QF_OK) return st;
     if (p.tile_splits > 1) {
       const Combine c = combine_of<true, 2, 4>(D);
-      st = launch(c.fn, dim3((unsigned)(p.row_tiles * (tile_rows(D) / 16 * (D / 32)) * c.slices), a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
+      const int parts = tile_rows(D) / 16 * (D / 32) * c.slices;  // of a row tile
+      st = launch(c.fn, dim3((unsigned)(p.row_tiles * parts), a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
       if (st != QF_OK) return st;
     }
     if (!p.split) return QF_OK;
@@ -1217,7 +1225,8 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   // Where a workgroup a compute unit is all there is, none takes two of them: each asks for more than half of the LDS (100 000
   // positions 35.7 -> 30.8 us, 30 000 17.0 -> 15.5, D = 256 19.6 -> 16.5; at 1000 8.6 -> 8.9, so not for tables that end there).
   const bool alone = (int64_t)p.slots * a.HKV <= compute_units() * 5 / 4 && (int64_t)a.max_blocks * a.page >= kManyPositions;
-  const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, alone ? std::max(k.lds, kAloneLds) : k.lds, g_raised[di][k.row_tiles], s, a);
+  const int lds = alone ? std::max(k.lds, kAloneLds) : k.lds;
+  const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, lds, g_raised[di][k.row_tiles], s, a);
   if (st != QF_OK) return st;
   return launch(c.fn, dim3(k.row_tiles * D / 32 * c.slices, a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
 }

@@ -170,7 +170,8 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (cos_sin != nullptr) {
     u.cos_sin_f32 = cos_sin->scalar_type() == at::kFloat;
     if (cos_sin->dim() != 2 || (!u.cos_sin_f32 && cos_sin->scalar_type() != at::kBFloat16) || !cos_sin->is_contiguous() ||
-        cos_sin->size(0) < 1 || cos_sin->size(1) > D || cos_sin->size(1) % 16 || cos_sin->size(1) < 16 || !aligned(cos_sin->data_ptr()) ||
+        cos_sin->size(0) < 1 || cos_sin->size(1) > D || cos_sin->size(1) % 16 || cos_sin->size(1) < 16 ||
+        !aligned(cos_sin->data_ptr()) ||
         !vec(*positions, at::kLong, T))
       Py_RETURN_NONE;
     u.rot = (int)cos_sin->size(1);
@@ -281,7 +282,8 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     Py_RETURN_NONE;
   const int64_t T = query->size(0), H = query->size(1), B = seq->size(0);
   if (T < 1 || T > kIntMax || B < 1 || B > kIntMax || H < 1 || H > kIntMax || HK > kIntMax || H % HK || q_len < 1 ||
-      q_len > kIntMax || bt->size(1) * page > 0x7fffffc0 || !heads(*query, T, H, D, &u.query) || !vec(*seq, at::kInt, B) || !table(*bt, B, &u.bt_stride) ||
+      q_len > kIntMax || bt->size(1) * page > 0x7fffffc0 || !heads(*query, T, H, D, &u.query) || !vec(*seq, at::kInt, B) ||
+      !table(*bt, B, &u.bt_stride) ||
       !(u.scale == u.scale) || (cu != nullptr ? !vec(*cu, at::kInt, B + 1) : B * q_len > T))
     Py_RETURN_NONE;
   u.cache = c->data_ptr();

@@ -6,9 +6,9 @@
 // values their page, or blocks of 32 values (4 lanes) to 4 bits.
 //
 // A wavefront takes several chunks of one kind, the next one's rows requested before the last one's work, and the angles and
-// weights, which a lane needs for one token only, once for all of them.  Queries: the chunks are heads of one token.  Keys and values: a chunk is one head
-// of 64 / L neighbouring tokens, whose bytes of a 4-bit record stand together, and the 4 wavefronts of a workgroup take further
-// neighbours.
+// weights, which a lane needs for one token only, once for all of them.  Queries: the chunks are heads of one token.  Keys and
+// values: a chunk is one head of 64 / L neighbouring tokens, whose bytes of a 4-bit record stand together, and the 4 wavefronts
+// of a workgroup take further neighbours.
 //
 // Memory bounds it where there are many rows (2048 tokens of 64 + 8 heads of 128 into 4 bits: 80 MB in 19 us, 4.2 TB/s; 8191 of 16 + 2
 // into bf16 pages: 86 MB in 16.8 us, 5.1 TB/s, part of it in the caches), the chain position, angles, stores where there are few
