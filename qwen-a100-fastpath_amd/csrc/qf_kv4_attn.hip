@@ -46,6 +46,8 @@ struct AttnArgs {
   float* o_part;   // [HKV][slots][rows][D]
   float2* ml_part; // [HKV][slots][rows]: exponent reference, sum
   int2* plan;      // [B]: first slot and slots of a request
+  int fast;  // tile kernel: workgroups that stand together, the heads of a row tile or the row tiles of a head
+  Divisor by_fast;
   int row_tiles, tile_splits;  // tile kernel: of a request at most, and of a row tile at most; partials [B][HKV][row tile][split]
   int slots;
 };
@@ -734,10 +736,11 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ uint32_t odd[2][S::kWaves];  // a wavefront met a block of NaN that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int hkv = blockIdx.y, b = blockIdx.z;
+  const int b = blockIdx.z, quotient = divide(blockIdx.x, a.by_fast), rest = blockIdx.x - quotient * a.fast;
+  const int x = a.tile_splits == 1 ? quotient : rest, hkv = a.tile_splits == 1 ? rest : quotient;
   const Request r = request(a, b);
   const int rows = r.n * a.G;
-  const int row_tile = a.row_tiles - 1 - blockIdx.x / a.tile_splits;  // the rows that see most come first
+  const int row_tile = a.row_tiles - 1 - x / a.tile_splits;  // the rows that see most come first
   const int row0 = row_tile * S::kRows;
   if (row0 >= rows || rows <= a.few) return;
   const int r0 = row0 + wave * 16 * S::kRT;
@@ -748,7 +751,7 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   const int end = seen(row0 + S::kRows - 1), all_see = seen(row0);
   int splits, per;
   stage_splits(a, end, splits, per);
-  const int split = blockIdx.x % a.tile_splits;
+  const int split = x % a.tile_splits;
   if (split >= splits) return;
   const int first_stage = split * per, n_stages = min((end + kStage - 1) / kStage, first_stage + per);
   const int last_tile = (end - 1) / kTile * kTile;
@@ -1203,7 +1206,14 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
     static_assert(TileShape<64>::kWaves == TileShape<128>::kWaves && TileShape<256>::kWaves == TileShape<128>::kWaves, "one shape");
     const AttnFn fn = D == 64 ? &attn_tile_kernel<64> : D == 128 ? &attn_tile_kernel<128> : &attn_tile_kernel<256>;
     const int lds = D == 64 ? TileShape<64>::kLds : D == 128 ? TileShape<128>::kLds : TileShape<256>::kLds;
-    const dim3 grid((unsigned)(p.row_tiles * p.tile_splits), a.HKV, a.B);
+    const int64_t groups = (int64_t)p.row_tiles * p.tile_splits * a.HKV;
+    if (!grid_fits(groups, TileShape<128>::kWaves * kWave)) return QF_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)groups, 1, a.B);
+    // The heads of a row tile together: those that see most come first over all heads, and where the heads are a multiple of 8
+    // an XCD's L2 holds its own heads' positions (4096 tokens of 32 heads over 8 from the start 234 -> 137 us; 2048 of 64 over 8 behind
+    // 8192 positions 556 -> 510; D = 256 341 -> 300).  With positions split a head's workgroups together (34.7 us, 37.6).
+    a.fast = p.tile_splits == 1 ? a.HKV : p.row_tiles * p.tile_splits;
+    a.by_fast = divisor(a.fast);
     int st = launch(fn, grid, TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
     if (st != QF_OK) return st;
     if (p.tile_splits > 1) {
