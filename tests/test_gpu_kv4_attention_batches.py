@@ -47,3 +47,18 @@ def test_a_wide_table_after_a_narrow_one():
             wide[:, :s["table"].shape[1]] = s["table"]
             s["table"] = wide
             _check(s, _call(s))
+
+
+@pytest.mark.parametrize("B,D", [(7, 128), (7, 256), (64, 64), (70, 64)])
+def test_chunks_in_any_order(B, D):
+    """Requests of equal and of different lengths, the longest last, some that only single tokens have, some with none."""
+    g = H.gen(B + D)
+    seq = sorted(_lengths(D, B, 260))
+    seq[1] = seq[2] = seq[3]
+    q = [int(torch.randint(0, 60, (1,), generator=g)) for _ in range(B)]
+    q[0], q[B - 1], q[B - 2] = 0, 90, 1
+    s = _batch(B * D, seq, q, 4, 2, D, 16)
+    _check(s, _call(s))
+    back = dict(s, seq=seq[::-1], q=q[::-1], cu=torch.tensor([0] + q[::-1]).cumsum(0), table=s["table"].flip(0), keys=s["keys"][::-1],
+                vals=s["vals"][::-1])
+    _check(back, _call(back))
