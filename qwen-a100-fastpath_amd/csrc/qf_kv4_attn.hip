@@ -12,7 +12,7 @@
 //                        join, 3.5 TB/s; a wavefront's own step of 2000 cycles is what keeps it from more), by the chain lengths,
 //                        block ids, codes, states, partial results where it is short (1000 positions: 5.4 us and 4.3 us)
 //   attn_tile_kernel     many rows (prompt chunks): each wavefront its own rows, all of a workgroup the same positions.  Bound by
-//                        the matrix cores at D = 128 (2048 tokens behind 8192 positions, 64 heads over 8: 559 us, 1.11 PFLOP/s),
+//                        the matrix cores at D = 128 (2048 tokens behind 8192 positions, 64 heads over 8: 514 us, 1.21 PFLOP/s),
 //                        by LDS reads at D = 256 (16 rows a wavefront)
 #include "qf_kv4_common.h"
 
@@ -705,8 +705,9 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void attn_split_kernel(AttnArg
 
 // Many rows: 8 wavefronts with 16 kRT rows each walk over the same positions, 64 a stage.  A stage's keys and values are widened
 // once for all of them, an eighth a wavefront, into LDS, in the order of the operands (8 KiB of fragments a wavefront and step of
-// either, at D = 128): two buffers, one barrier a stage.  (2048 tokens behind 8192 positions, 64 heads over 8: 559 us; keys widened
-// by each wavefront for itself 681; 4 wavefronts of 64 rows, whose accumulators move between register files, 928.)
+// either, at D = 128): two buffers, one barrier a stage.  (2048 tokens behind 8192 positions, 64 heads over 8, before
+// attn_tile_kernel's order of workgroups: 555 us; keys widened by each wavefront for itself 681; 4 wavefronts of 64 rows, whose
+// accumulators move between register files, 928.)
 template <int D>
 struct TileShape {
   static constexpr int kRT = D == 256 ? 1 : 2;
