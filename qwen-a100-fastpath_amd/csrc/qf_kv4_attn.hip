@@ -46,9 +46,7 @@ struct AttnArgs {
   float* o_part;   // [HKV][slots][rows][D]
   float2* ml_part; // [HKV][slots][rows]: exponent reference, sum
   int2* plan;      // [B]: first slot and slots of a request
-  int fast;  // tile kernel: workgroups that stand together, the heads of a row tile or the row tiles of a head
-  Divisor by_fast;
-  int row_tiles, tile_splits;  // tile kernel: of a request at most, and of a row tile at most; partials [B][HKV][row tile][split]
+  int cus;  // compute units
   int slots;
 };
 
@@ -718,31 +716,77 @@ struct TileShape {
 };
 constexpr int kStage = 64;
 
-// The stages of a row tile that sees the positions below `end`, over at most a.tile_splits workgroups of 4 stages or more.
-__device__ __forceinline__ void stage_splits(const AttnArgs& a, int end, int& splits, int& per) {
+// The stages of a row tile that sees the positions below `end`, over at most `most` workgroups of 4 stages or more.
+__device__ __forceinline__ void stage_splits(int end, int most, int& splits, int& per) {
   const int n = max((end + kStage - 1) / kStage, 1);
-  splits = min(a.tile_splits, max(n / 4, 1));
+  splits = min(most, max(n / 4, 1));
   per = (n + splits - 1) / splits;
   splits = (n + per - 1) / per;
 }
-__device__ __forceinline__ int64_t tile_slot(const AttnArgs& a, int b, int hkv, int row_tile) {
-  return (((int64_t)b * a.HKV + hkv) * a.row_tiles + row_tile) * a.tile_splits;
-}
 
-// The request that stands at `place` by its positions, the longest first (those of the split kernel last): of up to 64 requests, a
-// lane each.  (Chunks of up to 700 tokens, the longest given last: 13 requests 164 -> 151 us, D = 256, 15 requests 185 -> 169;
-// given first 151 -> 149 and 171 -> 169.)
-__device__ __forceinline__ int by_length(const AttnArgs& a, int place) {
-  const int lane = threadIdx.x % kWave;
-  const Request r = request(a, min(lane, a.B - 1));
-  const int key = r.n * a.G > a.few ? r.seq : -1;
-  int rank = 0;
-  for (int j = 0; j < a.B; ++j) {
-    const int other = __builtin_amdgcn_readlane(key, j);
-    rank += other > key || (other == key && j < lane);
+// The row tiles that a batch holds, of the requests that are not the split kernel's, in an order: request by request, the longest
+// first where there are up to 64 (a lane each), each one's last tile, which sees most, first.  Every workgroup finds it out for
+// itself from the lengths, so that the launch is as large as the batch at most and nothing is read back.
+// (Chunks of up to 700 tokens, the longest given last: 13 requests 164 -> 151 us, D = 256, 15 requests 185 -> 169.  Splits by what
+// the batch holds instead of what it could hold: 7 chunks of up to 24 tokens behind up to 5800 positions, 48 heads of 256 over
+// 8: 118 -> 67 us; 9 of up to 165 behind 9000, 20 of 64 over 4: 110 -> 70; 40 chunks that fill the machine 146 -> 152.)
+constexpr int kMostSplits = 16;
+template <int ROWS>
+struct Batch {
+  static constexpr int kCap = 1 << 30;  // 64 requests more of at most 2^24 tiles each stay below 2^31
+  const AttnArgs& a;
+  int lane, mine, before, total;
+
+  __device__ __forceinline__ int tiles_of(const Request& r) const {
+    const int rows = r.n * a.G;
+    return rows > a.few ? (rows + ROWS - 1) / ROWS : 0;
   }
-  return __builtin_ctzll(__ballot(rank == place && lane < a.B));
-}
+  __device__ __forceinline__ int tiles_of(int b) const { return b < a.B ? tiles_of(request(a, b)) : 0; }
+
+  __device__ __forceinline__ explicit Batch(const AttnArgs& args) : a(args) {
+    lane = threadIdx.x % kWave;
+    total = before = mine = 0;
+    if (a.B <= kWave) {
+      const Request r = request(a, min(lane, a.B - 1));
+      mine = lane < a.B ? tiles_of(r) : 0;
+      for (int j = 0; j < a.B; ++j) {
+        const int tiles = __builtin_amdgcn_readlane(mine, j), seq = __builtin_amdgcn_readlane(r.seq, j);
+        if (seq > r.seq || (seq == r.seq && j < lane)) before += tiles;
+        total += tiles;
+      }
+    } else {
+      for (int base = 0; base < a.B; base += kWave)
+        total = min(total + __builtin_amdgcn_readlane(wave_scan(tiles_of(base + lane)), kWave - 1), kCap);
+    }
+  }
+
+  // Workgroups that share the positions of a row tile: several where the batch's tiles leave compute units idle.  There are at
+  // most a.cus partial results then.
+  __device__ __forceinline__ int splits() const {
+    const int64_t groups = (int64_t)total * a.HKV;
+    return groups > a.cus ? 1 : min(a.cus / max((int)groups, 1), kMostSplits);
+  }
+
+  // Tile t of the order: its request and its place among the request's; false where the batch has fewer.
+  __device__ __forceinline__ bool find(int t, int& b, int& row_tile) const {
+    int n = mine, first = before;
+    for (int base = 0, done = 0;; base += kWave) {
+      if (a.B > kWave) {
+        n = tiles_of(base + lane);
+        first = done + wave_scan(n) - n;
+        done = min(__builtin_amdgcn_readlane(first + n, kWave - 1), kCap);
+      }
+      const uint64_t here = __ballot(t >= first && t < first + n);
+      if (here != 0) {
+        const int i = __builtin_ctzll(here);
+        b = base + i;
+        row_tile = __builtin_amdgcn_readlane(n, i) - 1 - (t - __builtin_amdgcn_readlane(first, i));
+        return true;
+      }
+      if (base + kWave >= a.B) return false;
+    }
+  }
+};
 
 template <int D>
 __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel(AttnArgs a) {
@@ -752,14 +796,27 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ uint32_t odd[2][S::kWaves];  // a wavefront met a block of NaN that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int b = a.B > 1 && a.B <= kWave ? by_length(a, blockIdx.z) : blockIdx.z;
-  const int quotient = divide(blockIdx.x, a.by_fast), rest = blockIdx.x - quotient * a.fast;
-  const int x = a.tile_splits == 1 ? quotient : rest, hkv = a.tile_splits == 1 ? rest : quotient;
+  // The heads of a row tile stand together: those that see most come first over all heads, and where the heads are a multiple of
+  // 8 an XCD's L2 holds its own heads' positions (4096 tokens of 32 heads over 8 from the start 234 -> 137 us; 2048 of 64 over 8
+  // behind 8192 positions 556 -> 514; D = 256 341 -> 300).  With positions split a head's workgroups do (34.7 us, 37.6).
+  const Batch<S::kRows> batch(a);
+  const int most = batch.splits(), x = blockIdx.x;
+  int t, hkv, split = 0;
+  if (most == 1) {
+    t = x / a.HKV;
+    hkv = x - t * a.HKV;
+  } else {
+    if (batch.total == 0) return;
+    hkv = x / (batch.total * most);
+    if (hkv >= a.HKV) return;
+    t = (x - hkv * batch.total * most) / most;
+    split = (x - hkv * batch.total * most) % most;
+  }
+  int b, row_tile;
+  if (!batch.find(t, b, row_tile)) return;
   const Request r = request(a, b);
   const int rows = r.n * a.G;
-  const int row_tile = a.row_tiles - 1 - x / a.tile_splits;  // the rows that see most come first
   const int row0 = row_tile * S::kRows;
-  if (row0 >= rows || rows <= a.few) return;
   const int r0 = row0 + wave * 16 * S::kRT;
   W w(a);
   w.start(r, b, hkv, r0);
@@ -767,8 +824,7 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   const int own_end = r0 < rows ? seen(r0 + 16 * S::kRT - 1) : 0;  // positions that a row of this wavefront sees
   const int end = seen(row0 + S::kRows - 1), all_see = seen(row0);
   int splits, per;
-  stage_splits(a, end, splits, per);
-  const int split = x % a.tile_splits;
+  stage_splits(end, most, splits, per);
   if (split >= splits) return;
   const int first_stage = split * per, n_stages = min((end + kStage - 1) / kStage, first_stage + per);
   const int last_tile = (end - 1) / kTile * kTile;
@@ -935,7 +991,7 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
       w.write(r, hkv, row, rt);
       continue;
     }
-    const int64_t slot = tile_slot(a, b, hkv, row_tile) + split;
+    const int64_t slot = ((int64_t)t * a.HKV + hkv) * most + split;
     const int at = wave * S::kRT + rt;
 #pragma unroll
     for (int u = 0; u < W::kDTiles; ++u)
@@ -947,44 +1003,20 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
 // A workgroup a slice (SLICES of them, 2 or 4) of a pair of tiles (values n and n + 1 of each lane's run): the splits are shared by
 // its wavefronts, and by halves of a wavefront where SLICES is 4, 4 requested by each at once (they come from other XCDs'
 // writes, a microsecond away); then the shares through LDS.
-// TILED: of the tile kernel's splits, else of the split kernel's.
-template <int D, bool TILED, int SLICES, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave) void attn_combine_kernel(AttnArgs a) {
+template <int D, int SLICES, int WAVES>
+__device__ __forceinline__ void combine(const AttnArgs& a, const Request& r, int hkv, int row0, int pair, int slice, int64_t slot,
+                                        int splits, int tiles, int slot_rows) {
   using W = Walk<D, 1>;
-  constexpr int kPairs = TileShape<D>::kRows / 16 * W::kDTiles / 2;  // of a row tile (TILED)
-  constexpr int kSlice = kWave / SLICES;                             // lanes of a tile
+  constexpr int kSlice = kWave / SLICES;  // lanes of a tile
   constexpr int kGroups = WAVES * SLICES / 2;
   __shared__ float2 sm_ml[kGroups][kSlice];
   __shared__ __align__(16) f32x4_t sm_o[kGroups][2][kSlice];
-  const int hkv = blockIdx.y, b = blockIdx.z;
-  const int slice = blockIdx.x % SLICES, x = blockIdx.x / SLICES;
-  const int pair = TILED ? x % kPairs : x, row_tile = TILED ? x / kPairs : 0;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int at = lane % kSlice, odd = lane / kSlice % 2, g = wave * (SLICES / 2) + lane / (2 * kSlice);
   const int tile_lane = slice * kSlice + at, tile = 2 * pair + odd;
   const int l16 = tile_lane % 16, qg = tile_lane / 16, part_row = tile / W::kDTiles * 16 + l16;
-  const int row = row_tile * TileShape<D>::kRows + part_row;
-  const Request r = request(a, b);
-  const int rows = r.n * a.G;
+  const int row = row0 + part_row, rows = r.n * a.G;
   if (row - l16 >= rows) return;
-  int splits, tiles, slot_rows;
-  int64_t slot;
-  if constexpr (TILED) {
-    if (rows <= a.few) return;
-    int per;
-    const int last_row = min((row_tile + 1) * TileShape<D>::kRows, rows) - 1;
-    stage_splits(a, max(r.seq - r.n + divide(last_row, a.by_g) + 1, 0), splits, per);
-    slot = tile_slot(a, b, hkv, row_tile);
-    tiles = 2 * kPairs;
-    slot_rows = TileShape<D>::kRows;
-  } else {
-    const int2 place = a.plan[b];
-    splits = place.y;
-    slot = (int64_t)hkv * a.slots + place.x;
-    tiles = gridDim.x / SLICES * 2;
-    slot_rows = a.rows;
-  }
-  if (splits < 2) return;
   float m = -__builtin_inff(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   if (row < rows) {
@@ -1043,6 +1075,39 @@ __global__ __launch_bounds__(WAVES * kWave) void attn_combine_kernel(AttnArgs a)
   for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(to + Rec::kWidth * i) = pack_bf16(evens[i] * inv, odds[i] * inv);
 }
 
+template <int D, int SLICES, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void attn_combine_kernel(AttnArgs a) {
+  const int hkv = blockIdx.y, b = blockIdx.z;
+  const int2 place = a.plan[b];
+  if (place.y < 2) return;
+  combine<D, SLICES, WAVES>(a, request(a, b), hkv, 0, blockIdx.x / SLICES, blockIdx.x % SLICES, (int64_t)hkv * a.slots + place.x,
+                            place.y, gridDim.x / SLICES * 2, a.rows);
+}
+
+// Of the tile kernel's splits: workgroups over the slices of all row tiles that have several.
+// (With cu_q so many whatever the batch holds: 40 chunks that split nothing 153 us, 156 with 2048; 7 that split 67 and 66.)
+constexpr int kTileCombine = 1024;
+template <int D>
+__global__ __launch_bounds__(4 * kWave) void attn_tile_combine_kernel(AttnArgs a) {
+  using S = TileShape<D>;
+  constexpr int kSlices = 2, kPairs = S::kRows / 16 * (D / 16) / 2;
+  const Batch<S::kRows> batch(a);
+  const int most = batch.splits();
+  if (most < 2) return;
+  for (int u = blockIdx.x; u < batch.total * a.HKV * (kPairs * kSlices); u += gridDim.x) {
+    const int unit = u / (kPairs * kSlices), part = u % (kPairs * kSlices), t = unit / a.HKV;
+    int b, row_tile, splits, per;
+    if (!batch.find(t, b, row_tile)) continue;
+    const Request r = request(a, b);
+    const int last_row = min((row_tile + 1) * S::kRows, r.n * a.G) - 1;
+    stage_splits(max(r.seq - r.n + divide(last_row, a.by_g) + 1, 0), most, splits, per);
+    if (splits < 2) continue;
+    combine<D, kSlices, 4>(a, r, unit - t * a.HKV, row_tile * S::kRows, part / kSlices, part % kSlices, (int64_t)unit * most, splits,
+                           2 * kPairs, S::kRows);
+    __syncthreads();  // what it left in LDS has been read
+  }
+}
+
 typedef void (*AttnFn)(AttnArgs);
 
 struct Split {
@@ -1065,11 +1130,11 @@ struct Combine {
   AttnFn fn;
   int slices, threads;
 };
-template <bool TILED, int SLICES, int WAVES>
+template <int SLICES, int WAVES>
 Combine combine_of(int D) {
-  return {D == 64    ? &attn_combine_kernel<64, TILED, SLICES, WAVES>
-          : D == 128 ? &attn_combine_kernel<128, TILED, SLICES, WAVES>
-                     : &attn_combine_kernel<256, TILED, SLICES, WAVES>,
+  return {D == 64    ? &attn_combine_kernel<64, SLICES, WAVES>
+          : D == 128 ? &attn_combine_kernel<128, SLICES, WAVES>
+                     : &attn_combine_kernel<256, SLICES, WAVES>,
           SLICES, WAVES * kWave};
 }
 
@@ -1077,12 +1142,14 @@ Combine combine_of(int D) {
 struct Plan {
   bool tiles, split;  // the tile kernel; the split kernel with the combination
   int workers, slots, rows;         // split kernel
-  int row_tiles, tile_splits;       // tile kernel
+  int row_tiles;                    // tile kernel: of a request at most
+  int64_t tile_groups;              // its workgroups
+  bool cut;                         // it may split positions
+  int combine_groups;               // whose results are added by as many
   size_t o, ml, plan, tile_o, tile_ml, bytes;  // offsets and size of the workspace
 };
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-constexpr size_t kTilePartials = (size_t)128 << 20;  // most bytes of the tile kernel's partial results
 int tile_rows(int D) { return D == 256 ? TileShape<256>::kRows : D == 128 ? TileShape<128>::kRows : TileShape<64>::kRows; }
 
 // Requests of up to QF_KV4_MAX_ROWS packed rows are split over positions, larger ones tiled over rows; a batch with lengths of its
@@ -1096,22 +1163,20 @@ Plan plan_of(const qf_kv4_attention_args& u) {
   if (p.tiles) {
     const int per = tile_rows(u.head_size);
     p.row_tiles = (int)((rows + per - 1) / per);
-    // Positions are split where the row tiles leave compute units idle (100 tokens behind 4000 positions, 64 heads over 8: 115 -> 34
-    // us; twice as many splits 47).
+    // The row tiles of the batch: as many as all requests could have, or with cu_q as the tokens fill, each request's last one being
+    // short.  Positions are split where the tiles that the requests turn out to have leave compute units idle (100 tokens behind
+    // 4000 positions, 64 heads over 8: 115 -> 34 us): without cu_q that is known here.
     const int64_t all = (int64_t)p.row_tiles * u.num_reqs;
     const int64_t by_tokens = ((int64_t)u.num_tokens * (u.num_heads / u.num_kv_heads) + per - 1) / per + u.num_reqs;
-    const int64_t groups = (all < by_tokens ? all : by_tokens) * u.num_kv_heads;
-    int64_t splits = compute_units() / groups;
-    splits = splits < 1 ? 1 : splits > 16 ? 16 : splits;
-    const size_t slot = (size_t)per * u.head_size * sizeof(float);
-    while (splits > 1 && (size_t)all * u.num_kv_heads * splits * slot > kTilePartials) --splits;
-    p.tile_splits = (int)splits;
-    if (splits > 1) {
-      const size_t slots = (size_t)all * u.num_kv_heads * splits;
+    p.tile_groups = (u.cu_q && by_tokens < all ? by_tokens : all) * u.num_kv_heads;
+    p.cut = u.cu_q || compute_units() / p.tile_groups >= 2;
+    if (p.cut) {
+      p.combine_groups = u.cu_q ? kTileCombine : (int)p.tile_groups * (per / 16) * (u.head_size / 16);
+      p.tile_groups = std::max<int64_t>(p.tile_groups, compute_units());
       p.tile_o = n;
-      n += slots * slot;
+      n += (size_t)compute_units() * per * u.head_size * sizeof(float);
       p.tile_ml = n;
-      n += round256(slots * per * sizeof(float2));
+      n += round256((size_t)compute_units() * per * sizeof(float2));
     }
   }
   if (!p.split) {
@@ -1215,28 +1280,21 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   a.by_workers = divisor(p.split ? p.workers : 1);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int D = u.head_size, di = D == 64 ? 0 : D == 128 ? 1 : 2;
-  a.row_tiles = p.row_tiles;
-  a.tile_splits = p.tile_splits;
+  a.cus = compute_units();
   if (p.tiles) {
     a.o_part = reinterpret_cast<float*>(ws + p.tile_o);
     a.ml_part = reinterpret_cast<float2*>(ws + p.tile_ml);
     static_assert(TileShape<64>::kWaves == TileShape<128>::kWaves && TileShape<256>::kWaves == TileShape<128>::kWaves, "one shape");
     const AttnFn fn = D == 64 ? &attn_tile_kernel<64> : D == 128 ? &attn_tile_kernel<128> : &attn_tile_kernel<256>;
     const int lds = D == 64 ? TileShape<64>::kLds : D == 128 ? TileShape<128>::kLds : TileShape<256>::kLds;
-    const int64_t groups = (int64_t)p.row_tiles * p.tile_splits * a.HKV;
-    if (!grid_fits(groups, TileShape<128>::kWaves * kWave)) return QF_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)groups, 1, a.B);
-    // The heads of a row tile together: those that see most come first over all heads, and where the heads are a multiple of 8
-    // an XCD's L2 holds its own heads' positions (4096 tokens of 32 heads over 8 from the start 234 -> 137 us; 2048 of 64 over 8 behind
-    // 8192 positions 556 -> 510; D = 256 341 -> 300).  With positions split a head's workgroups together (34.7 us, 37.6).
-    a.fast = p.tile_splits == 1 ? a.HKV : p.row_tiles * p.tile_splits;
-    a.by_fast = divisor(a.fast);
-    int st = launch(fn, grid, TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
+    if (!grid_fits(p.tile_groups, TileShape<128>::kWaves * kWave)) return QF_ERR_UNSUPPORTED;
+    int st = launch(fn, dim3((unsigned)p.tile_groups), TileShape<128>::kWaves * kWave, lds, g_raised[di][3], s, a);
     if (st != QF_OK) return st;
-    if (p.tile_splits > 1) {
-      const Combine c = combine_of<true, 2, 4>(D);
-      const int parts = tile_rows(D) / 16 * (D / 32) * c.slices;  // of a row tile
-      st = launch(c.fn, dim3((unsigned)(p.row_tiles * parts), a.HKV, a.B), c.threads, 0, g_raised[di][0], s, a);
+    if (p.cut) {
+      const AttnFn comb = D == 64    ? &attn_tile_combine_kernel<64>
+                          : D == 128 ? &attn_tile_combine_kernel<128>
+                                     : &attn_tile_combine_kernel<256>;
+      st = launch(comb, dim3(p.combine_groups), 4 * kWave, 0, g_raised[di][0], s, a);
       if (st != QF_OK) return st;
     }
     if (!p.split) return QF_OK;
@@ -1248,7 +1306,7 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   const int64_t pairs = (int64_t)k.row_tiles * (D / 32) * a.HKV * a.B;
   // Small slices where that gives a compute unit a few workgroups at most (3 queries behind 38 000 positions, 64 splits of 18 rows of
   // 256: 26.4 -> 23.1 us with the splits themselves, 7 requests of 4 queries 12.6 -> 10.8; 16 requests of up to 3000 18.5, 18.7).
-  const Combine c = 4 * pairs <= 4 * compute_units() ? combine_of<false, 4, 8>(D) : combine_of<false, 2, 4>(D);
+  const Combine c = 4 * pairs <= 4 * compute_units() ? combine_of<4, 8>(D) : combine_of<2, 4>(D);
   // Where a workgroup a compute unit is all there is, none takes two of them: each asks for more than half of the LDS (100 000
   // positions 35.7 -> 30.8 us, 30 000 17.0 -> 15.5, D = 256 19.6 -> 16.5; at 1000 8.6 -> 8.9, so not for tables that end there).
   const bool alone = (int64_t)p.slots * a.HKV <= compute_units() * 5 / 4 && (int64_t)a.max_blocks * a.page >= kManyPositions;
