@@ -714,7 +714,6 @@ struct TileShape {
   static constexpr int kFragments = 4 * (D / 32) + 2 * (D / 16);  // KiB of a stage: 4 records' keys, 2 steps' values
   static constexpr int kLds = 2 * kFragments * 1024;
 };
-constexpr int kStage = 64;
 
 // The stages of a row tile that sees the positions below `end`, over at most `most` workgroups of 4 stages or more.
 __device__ __forceinline__ void stage_splits(int end, int most, int& splits, int& per) {
@@ -836,7 +835,7 @@ __global__ __launch_bounds__(TileShape<D>::kWaves * kWave) void attn_tile_kernel
   // The records of 16 stages are looked up at once, a record a lane.
   uint32_t rec_lo = 0, rec_hi = 0;
   auto look_up = [&](int stage) {
-    const int64_t at = w.record(min(stage * kStage + w.lane * kTile, last_tile));
+    const int64_t at = w.record(stage_record(stage, w.lane, last_tile));
     rec_lo = (uint32_t)at;
     rec_hi = (uint32_t)(at >> 32);
   };

@@ -4,6 +4,7 @@
 
 #include "qf_block_common.h"
 #include "qf_kv4.h"
+#include "qf_kv4_places.h"
 
 #include <algorithm>
 #include <atomic>
@@ -12,7 +13,6 @@ namespace qfk {
 
 using namespace qfb;
 
-constexpr int kTile = QF_KV4_TILE;
 constexpr int kGroup = 32;  // values that share a scale
 
 // Division of 0 <= n < 2^31 by an invariant d >= 1 (Granlund and Montgomery, PLDI 1994): with l = ceil(log2 d) and
