@@ -21,7 +21,6 @@
 
 namespace qfk {
 
-constexpr int kStep = 2 * kTile;  // positions of a step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMinChunk = 4 * kStep;
 
@@ -569,8 +568,8 @@ __device__ __forceinline__ bool place_of(const AttnArgs& a, int slot, Place& p) 
     } else {
       total = (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)sum), kWave - 1);  // at most 64 * 2^26
     }
-    most = total < 0x80000000u ? (uint32_t)divide((int)total, a.by_workers) + 1 : (uint32_t)(total / (uint32_t)a.workers) + 1;
-    most = min(max(most, (uint32_t)(kMinChunk / kStep)), 1u << 26);
+    most = total < 0x80000000u ? (uint32_t)divide((int)total, a.by_workers) + 1 : chunk_steps(total, (uint32_t)a.workers);
+    most = min(max(most, (uint32_t)(kMinChunk / kStep)), kMostSteps);
   }
   p.chunk = (int)min(most * kStep, 0x7fffffe0u);
   int before = 0;

@@ -46,3 +46,24 @@ def _run(tmp_path, body):
 
 def test_a_stage_ahead_of_the_last_is_looked_up_inside_the_sequence(tmp_path):
     assert _run(tmp_path, _STAGES) == ""
+
+
+_CHUNKS = """
+// A batch of so many requests of `steps` each: the chunks that they are cut to, which have workers + requests places.
+int main() {
+  const long most = 1l << 26;
+  for (long requests : {1l, 65l, 129l, 4096l, 65535l})
+    for (long workers : {1l, 2l, 32l, 256l, 768l})
+      for (long steps : {1l, 3l, 1000l, most / 2, most - 2}) {
+        const long chunk = qfk::chunk_steps((uint64_t)(requests * steps), (uint32_t)workers);
+        const long chunks = requests * ((steps + chunk - 1) / chunk);
+        if (chunk < 1 || chunk > most || chunks > workers + requests)
+          printf("%ld requests of %ld steps over %ld: %ld chunks of %ld\\n", requests, steps, workers, chunks, chunk);
+      }
+  return 0;
+}
+"""
+
+
+def test_a_batch_has_no_more_chunks_than_places(tmp_path):
+    assert _run(tmp_path, _CHUNKS) == ""
