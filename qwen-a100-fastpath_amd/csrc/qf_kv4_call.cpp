@@ -20,6 +20,7 @@
 namespace {
 
 constexpr int64_t kIntMax = 0x7fffffff;
+constexpr int64_t kFar = 0x7fffffffffffffff;  // past any stride
 
 bool unpack(PyObject* o, int64_t device, const at::Tensor** t) {
   if (!THPVariable_CheckExact(o)) return false;
@@ -43,7 +44,7 @@ bool heads(const at::Tensor& t, int64_t T, int64_t H, int64_t D, qf_heads* out) 
 }
 // A tensor that is written: no two of its heads may share memory.
 bool separate(const qf_heads& h, int64_t T, int64_t H, int64_t D) {
-  const int64_t t = T > 1 ? h.stride_tok : kIntMax, n = H > 1 ? h.stride_head : kIntMax;
+  const int64_t t = T > 1 ? h.stride_tok : kFar, n = H > 1 ? h.stride_head : kFar;
   return n <= t ? n >= D && (T == 1 || t >= (H == 1 ? D : (H - 1) * n + D)) : t >= D && n >= (T - 1) * t + D;
 }
 bool pages(const at::Tensor& t, int64_t H, int64_t D, qf_pages* out) {
