@@ -16,8 +16,8 @@
 //                        by LDS reads at D = 256 (16 rows a wavefront)
 #include "qf_kv4_common.h"
 
-#include <float.h>
 #include <math.h>
+#include <string.h>
 
 namespace qfk {
 
@@ -1210,6 +1210,18 @@ bool sizes_fit(const qf_kv4_attention_args& u) {
 
 constexpr int kAloneLds = 82 * 1024;  // of 160 KiB
 constexpr int kManyPositions = 4096;
+
+// |scale| log2 e.  A masked score is -inf, which 0 would make no number: then 2^-149, the least number there is (the kernels keep such
+// numbers), which moves no score of fp32 by more than 2^-21.  By its bits: a host thread may flush it to 0.
+float base2_scale(float scale) {
+  const float s = fabsf(scale) * kLog2e;
+  uint32_t bits;
+  memcpy(&bits, &s, sizeof bits);
+  bits = std::max(bits, 1u);
+  float out;
+  memcpy(&out, &bits, sizeof out);
+  return out;
+}
 std::atomic<uint64_t> g_raised[3][5];
 
 int launch(AttnFn fn, dim3 grid, int threads, size_t lds, std::atomic<uint64_t>& raised, hipStream_t s, const AttnArgs& a) {
@@ -1271,7 +1283,7 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   a.few = p.split ? p.rows : 0;
   a.workers = p.workers;
   a.slots = p.slots;
-  a.qk_scale = fmaxf(fabsf(u.scale) * kLog2e, FLT_MIN);  // not 0: a masked score is -inf
+  a.qk_scale = base2_scale(u.scale);
   a.flip = u.scale < 0 ? 0x80008000u : 0;
   a.by_g = divisor(a.G);
   a.by_page = divisor(u.page_size);
