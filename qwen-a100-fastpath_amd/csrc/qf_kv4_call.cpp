@@ -15,6 +15,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+
 #include "qf_kv4.h"
 
 namespace {
@@ -52,6 +54,15 @@ bool pages(const at::Tensor& t, int64_t H, int64_t D, qf_pages* out) {
       t.stride(3) != 1)
     return false;
   *out = {static_cast<uint16_t*>(t.data_ptr()), t.stride(0), t.stride(1), t.stride(2)};
+  // they are written: no two heads may share memory, in whichever order the dimensions stand
+  int order[] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return t.stride(a) < t.stride(b); });
+  int64_t room = D;
+  for (int i : order) {
+    if (t.size(i) == 1) continue;
+    if (t.stride(i) < room) return false;
+    room += (t.size(i) - 1) * t.stride(i);
+  }
   return aligned(out->data) && out->stride_block >= 0 && out->stride_tok >= 0 && out->stride_head >= 0 &&
          out->stride_block % 8 == 0 && out->stride_tok % 8 == 0 && out->stride_head % 8 == 0;
 }

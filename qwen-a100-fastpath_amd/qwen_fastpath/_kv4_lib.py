@@ -171,13 +171,13 @@ def output(t: torch.Tensor | None, shape: tuple, name: str) -> torch.Tensor | No
     """A tensor that is written: no copy can stand for it."""
     if t is None:
         return None
-    if t.dtype is not torch.bfloat16 or tuple(t.shape) != shape or not _fit(t) or _overlaps(t):
+    if t.dtype is not torch.bfloat16 or tuple(t.shape) != shape or not _fit(t) or overlaps(t):
         raise ValueError(f"{name} must be bf16 {list(shape)} with 16-byte aligned heads that do not overlap, the last dimension "
                          f"contiguous and strides of multiples of 8, got {t.dtype} {list(t.shape)} with strides {t.stride()}")
     return plain(t)
 
 
-def _overlaps(t: torch.Tensor) -> bool:
+def overlaps(t: torch.Tensor) -> bool:
     room = 1
     for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if s < room:

@@ -100,6 +100,8 @@ def _run(query, key, positions, cos_sin, q_weight, k_weight, value, cache, slots
                 if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
                     raise ValueError(f"{n} must be 16-byte aligned, its last dimension contiguous and its strides multiples of 8, got "
                                      f"{t.stride()}")
+                if K.overlaps(t):
+                    raise ValueError(f"{n} is written, its heads must not share memory, got strides {t.stride()}")
             cache = tuple(K.plain(t) for t in pages)
     if T == 0:
         return (query_out if query is None or query_out is not None else torch.empty_like(query),
