@@ -128,3 +128,24 @@ def test_a_grid_past_32_bits_is_refused():
     for call, (rc, _, made) in zip(*(lambda c: (c, _record(c)))([
             ("attention", 1, 1 << 27, 512, 64, 128, 0, 8), ("rope", 1 << 30, 64, 8, 128, 0, 0, 2), ("load", 1 << 30, 1, 256)])):
         assert rc == 2 and not made, (call, rc, made)
+
+
+def test_workspaces_hold_what_the_launches_write():
+    """The partial results that the launched grids have places for, in the bytes that the call asks for: a tile of fp32 sums with a
+    maximum and a sum a row for each workgroup of the split kernel, and for each compute unit where row tiles may be split."""
+    cus, seen = 256, set()  # what the library takes without a device
+    calls = [c for c in _calls() if c[0] == "attention"]
+    for call, (_, given, made) in zip(calls, _record(calls)):
+        _, B, q, heads, kv, D, _, _ = call
+        need, kinds = 0, tuple(re.search(r"attn_\w+?_kernel", m[0]).group(0) for m in made)
+        for symbol, grid, *_ in made:
+            if "attn_split_kernel" in symbol:
+                _, rt, rg = map(int, re.search(r"attn_split_kernelILi(\d+)ELi(\d+)ELi(\d+)E", symbol).groups())
+                assert 16 * rt * rg >= min(q * heads // kv, 64) and grid[1] == kv, call
+                need += grid[0] * kv * (16 * rt * rg * D * 4 + min(q * heads // kv, 64) * 8) + B * 8
+            if "attn_tile_combine_kernel" in symbol:
+                need += cus * (128 if D == 256 else 256) * (4 * D + 8)
+        assert given >= need, (call, kinds, given, need)
+        assert (given == 0) == (need == 0), (call, kinds)
+        seen.add(kinds)
+    assert len(seen) == 4, seen  # few rows; tiles; tiles that may be split; tiles beside few rows
