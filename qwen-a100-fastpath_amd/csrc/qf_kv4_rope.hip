@@ -12,7 +12,8 @@
 //
 // Memory bounds it where there are many rows (2048 tokens of 64 + 8 heads of 128 into 4 bits: 80 MB in 19 us, 4.2 TB/s; 8191 of 16 + 2
 // into bf16 pages: 86 MB in 16.8 us, 5.1 TB/s, part of it in the caches), the chain position, angles, stores where there are few
-// (5 tokens 3.7 us).  The fp64 rows of keys are a few in a hundred and cost no registers: 78 a lane, 6 wavefronts a SIMD.
+// (5 tokens 3.7 us).  The fp64 rows of keys are one in eight to ten (64 + 8 + 8 heads: 10%, 24 + 4 + 4: 12%) and cost no registers: 78
+// a lane, 6 wavefronts a SIMD.
 #include "qf_kv4_common.h"
 
 namespace qfk {
