@@ -12,8 +12,11 @@
 //                        join, 3.5 TB/s; a wavefront's own step of 2000 cycles is what keeps it from more), by the chain lengths,
 //                        block ids, codes, states, partial results where it is short (1000 positions: 5.4 us and 4.3 us)
 //   attn_tile_kernel     many rows (prompt chunks): each wavefront its own rows, all of a workgroup the same positions.  Bound by
-//                        the matrix cores at D = 128 (2048 tokens behind 8192 positions, 64 heads over 8: 514 us, 1.21 PFLOP/s),
-//                        by LDS reads at D = 256 (16 rows a wavefront)
+//                        the matrix cores at D = 128 (2048 tokens behind 8192 positions, 64 heads over 8: 514 us, 1.21 PFLOP/s).
+//                        At D = 256 (16 rows a wavefront: twice the operand reads a product) by no unit alone: with row tiles that
+//                        fill the machine twice LDS is busy 55% of the time and the matrix cores 40%, the chain product, softmax,
+//                        product behind a barrier a stage has two wavefronts a SIMD to hide it; in a ragged batch by its longest
+//                        request, whose row tiles come last to an end
 #include "qf_kv4_common.h"
 
 #include <math.h>
