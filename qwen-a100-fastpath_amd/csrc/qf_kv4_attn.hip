@@ -1190,6 +1190,9 @@ Plan plan_of(const qf_kv4_attention_args& u) {
   // three; 16 requests, which do not fill it, 18.6 with one, 22.9 with two.  Not where the registers of a workgroup (over 180 a
   // lane) leave no room for three (40 requests of 32 rows 29.8, 32.9, 33.0; D = 256, 70 requests of 30 rows 39.9, 46.4, 55.1), nor
   // where each workgroup's look at all requests counts (260 over one kv head 16.3, 17.6, 18.9; 400 over 8 heads 56, 58, 60).
+  // About 128 requests neither is the better one throughout (three, one; 64 heads of 128 over 8): of up to 2000 positions 64 requests
+  // 26.9 and 23.9, 96 34.2 and 37.3, 128 44.8 and 39.6, 160 51.3 and 51.5, 260 71.7 and 70.3; of up to 9000 128 149.5 and 144.1, 160
+  // 169 and 179; 32 heads of 64 over 4, of up to 4000, 128 22.4 and 32.6, 160 30.2 and 38.1.
   const int row_tiles = split_of(u.head_size, p.rows).row_tiles;
   const bool full = (int64_t)u.num_reqs * u.num_kv_heads >= compute_units();
   const int cus = compute_units() * (full && std::min(row_tiles, 2) * u.head_size <= 128 && u.num_reqs <= 128 ? 3 : 1);
@@ -1322,6 +1325,8 @@ extern "C" int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspa
   const Combine c = 4 * pairs <= 4 * compute_units() ? combine_of<4, 8>(D) : combine_of<2, 4>(D);
   // Where a workgroup a compute unit is all there is, none takes two of them: each asks for more than half of the LDS (100 000
   // positions 35.7 -> 30.8 us, 30 000 17.0 -> 15.5, D = 256 19.6 -> 16.5; at 1000 8.6 -> 8.9, so not for tables that end there).
+  // The lengths are on the device, the table's width stands for them: a short request behind a server's wide table pays for it
+  // (64 heads of 128 over 8 behind 2560 pages of 16: 1000 positions 8.4 -> 8.7 us, 2000 8.4 -> 8.8, 4000 9.4 -> 9.5, 100 and 300 level).
   const bool alone = (int64_t)p.slots * a.HKV <= compute_units() * 5 / 4 && (int64_t)a.max_blocks * a.page >= kManyPositions;
   const int lds = alone ? std::max(k.lds, kAloneLds) : k.lds;
   const int st = launch(k.fn, dim3(p.slots, a.HKV), k.threads, lds, g_raised[di][k.row_tiles], s, a);
