@@ -45,6 +45,8 @@ extern "C" {
 #define QF_STEP_MAX_REQS 4096
 /* Most tokens and pages of qf_step_tables. */
 #define QF_STEP_MAX_TOKENS (1 << 29)
+/* Most requests, and most kv heads, of qf_kv4_attention. */
+#define QF_KV4_MAX_REQS 65535
 /* Longest packed row tile of the split attention: query tokens of a request * (H / H_kv). */
 #define QF_KV4_MAX_ROWS 64
 
@@ -137,7 +139,8 @@ typedef struct qf_kv4_attention_args {
  * sums are fp32; the cache's values are exact in the products, the softmax weights are rounded to bf16 before they multiply
  * V; the output is rounded once to bf16.
  * Lengths are kept inside the tables (0 <= seq_lens <= max_blocks * page_size, 0 <= cu_q <= num_tokens, at most q_len tokens
- * a request), block ids inside the cache.  out may be query itself.  num_heads % num_kv_heads == 0, max_blocks * page_size <= 2^31 - 64.
+ * a request), block ids inside the cache.  out may be query itself.  num_heads % num_kv_heads == 0, num_heads / num_kv_heads * q_len < 2^30,
+ * max_blocks * page_size <= 2^31 - 64, at most QF_KV4_MAX_REQS requests and kv heads.
  * Workspace: qf_kv4_attention_workspace_bytes(args); it needs no clearing and is free again when the last launch ends; calls
  * that may run at the same time need distinct ones (16-byte aligned). */
 int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);

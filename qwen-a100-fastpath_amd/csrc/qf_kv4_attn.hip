@@ -1214,7 +1214,8 @@ Plan plan_of(const qf_kv4_attention_args& u) {
 bool sizes_fit(const qf_kv4_attention_args& u) {
   return u.num_reqs >= 1 && u.q_len >= 1 && u.num_heads >= 1 && u.num_kv_heads >= 1 && u.num_heads % u.num_kv_heads == 0 &&
          (u.head_size == 64 || u.head_size == 128 || u.head_size == 256) &&
-         (int64_t)u.q_len * (u.num_heads / u.num_kv_heads) <= 0x3fffffff && u.num_kv_heads <= 65535 && u.num_reqs <= 65535;
+         (int64_t)u.q_len * (u.num_heads / u.num_kv_heads) <= 0x3fffffff && u.num_kv_heads <= QF_KV4_MAX_REQS &&
+         u.num_reqs <= QF_KV4_MAX_REQS;
 }
 
 constexpr int kAloneLds = 82 * 1024;  // of 160 KiB

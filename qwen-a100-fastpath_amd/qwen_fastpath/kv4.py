@@ -62,7 +62,7 @@ def kv4_attention(query: torch.Tensor, cache: torch.Tensor, seq_lens: torch.Tens
     [T, H, D]; cache as kv4_cache's; seq_lens int32 [B]; block_table int32 [>= B, most pages].  Either q_len: every request has
     q_len tokens (token b * q_len + i), or cu_q int32 [B + 1], the first token of each request (StepTables.cu_q), with
     max_q, the most tokens a request may have.  Rows behind the last request's tokens are not written (out: as they were).
-    out may be query itself.
+    out may be query itself.  At most 65535 requests.
     Lengths are kept inside the tables and block ids inside the cache.  Sums and the softmax are fp32; its weights are
     rounded to bf16 before they multiply the values, the output once."""
     if (q_len is None) == (cu_q is None) or (cu_q is None) != (max_q is None):
