@@ -139,8 +139,8 @@ typedef struct qf_kv4_attention_args {
  * sums are fp32; the cache's values are exact in the products, the softmax weights are rounded to bf16 before they multiply
  * V; the output is rounded once to bf16.
  * Lengths are kept inside the tables (0 <= seq_lens <= max_blocks * page_size, 0 <= cu_q <= num_tokens, at most q_len tokens
- * a request), block ids inside the cache.  out may be query itself.  num_heads % num_kv_heads == 0, num_heads / num_kv_heads * q_len < 2^30,
- * max_blocks * page_size <= 2^31 - 64, at most QF_KV4_MAX_REQS requests and kv heads.
+ * a request), block ids inside the cache.  out may be query itself.  num_heads % num_kv_heads == 0, num_heads / num_kv_heads *
+ * q_len < 2^30, max_blocks * page_size <= 2^31 - 64, at most QF_KV4_MAX_REQS requests and kv heads.
  * Workspace: qf_kv4_attention_workspace_bytes(args); it needs no clearing and is free again when the last launch ends; calls
  * that may run at the same time need distinct ones (16-byte aligned). */
 int qf_kv4_attention(const qf_kv4_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
